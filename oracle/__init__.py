@@ -37,10 +37,15 @@ REF_ROOT = Path(os.environ.get("ELIPS_REF_ROOT", str(HERE.parent.parent / "refer
 METRIC = {"cosine": 0, "euclidean": 1, "dot_product": 2}
 
 
+def _ref_sources() -> bool:
+    """Whether REF_ROOT holds the reference's sources (an empty folder does not)."""
+    return (REF_ROOT / "src" / "Metrics.cpp").exists()
+
+
 def build(ref: bool = True) -> None:
     """Builds liboracle.so and, when the reference sources are present, _ref."""
     subprocess.run(["make", "-s", "-C", str(HERE)], check=True)
-    if ref and REF_ROOT.exists():
+    if ref and _ref_sources():
         targets = ["ref", "ref_b200"] if PRODUCT_SO.exists() else ["ref"]
         subprocess.run(["make", "-s", "-j8", "-C", str(HERE), *targets, f"REF_ROOT={REF_ROOT}"], check=True)
 
@@ -65,7 +70,7 @@ def orc() -> ctypes.CDLL:
 
 
 def ref_available() -> bool:
-    return REF_SO.exists() or REF_ROOT.exists()
+    return REF_SO.exists() or _ref_sources()
 
 
 def _declare(lib: ctypes.CDLL) -> ctypes.CDLL:
