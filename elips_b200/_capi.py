@@ -38,6 +38,19 @@ CODEC_PQ = 1
 CODEC_OPQ = 2
 CODEC_SQ8 = 3
 
+
+class Cache(ctypes.Structure):
+    """elips_b200_cache."""
+    _fields_ = [("codes", c_void_p), ("scales", c_void_p), ("parts", c_int64), ("pages", c_int64),
+                ("page_size", c_int64), ("heads", c_int64), ("dim", c_int64), ("code_strides", c_int64 * 4),
+                ("scale_strides", c_int64 * 4)]
+
+
+class Rows(ctypes.Structure):
+    """elips_b200_rows."""
+    _fields_ = [("data", c_void_p), ("stride_row", c_int64), ("stride_head", c_int64)]
+
+
 # (name, restype, argtypes) for every entry point in include/elips_b200.h.
 SIGNATURES = [
     ("elips_b200_status_string", c_char_p, [c_int]),
@@ -141,6 +154,18 @@ SIGNATURES = [
     ("elips_b200_ivfflat_search_device", c_int,
      [c_void_p, c_void_p, c_size_t, c_size_t, c_void_p, c_void_p, c_void_p]),
     ("elips_b200_ivfflat_destroy", c_int, [c_void_p]),
+    ("elips_b200_quantize_rows", c_int,
+     [c_int, c_void_p, c_int, c_size_t, c_size_t, c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
+    ("elips_b200_gemm_int8", c_int,
+     [c_int, c_void_p, c_size_t, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p, c_int, c_size_t, c_size_t,
+      c_size_t, c_void_p, c_int, c_size_t, c_void_p]),
+    ("elips_b200_linear_int8", c_int,
+     [c_int, c_void_p, c_int, c_int64, c_void_p, c_size_t, c_void_p, c_void_p, c_int, c_size_t, c_size_t, c_size_t,
+      c_void_p, c_int, c_size_t, c_void_p]),
+    ("elips_b200_cache_write", c_int, [c_int, POINTER(Cache), POINTER(Rows), c_int, c_size_t, c_void_p, c_int, c_void_p]),
+    ("elips_b200_cache_read", c_int,
+     [c_int, POINTER(Cache), c_void_p, c_int, c_int64, c_size_t, c_size_t, c_void_p, c_int, c_size_t, POINTER(Rows),
+      c_int, c_int, c_void_p]),
     ("elips_b200_profiler_enable", c_int, [c_int]),
     ("elips_b200_profiler_stats", c_int,
      [c_char_p, POINTER(ctypes.c_uint64), POINTER(ctypes.c_double), POINTER(ctypes.c_uint64)]),

@@ -1,0 +1,309 @@
+// 8-bit row operators: quantise rows, multiply int8 matrices with a scale per
+// row and channel, write rows into the pages of a cache and read them back.
+// Kernels in int8_kernels.cuh; the C ABI at the end of this file.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <string>
+
+#include "../../include/elips_b200.h"
+#include "capi_util.cuh"
+#include "engine.cuh"
+#include "int8_kernels.cuh"
+#include "profiler.cuh"
+
+namespace eb {
+namespace {
+
+void launch_ok(const char* what) { check_cuda(cudaGetLastError(), ELIPS_B200_KERNEL_LAUNCH_FAILED, what); }
+
+[[noreturn]] void bad(const std::string& what) { fail(ELIPS_B200_INVALID_ARGUMENT, what); }
+
+uint32_t blocks_for(uint64_t items, uint32_t per_block) {
+    const uint64_t b = (items + per_block - 1) / per_block;
+    if (b > 0x7FFFFFFFull) bad("too many rows in one call");
+    return static_cast<uint32_t>(b);
+}
+
+constexpr size_t kMaxDim = size_t{1} << 24;
+constexpr size_t kMaxRows = 0x7FFFFFF0ull;
+// Largest k whose sum of products of int8 values (at most 2^14 each) stays
+// below 2^31.
+constexpr size_t kMaxK = 131071;
+
+void check_float_type(int type) {
+    if (type != ELIPS_B200_PRECISION_FP32 && type != ELIPS_B200_PRECISION_FP16 && type != ELIPS_B200_PRECISION_BF16)
+        bad("element types are fp32, fp16 and bf16");
+}
+
+void check_rows(size_t n, size_t d, int type) {
+    check_float_type(type);
+    if (d == 0 || d > kMaxDim) bad("row width must be in [1, 2^24]");
+    if (n > kMaxRows) bad("too many rows in one call");
+}
+
+// fn is called with a value of the element type that `type` names.
+template <class Fn>
+void with_float_type(int type, Fn&& fn) {
+    switch (type) {
+        case ELIPS_B200_PRECISION_FP32: fn(float{}); return;
+        case ELIPS_B200_PRECISION_FP16: fn(__half{}); return;
+        case ELIPS_B200_PRECISION_BF16: fn(__nv_bfloat16{}); return;
+        default: check_float_type(type);
+    }
+}
+
+void launch_quantize(int type, const QuantParams& p, bool claimed, cudaStream_t stream) {
+    const uint64_t rows = static_cast<uint64_t>(p.t) * p.parts * p.heads;
+    with_float_type(type, [&](auto tag) {
+        quantize_rows_kernel<decltype(tag)><<<blocks_for(rows, 8), 256, 0, stream>>>(p, claimed ? 1 : 0);
+    });
+    launch_ok("row quantisation launch");
+}
+
+void quantize_rows(const void* x, int type, size_t n, size_t d, int64_t x_pitch, int8_t* codes, size_t code_pitch,
+                   float* scales, cudaStream_t stream) {
+    if (n == 0) return;
+    QuantParams p{};
+    p.x[0] = x;
+    p.x_stride_t[0] = x_pitch;
+    p.codes = codes;
+    p.scales = scales;
+    p.code_page = static_cast<int64_t>(code_pitch);
+    p.scale_page = 1;
+    p.t = static_cast<uint32_t>(n);
+    p.parts = p.heads = p.page = 1;
+    p.d = static_cast<uint32_t>(d);
+    p.num_slots = static_cast<int64_t>(n);
+    Profiler::Scope prof("quantize_rows", stream, n);
+    launch_quantize(type, p, false, stream);
+}
+
+void check_cache(const elips_b200_cache& c) {
+    if (c.parts < 1 || c.parts > 2) bad("a cache has one or two parts");
+    if (c.pages < 0 || c.page_size < 1 || c.heads < 1 || c.dim < 1) bad("cache sizes must be positive");
+    if (c.dim > static_cast<int64_t>(kMaxDim) || c.heads > (1 << 20)) bad("cache rows too wide");
+    if (c.page_size > 0x7FFFFFFFll || c.pages > 0x7FFFFFFFll || c.pages * c.page_size > 0x7FFFFFFFll)
+        bad("a cache holds fewer than 2^31 slots");
+    if (c.pages > 0 && (c.codes == nullptr || c.scales == nullptr)) bad("cache without storage");
+}
+
+void check_cache_rows(const elips_b200_cache& c, const elips_b200_rows* rows, int type, size_t t) {
+    check_float_type(type);
+    if (t > kMaxRows) bad("too many rows in one call");
+    for (int64_t i = 0; t > 0 && i < c.parts; ++i)
+        if (rows[i].data == nullptr) bad("rows missing");
+}
+
+template <class P>
+void set_cache(P& p, const elips_b200_cache& c) {
+    p.codes = static_cast<int8_t*>(c.codes);
+    p.scales = c.scales;
+    p.code_part = c.code_strides[0];
+    p.code_page = c.code_strides[1];
+    p.code_row = c.code_strides[2];
+    p.code_head = c.code_strides[3];
+    p.scale_part = c.scale_strides[0];
+    p.scale_page = c.scale_strides[1];
+    p.scale_row = c.scale_strides[2];
+    p.scale_head = c.scale_strides[3];
+    p.parts = static_cast<uint32_t>(c.parts);
+    p.heads = static_cast<uint32_t>(c.heads);
+    p.page = static_cast<uint32_t>(c.page_size);
+    p.d = static_cast<uint32_t>(c.dim);
+}
+
+void cache_write(const elips_b200_cache& c, const elips_b200_rows* rows, int type, size_t t, const void* slots,
+                 int slots64, cudaStream_t stream) {
+    if (t == 0 || c.pages == 0) return;
+    QuantParams p{};
+    set_cache(p, c);
+    for (int64_t i = 0; i < c.parts; ++i) {
+        p.x[i] = rows[i].data;
+        p.x_stride_t[i] = rows[i].stride_row;
+        p.x_stride_h[i] = rows[i].stride_head;
+    }
+    p.slots = slots;
+    p.slots64 = slots64;
+    p.t = static_cast<uint32_t>(t);
+    p.num_slots = c.pages * c.page_size;
+    const uint64_t groups = static_cast<uint64_t>(t) * p.parts * p.heads;
+    const bool claimed = t > 1;
+    if (claimed) {
+        for (int clear = 1; clear >= 0; --clear) {
+            Profiler::Scope prof("cache_claim", stream, groups);
+            cache_claim_kernel<<<blocks_for(groups, 256), 256, 0, stream>>>(p, clear);
+            launch_ok("cache claim launch");
+        }
+    }
+    Profiler::Scope prof("cache_write", stream, groups);
+    launch_quantize(type, p, claimed, stream);
+}
+
+void cache_read(const elips_b200_cache& c, const void* table, int table64, int64_t table_stride, size_t sequences,
+                size_t table_width, const void* offsets, int offsets64, size_t total, const elips_b200_rows* out,
+                int type, int zero_behind, cudaStream_t stream) {
+    if (total == 0) return;
+    ReadParams p{};
+    set_cache(p, c);
+    for (int64_t i = 0; i < c.parts; ++i) {
+        p.out[i] = const_cast<void*>(out[i].data);
+        p.out_stride_t[i] = out[i].stride_row;
+        p.out_stride_h[i] = out[i].stride_head;
+    }
+    p.table = table;
+    p.table64 = table64;
+    p.table_stride = table_stride;
+    p.offsets = offsets;
+    p.offsets64 = offsets64;
+    p.sequences = static_cast<uint32_t>(sequences);
+    p.table_width = static_cast<uint32_t>(table_width);
+    p.pages = static_cast<uint32_t>(c.pages);
+    p.total = static_cast<uint32_t>(total);
+    p.zero_behind = zero_behind;
+    const uint64_t groups = static_cast<uint64_t>(total) * p.parts * p.heads;
+    Profiler::Scope prof("cache_read", stream, groups);
+    with_float_type(type, [&](auto tag) {
+        cache_read_kernel<decltype(tag)><<<blocks_for(groups, 8), 256, 0, stream>>>(p);
+    });
+    launch_ok("cache read launch");
+}
+
+void gemm_int8(const GemmParams& p, int out_type, cudaStream_t stream) {
+    if (p.m == 0 || p.n == 0) return;
+    const dim3 grid(blocks_for(p.n, 64), blocks_for(p.m, 64));
+    if (grid.y > 65535) bad("too many rows in one call");
+    Profiler::Scope prof("gemm_int8", stream, static_cast<uint64_t>(p.m) * p.n);
+    with_float_type(out_type, [&](auto tag) {
+        gemm_int8_tile_kernel<decltype(tag)><<<grid, 256, 0, stream>>>(p);
+    });
+    launch_ok("int8 product launch");
+}
+
+void check_gemm(size_t m, size_t n, size_t k, size_t b_pitch, const void* bias, int bias_type, int out_type,
+                size_t out_pitch) {
+    check_float_type(out_type);
+    if (bias != nullptr) check_float_type(bias_type);
+    if (m > kMaxRows || n > kMaxRows) bad("matrix sizes must be below 2^31");
+    if (k > kMaxK) bad("k must be below 2^17: the int32 sum could overflow");
+    if (b_pitch < k || out_pitch < n) bad("neighbouring matrix rows overlap");
+}
+
+GemmParams gemm_params(const int8_t* a, size_t a_pitch, const float* a_scales, const int8_t* b, size_t b_pitch,
+                       const float* b_scales, const void* bias, int bias_type, size_t m, size_t n, size_t k, void* out,
+                       size_t out_pitch) {
+    GemmParams p{};
+    p.a = a;
+    p.b = b;
+    p.a_pitch = static_cast<int64_t>(a_pitch);
+    p.b_pitch = static_cast<int64_t>(b_pitch);
+    p.a_scales = a_scales;
+    p.b_scales = b_scales;
+    p.bias = bias;
+    p.bias_type = bias_type;
+    p.out = out;
+    p.out_pitch = static_cast<int64_t>(out_pitch);
+    p.m = static_cast<uint32_t>(m);
+    p.n = static_cast<uint32_t>(n);
+    p.k = static_cast<uint32_t>(k);
+    return p;
+}
+
+void linear_int8(const void* x, int x_type, int64_t x_pitch, const int8_t* b, size_t b_pitch, const float* b_scales,
+                 const void* bias, int bias_type, size_t m, size_t n, size_t k, void* out, int out_type,
+                 size_t out_pitch, cudaStream_t stream) {
+    if (m == 0 || n == 0) return;
+    const size_t pitch = (k + 15) / 16 * 16;
+    const size_t code_bytes = (m * pitch + 255) / 256 * 256;
+    StreamScratch s(code_bytes + m * sizeof(float), stream);
+    int8_t* codes = reinterpret_cast<int8_t*>(s.get());
+    float* scales = reinterpret_cast<float*>(s.get() + code_bytes);
+    quantize_rows(x, x_type, m, k, x_pitch, codes, pitch, scales, stream);
+    gemm_int8(gemm_params(codes, pitch, scales, b, b_pitch, b_scales, bias, bias_type, m, n, k, out, out_pitch),
+              out_type, stream);
+}
+
+cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
+
+}  // namespace
+}  // namespace eb
+
+using eb::guarded;
+
+extern "C" {
+
+int elips_b200_quantize_rows(int device, const void* x, int type, size_t n, size_t d, int64_t x_stride, int8_t* codes,
+                             size_t code_stride, float* scales, void* stream) {
+    if (n > 0 && (x == nullptr || codes == nullptr || scales == nullptr)) return ELIPS_B200_INVALID_ARGUMENT;
+    return guarded([&] {
+        eb::check_rows(n, d, type);
+        if (code_stride < d) eb::bad("codes of neighbouring rows overlap");
+        eb::DeviceGuard g(device);
+        eb::device_props(device);
+        eb::quantize_rows(x, type, n, d, x_stride, codes, code_stride, scales, eb::as_stream(stream));
+    });
+}
+
+int elips_b200_gemm_int8(int device, const int8_t* a, size_t a_stride, const float* a_scales, const int8_t* b,
+                         size_t b_stride, const float* b_scales, const void* bias, int bias_type, size_t m, size_t n,
+                         size_t k, void* out, int out_type, size_t out_stride, void* stream) {
+    if (m > 0 && n > 0 && ((k > 0 && (a == nullptr || b == nullptr)) || a_scales == nullptr || b_scales == nullptr || out == nullptr))
+        return ELIPS_B200_INVALID_ARGUMENT;
+    return guarded([&] {
+        eb::check_gemm(m, n, k, b_stride, bias, bias_type, out_type, out_stride);
+        if (a_stride < k) eb::bad("neighbouring matrix rows overlap");
+        eb::DeviceGuard g(device);
+        eb::device_props(device);
+        eb::gemm_int8(eb::gemm_params(a, a_stride, a_scales, b, b_stride, b_scales, bias, bias_type, m, n, k, out,
+                                      out_stride),
+                      out_type, eb::as_stream(stream));
+    });
+}
+
+int elips_b200_linear_int8(int device, const void* x, int x_type, int64_t x_stride, const int8_t* w, size_t w_stride,
+                           const float* w_scales, const void* bias, int bias_type, size_t m, size_t n, size_t k,
+                           void* out, int out_type, size_t out_stride, void* stream) {
+    if (m > 0 && n > 0 && (x == nullptr || w == nullptr || w_scales == nullptr || out == nullptr))
+        return ELIPS_B200_INVALID_ARGUMENT;
+    return guarded([&] {
+        eb::check_gemm(m, n, k, w_stride, bias, bias_type, out_type, out_stride);
+        eb::check_rows(m, k, x_type);
+        eb::DeviceGuard g(device);
+        eb::device_props(device);
+        eb::linear_int8(x, x_type, x_stride, w, w_stride, w_scales, bias, bias_type, m, n, k, out, out_type,
+                        out_stride, eb::as_stream(stream));
+    });
+}
+
+int elips_b200_cache_write(int device, const elips_b200_cache* cache, const elips_b200_rows* rows, int type, size_t t,
+                           const void* slots, int slots_64bit, void* stream) {
+    if (cache == nullptr || (t > 0 && rows == nullptr)) return ELIPS_B200_INVALID_ARGUMENT;
+    return guarded([&] {
+        eb::check_cache(*cache);
+        eb::check_cache_rows(*cache, rows, type, t);
+        if (t > 0 && slots == nullptr) eb::bad("slots missing");
+        eb::DeviceGuard g(device);
+        eb::device_props(device);
+        eb::cache_write(*cache, rows, type, t, slots, slots_64bit, eb::as_stream(stream));
+    });
+}
+
+int elips_b200_cache_read(int device, const elips_b200_cache* cache, const void* page_table, int table_64bit,
+                          int64_t table_stride, size_t sequences, size_t table_width, const void* offsets,
+                          int offsets_64bit, size_t total, const elips_b200_rows* out, int type, int zero_behind,
+                          void* stream) {
+    if (cache == nullptr || (total > 0 && out == nullptr)) return ELIPS_B200_INVALID_ARGUMENT;
+    return guarded([&] {
+        eb::check_cache(*cache);
+        eb::check_cache_rows(*cache, out, type, total);
+        if (sequences > eb::kMaxRows || table_width > eb::kMaxRows) eb::bad("page table too large");
+        if (total > 0 && sequences > 0 && offsets == nullptr) eb::bad("offsets missing");
+        if (total > 0 && sequences > 0 && table_width > 0 && page_table == nullptr) eb::bad("page table missing");
+        eb::DeviceGuard g(device);
+        eb::device_props(device);
+        eb::cache_read(*cache, page_table, table_64bit, table_stride, sequences, table_width, offsets, offsets_64bit,
+                       total, out, type, zero_behind, eb::as_stream(stream));
+    });
+}
+
+}  // extern "C"

@@ -572,6 +572,82 @@ ELIPS_B200_API int elips_b200_ivfpq_train(int device, int metric, const float* r
                                           uint32_t* assignments_out, float* codebook_out,
                                           uint8_t* codes_out, int pointers_on_device, void* stream);
 
+/* ------------------------------------------------- 8-bit row operators */
+/* No counterpart in the reference, whose scalar quantiser has one scale per
+ * dimension and gives distances, not products: operators on rows held as int8
+ * codes with one fp32 scale per row, for the models that make and use the
+ * vectors an index stores. A row x is held as s = fl32(max |x_j| / 127) (at
+ * most the largest s whose 127-fold is finite) and
+ * q_j = the integer nearest to x_j / s (ties to even). A row whose s would be
+ * below 2^-126 is held as zeros with s = 0; a row with an infinity or a NaN
+ * has codes 0 and a scale that is inf or NaN, so it reads back as NaN.
+ * Element types are ELIPS_B200_PRECISION_FP32, _FP16 or _BF16. All pointers
+ * are DEVICE pointers on `device`, every call is asynchronous on `stream` and
+ * can be captured into a CUDA graph. Strides are in elements; the innermost
+ * axis has stride 1. No sizes are too small: zero rows launch nothing. */
+
+/* codes[i * code_stride + j] and scales[i] of n rows of d values (d in
+ * [1, 2^24]) at x + i * x_stride. A code_stride that is a multiple of 16 and
+ * codes on 16 bytes let elips_b200_gemm_int8 read them without a copy. */
+ELIPS_B200_API int elips_b200_quantize_rows(int device, const void* x, int type, size_t n, size_t d, int64_t x_stride,
+                                            int8_t* codes, size_t code_stride, float* scales, void* stream);
+
+/* out[i][j] = (sum_l a[i][l] * b[j][l]) * a_scales[i] * b_scales[j] + bias[j],
+ * rounded once to out_type: a is m x k, b is n x k (a layer's weight, or the
+ * stored rows that queries are scored against), both int8 and row-major, the
+ * sum exact in int32 (k < 2^17). bias may be NULL, its type is bias_type. */
+ELIPS_B200_API int elips_b200_gemm_int8(int device, const int8_t* a, size_t a_stride, const float* a_scales,
+                                        const int8_t* b, size_t b_stride, const float* b_scales, const void* bias,
+                                        int bias_type, size_t m, size_t n, size_t k, void* out, int out_type,
+                                        size_t out_stride, void* stream);
+
+/* elips_b200_gemm_int8 over rows of x quantised on the way (one scale per row
+ * of x, as elips_b200_quantize_rows gives): a layer whose weight is int8.
+ * k >= 1. */
+ELIPS_B200_API int elips_b200_linear_int8(int device, const void* x, int x_type, int64_t x_stride, const int8_t* w,
+                                          size_t w_stride, const float* w_scales, const void* bias, int bias_type,
+                                          size_t m, size_t n, size_t k, void* out, int out_type, size_t out_stride,
+                                          void* stream);
+
+/* A paged cache of quantised rows: codes [parts][pages][page_size][heads][dim]
+ * and scales [parts][pages][page_size][heads] with the given strides (the
+ * innermost one of codes is 1). One part holds one kind of row (vectors), two
+ * hold keys and values. Slot s is row s % page_size of page s / page_size;
+ * fewer than 2^31 slots. */
+typedef struct {
+    void* codes;
+    float* scales;
+    int64_t parts, pages, page_size, heads, dim;
+    int64_t code_strides[4];
+    int64_t scale_strides[4];
+} elips_b200_cache;
+
+/* Rows [t][heads][dim] of one part, innermost stride 1. */
+typedef struct {
+    const void* data;
+    int64_t stride_row, stride_head;
+} elips_b200_rows;
+
+/* Quantises rows[part][i] into slot slots[i] (int32, or int64 where
+ * slots_64bit) for i < t, one scale per row and head. A slot below 0 or past
+ * the last one is skipped; of a slot given twice the last row is kept. rows:
+ * one entry per part. Calls on different streams may run at once on disjoint
+ * slots. */
+ELIPS_B200_API int elips_b200_cache_write(int device, const elips_b200_cache* cache, const elips_b200_rows* rows,
+                                          int type, size_t t, const void* slots, int slots_64bit, void* stream);
+
+/* Reads sequences back into packed rows: output row r of each part belongs to
+ * the sequence b with offsets[b] <= r < offsets[b + 1] (offsets ascending,
+ * sequences + 1 entries) and is position i = r - offsets[b] of it, in page
+ * page_table[b * table_stride + i / page_size]. A page that is no page of the
+ * cache, or past the table's width, reads as zeros. Rows from
+ * offsets[sequences] to `total` are zeroed where zero_behind, else left as
+ * they are. */
+ELIPS_B200_API int elips_b200_cache_read(int device, const elips_b200_cache* cache, const void* page_table,
+                                         int table_64bit, int64_t table_stride, size_t sequences, size_t table_width,
+                                         const void* offsets, int offsets_64bit, size_t total,
+                                         const elips_b200_rows* out, int type, int zero_behind, void* stream);
+
 /* ------------------------------------------------------------ profiling */
 /* Device-side counterpart of GpuProfiler (src/gpu_engine/GpuProfiler.cpp:
  * 5-23) and GpuConfig::enable_profiling (GpuConfig.hpp:83): while enabled,

@@ -1,0 +1,135 @@
+"""Arguments the 8-bit row operators refuse, in Python and at the C ABI. No GPU is needed: every check of sizes,
+types and strides comes before the device is touched."""
+import ctypes
+
+import pytest
+import torch
+
+from elips_b200 import DimensionMismatch, _capi
+from elips_b200 import int8 as ops
+
+
+def codes(m, k):
+    return torch.zeros((m, k), dtype=torch.int8)
+
+
+ONE = torch.ones(4)
+
+
+@pytest.mark.parametrize("call,error", [
+    (lambda: ops.quantize_rows(torch.zeros(4)), DimensionMismatch),
+    (lambda: ops.quantize_rows(torch.zeros((4, 0))), DimensionMismatch),
+    (lambda: ops.quantize_rows(torch.zeros((4, 4), dtype=torch.float64)), ValueError),
+    (lambda: ops.quantize_rows(torch.zeros((4, 8)).t()), ValueError),
+    (lambda: ops.quantize_rows(torch.zeros((4, 8), requires_grad=True)), ValueError),
+    (lambda: ops.quantize_rows(torch.zeros((4, 8))), ValueError),                         # not on a CUDA device
+    (lambda: ops.gemm_int8(codes(4, 8), codes(4, 9), ONE, ONE), DimensionMismatch),
+    (lambda: ops.gemm_int8(codes(4, 8), codes(4, 8), ONE[:3], ONE), DimensionMismatch),
+    (lambda: ops.gemm_int8(codes(4, 8), codes(4, 8), ONE, torch.ones(8)[::2]), ValueError),
+    (lambda: ops.gemm_int8(codes(4, 8), codes(4, 8), ONE, ONE.double()), ValueError),
+    (lambda: ops.gemm_int8(codes(4, 8).float(), codes(4, 8), ONE, ONE), ValueError),
+    (lambda: ops.gemm_int8(codes(4, 8), codes(8, 4).t(), ONE, ONE), ValueError),
+    (lambda: ops.gemm_int8(codes(1, 8).expand(4, 8), codes(4, 8), ONE, ONE), ValueError),
+    (lambda: ops.gemm_int8(codes(4, 8), codes(4, 8), ONE, ONE, bias=torch.ones(5)), DimensionMismatch),
+    (lambda: ops.gemm_int8(codes(4, 8), codes(4, 8), ONE, ONE, bias=torch.ones(4, dtype=torch.int32)), ValueError),
+    (lambda: ops.gemm_int8(codes(4, 8), codes(4, 8), ONE, ONE, out_dtype=torch.int32), ValueError),
+    (lambda: ops.gemm_int8(codes(4, 8), codes(4, 8), ONE, ONE, out=torch.zeros((4, 5))), DimensionMismatch),
+    (lambda: ops.gemm_int8(codes(4, 8), codes(4, 8), ONE, ONE, out=torch.zeros((1, 4)).expand(4, 4)), ValueError),
+    (lambda: ops.gemm_int8(codes(4, 8), codes(4, 8), ONE.clone().requires_grad_(), ONE), ValueError),
+    (lambda: ops.gemm_int8(codes(4, 8), codes(4, 8), ONE, ONE), ValueError),              # not on a CUDA device
+    (lambda: ops.linear_int8(torch.zeros((4, 8), requires_grad=True), codes(4, 8), ONE), ValueError),
+    (lambda: ops.linear_int8(torch.zeros((4, 0)), codes(4, 0), ONE), DimensionMismatch),
+    (lambda: ops.linear_int8(torch.zeros((4, 7)), codes(4, 8), ONE), DimensionMismatch),
+    (lambda: ops.linear_int8(torch.zeros((4, 8)), codes(4, 8), ONE), ValueError),         # not on a CUDA device
+])
+def test_products_and_rows_refused(call, error):
+    with pytest.raises(error):
+        call()
+
+
+def cache(parts=2, pages=3, page=4, heads=2, dim=8):
+    return torch.zeros((parts, pages, page, heads, dim), dtype=torch.int8), torch.zeros((parts, pages, page, heads))
+
+
+def rows(t=2, heads=2, dim=8, parts=2):
+    return tuple(torch.zeros((t, heads, dim)) for _ in range(parts))
+
+
+SLOTS = torch.zeros(2, dtype=torch.int64)
+TABLE = torch.zeros((2, 3), dtype=torch.int32)
+OFFSETS = torch.tensor([0, 1, 2])
+
+
+@pytest.mark.parametrize("call,error", [
+    (lambda c, s: ops.cache_write(c, s, rows(parts=1), SLOTS), DimensionMismatch),
+    (lambda c, s: ops.cache_write(c, s, rows(t=3), SLOTS), DimensionMismatch),
+    (lambda c, s: ops.cache_write(c, s, rows(dim=7), SLOTS), DimensionMismatch),
+    (lambda c, s: ops.cache_write(c, s, rows(), SLOTS.float()), ValueError),
+    (lambda c, s: ops.cache_write(c, s, rows(), torch.zeros(4, dtype=torch.int64)[::2]), DimensionMismatch),
+    (lambda c, s: ops.cache_write(c.int(), s, rows(), SLOTS), ValueError),
+    (lambda c, s: ops.cache_write(c, s[:, :2], rows(), SLOTS), DimensionMismatch),
+    (lambda c, s: ops.cache_write(c[:1].expand(2, 3, 4, 2, 8), s, rows(), SLOTS), ValueError),
+    (lambda c, s: ops.cache_write(torch.cat([c, c]), torch.cat([s, s]), rows(parts=4), SLOTS), DimensionMismatch),
+    (lambda c, s: ops.cache_write(c, s, (rows()[0], rows()[1].half()), SLOTS), ValueError),
+    (lambda c, s: ops.cache_write(c, s, tuple(x.requires_grad_() for x in rows()), SLOTS), ValueError),
+    (lambda c, s: ops.cache_write(c, s, rows(), SLOTS), ValueError),                      # not on a CUDA device
+    (lambda c, s: ops.cache_read(c, s, TABLE, OFFSETS[:2], 2), DimensionMismatch),
+    (lambda c, s: ops.cache_read(c, s, TABLE.float(), OFFSETS, 2), ValueError),
+    (lambda c, s: ops.cache_read(c, s, torch.zeros((3, 2), dtype=torch.int32).t(), OFFSETS, 2), ValueError),
+    (lambda c, s: ops.cache_read(c, s, TABLE, OFFSETS, -1), DimensionMismatch),
+    (lambda c, s: ops.cache_read(c, s, TABLE, OFFSETS, 2, dtype=torch.int8), ValueError),
+    (lambda c, s: ops.cache_read(c, s, TABLE, OFFSETS, 2, out=rows(parts=1)), DimensionMismatch),
+    (lambda c, s: ops.cache_read(c, s, TABLE, OFFSETS, 3, out=rows()), DimensionMismatch),
+    (lambda c, s: ops.cache_read(c, s, TABLE, OFFSETS, 2, out=tuple(x[:1].expand(2, 2, 8) for x in rows())), ValueError),
+    (lambda c, s: ops.cache_read(c, s, TABLE, OFFSETS, 2), ValueError),                   # not on a CUDA device
+])
+def test_cache_refused(call, error):
+    with pytest.raises(error):
+        call(*cache())
+
+
+def test_c_entry_points_refuse_before_the_device():
+    lib, bad = _capi.LIB, _capi.INVALID_ARGUMENT
+    f32, bf16, int8 = _capi.PRECISION_FP32, _capi.PRECISION_BF16, _capi.PRECISION_INT8
+    p = 16  # stands for a device address: none of these calls reaches the device
+    assert lib.elips_b200_quantize_rows(0, None, f32, 1, 8, 8, p, 16, p, None) == bad
+    assert lib.elips_b200_quantize_rows(0, p, int8, 1, 8, 8, p, 16, p, None) == bad
+    assert lib.elips_b200_quantize_rows(0, p, f32, 1, 0, 8, p, 16, p, None) == bad
+    assert lib.elips_b200_quantize_rows(0, p, f32, 1, (1 << 24) + 1, 8, p, 1 << 25, p, None) == bad
+    assert lib.elips_b200_quantize_rows(0, p, f32, 2, 8, 8, p, 7, p, None) == bad
+
+    def gemm(a=p, a_stride=16, m=4, n=4, k=16, b_stride=16, bias=None, bias_type=0, out_type=f32, out_stride=4):
+        return lib.elips_b200_gemm_int8(0, a, a_stride, p, p, b_stride, p, bias, bias_type, m, n, k, p, out_type,
+                                        out_stride, None)
+    assert gemm(a=None) == bad
+    assert gemm(a_stride=15) == bad
+    assert gemm(b_stride=15) == bad
+    assert gemm(out_stride=3) == bad
+    assert gemm(out_type=int8) == bad
+    assert gemm(bias=p, bias_type=9) == bad
+    assert gemm(k=1 << 17, a_stride=1 << 17, b_stride=1 << 17) == bad   # the int32 sum could pass 2^31
+    assert gemm(m=1 << 32) == bad
+    assert lib.elips_b200_linear_int8(0, p, int8, 16, p, 16, p, None, 0, 4, 4, 16, p, f32, 4, None) == bad
+    assert lib.elips_b200_linear_int8(0, p, f32, 16, p, 16, p, None, 0, 4, 4, 0, p, f32, 4, None) == bad
+
+    def described(**kw):
+        d = dict(codes=p, scales=p, parts=1, pages=3, page_size=4, heads=2, dim=8) | kw
+        return _capi.Cache(d["codes"], d["scales"], d["parts"], d["pages"], d["page_size"], d["heads"], d["dim"],
+                           (0, 64, 16, 8), (0, 8, 2, 1))
+    r = (_capi.Rows * 2)(_capi.Rows(p, 16, 8), _capi.Rows(None, 16, 8))
+    write = lambda c, t=2, type=bf16, slots=p: lib.elips_b200_cache_write(  # noqa: E731
+        0, None if c is None else ctypes.byref(c), r, type, t, slots, 1, None)
+    read = lambda c, total=2, type=bf16, table=p, offsets=p: lib.elips_b200_cache_read(  # noqa: E731
+        0, None if c is None else ctypes.byref(c), table, 0, 3, 2, 3, offsets, 0, total, r, type, 1, None)
+    for call in (write, read):
+        assert call(None) == bad
+        assert call(described(parts=3)) == bad
+        assert call(described(parts=2)) == bad            # the second part's rows are missing
+        assert call(described(dim=0)) == bad
+        assert call(described(page_size=0)) == bad
+        assert call(described(codes=None)) == bad
+        assert call(described(pages=1 << 30, page_size=2)) == bad
+        assert call(described(), type=int8) == bad
+    assert write(described(), slots=None) == bad
+    assert read(described(), table=None) == bad
+    assert read(described(), offsets=None) == bad
