@@ -148,11 +148,11 @@ void allow_dynamic_smem(const void* func, size_t bytes) {
 }
 
 CUtensorMap make_operand_map(const void* base, CUtensorMapDataType dtype, uint32_t elem_bytes,
-                             uint64_t cols, uint64_t rows, uint32_t box_rows) {
+                             uint64_t cols, uint64_t rows, uint32_t box_rows, uint64_t pitch_bytes) {
     CUtensorMap map;
     std::memset(&map, 0, sizeof(map));
     const cuuint64_t dims[2] = {cols, std::max<uint64_t>(rows, 1)};
-    const cuuint64_t strides[1] = {cols * elem_bytes};
+    const cuuint64_t strides[1] = {pitch_bytes != 0 ? pitch_bytes : cols * elem_bytes};
     const cuuint32_t box[2] = {128u / elem_bytes, box_rows};
     const cuuint32_t estr[2] = {1, 1};
     const CUresult r = tensor_map_encoder()(
@@ -1030,7 +1030,8 @@ int read_and_clear_device_error(int device) {
     const int zero = 0;
     check_cuda(cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int)), ELIPS_B200_TRANSFER_FAILED,
                "clear device error");
-    return code;
+    const int rows8 = take_int8_error(device);
+    return code != 0 ? code : rows8;
 }
 
 }  // namespace eb

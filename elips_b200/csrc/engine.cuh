@@ -87,9 +87,10 @@ private:
 };
 
 // Builds a 2-D tiled TMA descriptor over a row-major [rows x cols] matrix
-// with 128-byte swizzle and a {128 bytes, box_rows} box.
+// with 128-byte swizzle and a {128 bytes, box_rows} box. pitch_bytes: from one
+// row to the next (0: cols * elem_bytes).
 CUtensorMap make_operand_map(const void* base, CUtensorMapDataType dtype, uint32_t elem_bytes,
-                             uint64_t cols, uint64_t rows, uint32_t box_rows);
+                             uint64_t cols, uint64_t rows, uint32_t box_rows, uint64_t pitch_bytes = 0);
 
 // Partitioning of one exact search launch over `groups` MMA groups of `cg`
 // CTAs (1: single CTAs, 2: CTA pairs sharing each M = 256 MMA). grid counts
@@ -205,6 +206,9 @@ void merge_candidates(int device, const uint2* cand, uint32_t nq, uint32_t lists
                       uint32_t lists_last = 0, uint32_t len = 0);
 
 int read_and_clear_device_error(int device);
+// The error word of the 8-bit operators' kernels, read and cleared (no
+// synchronisation of its own).
+int take_int8_error(int device);
 // Launches a bounded wait that must expire after `budget` cycles and returns
 // the device error word it leaves (cleared again).
 int wait_selftest(int device, long long budget);

@@ -3,12 +3,14 @@
 // Kernels in int8_kernels.cuh; the C ABI at the end of this file.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <string>
 
 #include "../../include/elips_b200.h"
 #include "capi_util.cuh"
 #include "engine.cuh"
+#include "int8_gemm.cuh"
 #include "int8_kernels.cuh"
 #include "profiler.cuh"
 
@@ -169,15 +171,143 @@ void cache_read(const elips_b200_cache& c, const void* table, int table64, int64
     launch_ok("cache read launch");
 }
 
-void gemm_int8(const GemmParams& p, int out_type, cudaStream_t stream) {
-    if (p.m == 0 || p.n == 0) return;
-    const dim3 grid(blocks_for(p.n, 64), blocks_for(p.m, 64));
-    if (grid.y > 65535) bad("too many rows in one call");
-    Profiler::Scope prof("gemm_int8", stream, static_cast<uint64_t>(p.m) * p.n);
-    with_float_type(out_type, [&](auto tag) {
-        gemm_int8_tile_kernel<decltype(tag)><<<grid, 256, 0, stream>>>(p);
-    });
+uint32_t cdiv(uint64_t a, uint64_t b) { return static_cast<uint32_t>((a + b - 1) / b); }
+
+bool on_16(const void* ptr, int64_t pitch_bytes, uint32_t rows) {
+    return reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && (rows <= 1 || pitch_bytes % 16 == 0);
+}
+
+// What a tensor map needs of a pitch that no row uses.
+uint64_t map_pitch(int64_t pitch_bytes, uint64_t width_bytes, uint32_t rows) {
+    return rows > 1 ? static_cast<uint64_t>(pitch_bytes) : (width_bytes + 15) / 16 * 16;
+}
+
+CUtensorMap code_map(const int8_t* codes, int64_t pitch, uint32_t rows, uint32_t k, uint32_t box_rows) {
+    if (k == 0) return CUtensorMap{};  // nothing is loaded
+    return make_operand_map(codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, k, rows, box_rows, map_pitch(pitch, k, rows));
+}
+
+template <class T>
+void launch_dot(const GemmParams& p, int num_sms, cudaStream_t stream) {
+    // Warps that split k between them until every SM has sixteen.
+    const uint64_t groups = cdiv(p.n, kDotChannels);
+    uint32_t wk = 1;
+    while (wk < 8 && groups * wk < static_cast<uint64_t>(num_sms) * 16 && p.k > wk * 512u) wk *= 2;
+    const uint32_t blocks = blocks_for(groups * wk, 8);
+    if (p.m == 1) gemm_int8_dot_kernel<1, T><<<blocks, 256, 0, stream>>>(p, wk);
+    else if (p.m == 2) gemm_int8_dot_kernel<2, T><<<blocks, 256, 0, stream>>>(p, wk);
+    else if (p.m <= 4) gemm_int8_dot_kernel<4, T><<<blocks, 256, 0, stream>>>(p, wk);
+    else gemm_int8_dot_kernel<8, T><<<blocks, 256, 0, stream>>>(p, wk);
+}
+
+template <int BT, class T>
+void launch_wide(const GemmParams& p, int num_sms, cudaStream_t stream) {
+    constexpr uint32_t stage_bytes = (kWideChannels + BT) * kGemmStageK;
+    const uint32_t n_ct = cdiv(p.n, kWideChannels), n_rt = cdiv(p.m, BT);
+    if (n_ct > 65535 || n_rt > 65535) bad("too many rows in one call");
+    const uint32_t kblocks = cdiv(p.k, kGemmStageK);
+    const uint64_t tiles = static_cast<uint64_t>(n_ct) * n_rt;
+    uint32_t splits = 1;
+    while (splits < 8 && tiles * splits * 2 <= static_cast<uint64_t>(num_sms) * 2 && splits * 2 <= kblocks) splits *= 2;
+    const uint32_t per = std::max(1u, cdiv(kblocks, splits));
+    const uint32_t stages = std::min<uint32_t>(std::min<uint32_t>(kWideMaxStages, per), 196608u / stage_bytes);
+    const size_t smem = 1024 + std::max<size_t>(static_cast<size_t>(stages) * stage_bytes,
+                                                splits > 1 ? BT * kWideChannels * 4u : 0u);
+    const CUtensorMap mw = code_map(p.b, p.b_pitch, p.n, p.k, kWideChannels);
+    const CUtensorMap mx = code_map(p.a, p.a_pitch, p.m, p.k, BT);
+    allow_dynamic_smem(reinterpret_cast<const void*>(gemm_int8_wide_kernel<BT, T>), smem);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(splits, n_ct, n_rt);
+    cfg.blockDim = dim3(kWideThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = splits > 1 ? 1 : 0;
+    check_cuda(cudaLaunchKernelEx(&cfg, gemm_int8_wide_kernel<BT, T>, mw, mx, p, stages, splits),
+               ELIPS_B200_KERNEL_LAUNCH_FAILED, "int8 product launch");
+}
+
+template <class T>
+CUtensorMapDataType map_type();
+template <>
+CUtensorMapDataType map_type<float>() { return CU_TENSOR_MAP_DATA_TYPE_FLOAT32; }
+template <>
+CUtensorMapDataType map_type<__half>() { return CU_TENSOR_MAP_DATA_TYPE_FLOAT16; }
+template <>
+CUtensorMapDataType map_type<__nv_bfloat16>() { return CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; }
+
+template <class T>
+void launch_pair(const GemmParams& p, int num_sms, cudaStream_t stream) {
+    const uint32_t n_mt = cdiv(p.m, kPairM), n_nt = cdiv(p.n, kPairN);
+    if (static_cast<uint64_t>(n_mt) * n_nt > 0x7FFFFFFFull) bad("too many rows in one call");
+    const CUtensorMap ma = code_map(p.a, p.a_pitch, p.m, p.k, kPairM / 2);
+    const CUtensorMap mb = code_map(p.b, p.b_pitch, p.n, p.k, kPairN / 2);
+    const int64_t out_bytes = p.out_pitch * static_cast<int64_t>(sizeof(T));
+    const bool tma_out = on_16(p.out, out_bytes, p.m);
+    CUtensorMap mo{};
+    if (tma_out)
+        mo = make_operand_map(p.out, map_type<T>(), sizeof(T), p.n, p.m, 32,
+                              map_pitch(out_bytes, static_cast<uint64_t>(p.n) * sizeof(T), p.m));
+    allow_dynamic_smem(reinterpret_cast<const void*>(gemm_int8_pair_kernel<T>), kPairSmemBytes);
+    const uint32_t pairs = std::min<uint32_t>(n_mt * n_nt, static_cast<uint32_t>(num_sms) / 2);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(pairs * 2);
+    cfg.blockDim = dim3(kPairThreads);
+    cfg.dynamicSmemBytes = kPairSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    check_cuda(cudaLaunchKernelEx(&cfg, gemm_int8_pair_kernel<T>, ma, mb, mo, p, n_mt, n_nt, tma_out ? 1 : 0),
+               ELIPS_B200_KERNEL_LAUNCH_FAILED, "int8 product launch");
+}
+
+template <class T>
+void launch_gemm(const GemmParams& p, int num_sms, cudaStream_t stream) {
+    if (p.m <= 2 && p.k > 0) launch_dot<T>(p, num_sms, stream);
+    else if (p.m > 256 && p.k > 0) launch_pair<T>(p, num_sms, stream);
+    else if (p.m <= 16) launch_wide<16, T>(p, num_sms, stream);
+    else if (p.m <= 32) launch_wide<32, T>(p, num_sms, stream);
+    else if (p.m <= 64) launch_wide<64, T>(p, num_sms, stream);
+    else launch_wide<128, T>(p, num_sms, stream);
     launch_ok("int8 product launch");
+}
+
+void gemm_int8(int device, GemmParams p, int out_type, cudaStream_t stream) {
+    if (p.m == 0 || p.n == 0) return;
+    const int num_sms = device_props(device).num_sms;
+    // Operands whose rows do not start on 16 bytes are copied to rows that do:
+    // one more pass over them.
+    const bool a_ok = on_16(p.a, p.a_pitch, p.m), b_ok = on_16(p.b, p.b_pitch, p.n);
+    const size_t pitch = (static_cast<size_t>(p.k) + 15) / 16 * 16;
+    const size_t a_bytes = a_ok ? 0 : (p.m * pitch + 255) / 256 * 256, b_bytes = b_ok ? 0 : p.n * pitch;
+    auto product = [&] {
+        Profiler::Scope prof("gemm_int8", stream, static_cast<uint64_t>(p.m) * p.n);
+        with_float_type(out_type, [&](auto tag) { launch_gemm<decltype(tag)>(p, num_sms, stream); });
+    };
+    if ((a_ok && b_ok) || p.k == 0) {
+        product();
+        return;
+    }
+    StreamScratch s(a_bytes + b_bytes, stream);
+    auto repack = [&](const int8_t*& codes, int64_t& from, uint32_t rows, uint8_t* to) {
+        Profiler::Scope prof("repack_codes", stream, rows);
+        repack_codes_kernel<<<blocks_for(static_cast<uint64_t>(rows) * (pitch / 4), 256), 256, 0, stream>>>(
+            codes, from, reinterpret_cast<int8_t*>(to), static_cast<uint32_t>(pitch), rows, p.k);
+        launch_ok("operand copy launch");
+        codes = reinterpret_cast<const int8_t*>(to);
+        from = static_cast<int64_t>(pitch);
+    };
+    if (!a_ok) repack(p.a, p.a_pitch, p.m, s.get());
+    if (!b_ok) repack(p.b, p.b_pitch, p.n, s.get() + a_bytes);
+    product();
 }
 
 void check_gemm(size_t m, size_t n, size_t k, size_t b_pitch, const void* bias, int bias_type, int out_type,
@@ -209,7 +339,7 @@ GemmParams gemm_params(const int8_t* a, size_t a_pitch, const float* a_scales, c
     return p;
 }
 
-void linear_int8(const void* x, int x_type, int64_t x_pitch, const int8_t* b, size_t b_pitch, const float* b_scales,
+void linear_int8(int device, const void* x, int x_type, int64_t x_pitch, const int8_t* b, size_t b_pitch, const float* b_scales,
                  const void* bias, int bias_type, size_t m, size_t n, size_t k, void* out, int out_type,
                  size_t out_pitch, cudaStream_t stream) {
     if (m == 0 || n == 0) return;
@@ -219,13 +349,26 @@ void linear_int8(const void* x, int x_type, int64_t x_pitch, const int8_t* b, si
     int8_t* codes = reinterpret_cast<int8_t*>(s.get());
     float* scales = reinterpret_cast<float*>(s.get() + code_bytes);
     quantize_rows(x, x_type, m, k, x_pitch, codes, pitch, scales, stream);
-    gemm_int8(gemm_params(codes, pitch, scales, b, b_pitch, b_scales, bias, bias_type, m, n, k, out, out_pitch),
+    gemm_int8(device, gemm_params(codes, pitch, scales, b, b_pitch, b_scales, bias, bias_type, m, n, k, out, out_pitch),
               out_type, stream);
 }
 
 cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
 
 }  // namespace
+
+int take_int8_error(int device) {
+    DeviceGuard g(device);
+    int code = 0;
+    check_cuda(cudaMemcpyFromSymbol(&code, g_device_error, sizeof(int)), ELIPS_B200_TRANSFER_FAILED, "read device error");
+    if (code != 0) {
+        const int zero = 0;
+        check_cuda(cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int)), ELIPS_B200_TRANSFER_FAILED,
+                   "clear device error");
+    }
+    return code;
+}
+
 }  // namespace eb
 
 using eb::guarded;
@@ -254,7 +397,7 @@ int elips_b200_gemm_int8(int device, const int8_t* a, size_t a_stride, const flo
         if (a_stride < k) eb::bad("neighbouring matrix rows overlap");
         eb::DeviceGuard g(device);
         eb::device_props(device);
-        eb::gemm_int8(eb::gemm_params(a, a_stride, a_scales, b, b_stride, b_scales, bias, bias_type, m, n, k, out,
+        eb::gemm_int8(device, eb::gemm_params(a, a_stride, a_scales, b, b_stride, b_scales, bias, bias_type, m, n, k, out,
                                       out_stride),
                       out_type, eb::as_stream(stream));
     });
@@ -270,7 +413,7 @@ int elips_b200_linear_int8(int device, const void* x, int x_type, int64_t x_stri
         eb::check_rows(m, k, x_type);
         eb::DeviceGuard g(device);
         eb::device_props(device);
-        eb::linear_int8(x, x_type, x_stride, w, w_stride, w_scales, bias, bias_type, m, n, k, out, out_type,
+        eb::linear_int8(device, x, x_type, x_stride, w, w_stride, w_scales, bias, bias_type, m, n, k, out, out_type,
                         out_stride, eb::as_stream(stream));
     });
 }

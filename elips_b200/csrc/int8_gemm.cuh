@@ -1,0 +1,600 @@
+// The int8 matrix product with a scale per row and channel,
+//   out[i][j] = (sum_l a[i][l] b[j][l]) sa[i] sb[j] + bias[j],
+// in three forms; the host picks one by the number of rows (int8.cu).
+//
+//  * gemm_int8_dot_kernel: a few rows (the codes of single tokens). The
+//    weight is read once, 16 bytes a lane, and multiplied with dp4a.
+//  * gemm_int8_wide_kernel: rows up to a few hundred. The weight is the
+//    128-lane operand of the tensor core and the rows its narrow one; a
+//    cluster of CTAs shares one output tile and splits k, the partial sums
+//    meeting in shared memory.
+//  * gemm_int8_pair_kernel: many rows. Persistent CTA pairs, 256 x 256
+//    outputs per MMA, the epilogue of one tile under the products of the next.
+//
+// The sums are exact in int32 whatever their order, so every form and every
+// split gives the same bits: the conversion to fp32 (one rounding where the
+// sum passes 2^24), sa, then sb and the bias by one fused multiply-add, and
+// the rounding to the output's type.
+#pragma once
+
+#include <cstdint>
+
+#include "int8_kernels.cuh"
+#include "ptx.cuh"
+
+namespace eb {
+
+__device__ __forceinline__ float scaled(int32_t acc, float sa, float sb, float bias) {
+    return fmaf(static_cast<float>(acc) * sa, sb, bias);
+}
+
+// -------------------------------------------------------------- a few rows
+
+constexpr int kDotChannels = 4;  // weight rows per warp and step
+
+// MR rows of a against every row of b. A block's warps form groups of `wk`
+// that split k between them; a group takes kDotChannels rows of b. Rows of a
+// and b start on 16 bytes and their last 16 bytes may be read whole (the
+// bytes past k are masked out of a).
+template <int MR, class T>
+static __global__ void __launch_bounds__(256) gemm_int8_dot_kernel(const GemmParams p, uint32_t wk) {
+    __shared__ int32_t part[8][MR * kDotChannels];
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t group = (blockIdx.x * 8u + warp) / wk, kw = warp % wk;
+    const uint32_t n0 = group * kDotChannels;
+    const uint32_t chunks = (p.k + 15u) / 16u;
+    int32_t acc[MR][kDotChannels] = {};
+    const int8_t* br[kDotChannels];
+#pragma unroll
+    for (int c = 0; c < kDotChannels; ++c) br[c] = p.b + static_cast<int64_t>(min(n0 + c, p.n - 1u)) * p.b_pitch;
+    const uint32_t tail = p.k & 15u;
+#pragma unroll 4
+    for (uint32_t i = kw * 32u + lane; i < chunks; i += wk * 32u) {
+        int4 w[kDotChannels];
+#pragma unroll
+        for (int c = 0; c < kDotChannels; ++c) w[c] = __ldg(reinterpret_cast<const int4*>(br[c]) + i);
+#pragma unroll
+        for (int m = 0; m < MR; ++m) {
+            int4 x = __ldg(reinterpret_cast<const int4*>(p.a + static_cast<int64_t>(min(static_cast<uint32_t>(m), p.m - 1u)) * p.a_pitch) + i);
+            if (tail != 0u && i == chunks - 1u) {
+                int* xw = reinterpret_cast<int*>(&x);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int keep = static_cast<int>(tail) - 4 * j;
+                    xw[j] = keep >= 4 ? xw[j] : keep <= 0 ? 0 : xw[j] & ((1 << (8 * keep)) - 1);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < kDotChannels; ++c) {
+                int32_t s = acc[m][c];
+                s = __dp4a(x.x, w[c].x, s);
+                s = __dp4a(x.y, w[c].y, s);
+                s = __dp4a(x.z, w[c].z, s);
+                acc[m][c] = __dp4a(x.w, w[c].w, s);
+            }
+        }
+    }
+    int32_t mine = 0;  // lane m * kDotChannels + c keeps that sum
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+#pragma unroll
+        for (int c = 0; c < kDotChannels; ++c) {
+            const int32_t s = __reduce_add_sync(0xffffffffu, acc[m][c]);
+            if (lane == static_cast<uint32_t>(m * kDotChannels + c)) mine = s;
+        }
+    if (wk > 1u) {
+        if (lane < MR * kDotChannels) part[warp][lane] = mine;
+        __syncthreads();
+        if (kw != 0u) return;
+        if (lane < MR * kDotChannels)
+            for (uint32_t j = 1; j < wk; ++j) mine += part[warp + j][lane];
+    }
+    const uint32_t m = lane / kDotChannels, n = n0 + lane % kDotChannels;
+    if (lane >= MR * kDotChannels || m >= p.m || n >= p.n) return;
+    const float bias = p.bias == nullptr ? 0.0f : bias_at(p.bias, p.bias_type, n);
+    static_cast<T*>(p.out)[m * p.out_pitch + n] = from_f32<T>(scaled(mine, p.a_scales[m], p.b_scales[n], bias));
+}
+
+// ------------------------------------------------------------- wide kernel
+
+constexpr uint32_t kGemmStageK = 128;  // bytes of k per pipeline stage: one swizzle atom
+constexpr uint32_t kWideChannels = 128;
+constexpr uint32_t kWideMaxStages = 8;
+constexpr int kWideThreads = 192;  // TMA, MMA and four epilogue warps
+
+// A wait that must be sat out whatever else went wrong (an abort does not end
+// it, only its own limit): for what is under way before a CTA exits.
+__device__ __forceinline__ bool finish_wait(uint32_t bar, uint32_t parity) {
+    const long long start = clock64();
+    while (!mbar_try_wait(bar, parity)) {
+        if (clock64() - start > kWaitTimeoutCycles) {
+            record_device_error(kDevErrWaitTimeout);
+            return false;
+        }
+    }
+    return true;
+}
+
+// The last load issued to each stage (barriers `full0`, 8 bytes apart) lands.
+__device__ __forceinline__ void land_loads(uint32_t full0, uint32_t issued_mask, uint32_t issued_parity) {
+    while (issued_mask != 0u) {
+        const uint32_t s = __ffs(issued_mask) - 1u;
+        finish_wait(full0 + 8u * s, (issued_parity >> s) & 1u);
+        issued_mask &= issued_mask - 1u;
+    }
+}
+
+__device__ __forceinline__ int32_t ld_cluster(uint32_t addr) {
+    int32_t v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// One output tile of 128 channels x BT rows per cluster of `splits` CTAs
+// (grid: splits x channel tiles x row tiles). Each CTA sums its share of k in
+// TMEM. With one split a thread owns a channel and stores its column of the
+// tile straight from TMEM (a warp's stores of one row are neighbours); with
+// more, every CTA leaves its int32 tile in shared memory (over the pipeline's
+// buffers, which are done) and sums BT / splits rows over the cluster.
+template <int BT, class T>
+static __global__ void __launch_bounds__(kWideThreads)
+    gemm_int8_wide_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+                          const __grid_constant__ GemmParams p, uint32_t stages, uint32_t splits) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * kWideMaxStages + 1];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_word;
+    volatile int* const abort_flag = &abort_word;
+    constexpr uint32_t kWBytes = kWideChannels * kGemmStageK;
+    constexpr uint32_t kStageBytes = kWBytes + BT * kGemmStageK;
+    constexpr uint32_t kTmemCols = BT < 32 ? 32 : BT;
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t sbase = (raw + 1023u) & ~1023u;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t split = blockIdx.x;  // = rank in the cluster
+    const uint32_t n0 = blockIdx.y * kWideChannels, m0 = blockIdx.z * BT;
+    const uint32_t kblocks = (p.k + kGemmStageK - 1u) / kGemmStageK;
+    const uint32_t kb0 = static_cast<uint32_t>(static_cast<uint64_t>(kblocks) * split / splits);
+    const uint32_t kb1 = static_cast<uint32_t>(static_cast<uint64_t>(kblocks) * (split + 1u) / splits);
+    const uint32_t bar0 = smem_u32(bars);
+    auto full = [&](uint32_t s) { return bar0 + 8u * s; };
+    auto empty = [&](uint32_t s) { return bar0 + 8u * (kWideMaxStages + s); };
+    const uint32_t done = bar0 + 8u * (2 * kWideMaxStages);
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < stages; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        mbar_init(done, 1);
+        abort_word = 0;
+        fence_mbarrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(&tmem_slot), kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    if (warp == 0) {
+        if (elect_one_sync()) {
+            uint32_t stage = 0, phase = 0, issued_mask = 0, issued_parity = 0;
+            for (uint32_t kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait(empty(stage), phase ^ 1u, abort_flag)) break;
+                mbar_arrive_expect_tx(full(stage), kStageBytes);
+                const uint32_t dst = sbase + stage * kStageBytes;
+                tma_load_2d(dst, &tm_w, full(stage), static_cast<int32_t>(kb * kGemmStageK), static_cast<int32_t>(n0));
+                tma_load_2d(dst + kWBytes, &tm_x, full(stage), static_cast<int32_t>(kb * kGemmStageK), static_cast<int32_t>(m0));
+                issued_mask |= 1u << stage;
+                issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
+                if (++stage == stages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            land_loads(bar0, issued_mask, issued_parity);
+        }
+    } else if (warp == 1) {
+        if (elect_one_sync()) {
+            constexpr uint32_t idesc = make_idesc(2, 1, kWideChannels, BT);
+            uint32_t stage = 0, phase = 0;
+            for (uint32_t kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait(full(stage), phase, abort_flag)) break;
+                tc_fence_after();
+                const uint32_t w = sbase + stage * kStageBytes, x = w + kWBytes;
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k)
+                    tc_mma<MmaKind::I8>(tmem, smem_desc_k128(w + 32u * k), smem_desc_k128(x + 32u * k), idesc,
+                                        kb == kb0 && k == 0 ? 0u : 1u);
+                tc_commit(empty(stage));
+                if (++stage == stages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            tc_commit(done);
+        }
+    }
+    __syncwarp();
+    // Every warp waits for the sums: after this no load and no MMA is under
+    // way and the pipeline's buffers are free.
+    const bool ok = finish_wait(done, 0) && *abort_flag == 0;
+    tc_fence_after();
+    T* const out = static_cast<T*>(p.out);
+    if (warp >= 2) {
+        const uint32_t row = (warp & 3u) * 32u + lane;  // TMEM lane = channel of the tile
+        const uint32_t n = n0 + row;
+        const uint32_t taddr = tmem + (((warp & 3u) * 32u) << 16);
+        const bool valid = n < p.n;
+        float sb = 0.0f, bias = 0.0f;
+        if (splits == 1 && valid) {
+            sb = p.b_scales[n];
+            if (p.bias != nullptr) bias = bias_at(p.bias, p.bias_type, n);
+        }
+#pragma unroll 1
+        for (uint32_t c = 0; c < BT; c += 32) {
+            uint32_t v[32];
+            __syncwarp();
+            tmem_ld_32x32b_x32(taddr + c, v);
+            tmem_wait_ld();
+            if (kb0 == kb1) {
+#pragma unroll
+                for (uint32_t i = 0; i < 32; ++i) v[i] = 0;
+            }
+            if (splits == 1) {
+                if (!ok) continue;
+#pragma unroll
+                for (uint32_t i = 0; i < 32; ++i) {
+                    const uint32_t m = m0 + c + i;
+                    if (c + i < BT && m < p.m && valid)
+                        out[m * p.out_pitch + n] = from_f32<T>(scaled(static_cast<int32_t>(v[i]), __ldg(p.a_scales + m), sb, bias));
+                }
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < 32; ++i)
+                    if (c + i < BT)
+                        *reinterpret_cast<uint32_t*>(smem_raw + (sbase - raw) + ((c + i) * kWideChannels + row) * 4u) = v[i];
+            }
+        }
+    }
+    // TMEM goes back before this CTA waits for the others of its cluster: a CTA
+    // of another launch that waits for TMEM on this SM, and whose own partner
+    // holds the TMEM that a CTA of this cluster waits for, would never get it.
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemCols);
+    }
+    if (splits > 1) {
+        __syncwarp();
+        cluster_sync();
+        // Rows r of the tile with r % splits == split, one warp per row and
+        // step, a lane on every 32nd channel.
+        for (uint32_t r = split + splits * warp; r < BT && m0 + r < p.m; r += splits * (kWideThreads / 32)) {
+            const float sa = p.a_scales[m0 + r];
+#pragma unroll
+            for (uint32_t q = 0; q < kWideChannels / 32u; ++q) {
+                const uint32_t ch = q * 32u + lane, n = n0 + ch;
+                int32_t sum = 0;
+                for (uint32_t j = 0; j < splits; ++j)
+                    sum += ld_cluster(mapa_shared(sbase + (r * kWideChannels + ch) * 4u, j));
+                if (n < p.n) {
+                    const float bias = p.bias == nullptr ? 0.0f : bias_at(p.bias, p.bias_type, n);
+                    out[(m0 + r) * p.out_pitch + n] = from_f32<T>(scaled(sum, sa, p.b_scales[n], bias));
+                }
+            }
+        }
+        cluster_sync();  // the others may still read this CTA's sums
+    }
+}
+
+// ------------------------------------------------------------- pair kernel
+
+constexpr uint32_t kPairM = 256, kPairN = 256;
+constexpr uint32_t kPairStages = 5;
+constexpr uint32_t kPairEpilogueWarps = 8;
+constexpr int kPairThreads = 32 * (2 + kPairEpilogueWarps);
+constexpr uint32_t kPairStageBytes = (kPairM / 2 + kPairN / 2) * kGemmStageK;
+constexpr uint32_t kPairStoreBytes = 32 * 128;  // per epilogue warp: 32 rows of 128 bytes
+constexpr uint32_t kPairStoreOffset = kPairStages * kPairStageBytes;
+constexpr uint32_t kPairColsOffset = kPairStoreOffset + kPairEpilogueWarps * kPairStoreBytes;
+constexpr uint32_t kPairBarOffset = kPairColsOffset + kPairEpilogueWarps * (kPairN / 2) * 8;
+constexpr uint32_t kPairSmemBytes = 1024 + kPairBarOffset + 256;
+static_assert(8 * (2 * kPairStages + 5) + 16 <= 256, "barrier area");
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int32_t x, int32_t y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(src), "r"(x), "r"(y)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
+// Until this thread's bulk stores have read their shared memory.
+__device__ __forceinline__ void tma_store_wait_read() {
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+
+template <class T>
+struct Packed;
+template <>
+struct Packed<float> {
+    static __device__ __forceinline__ uint32_t pack(float a, float) { return __float_as_uint(a); }
+    static constexpr uint32_t per_word = 1;
+};
+template <>
+struct Packed<__half> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static constexpr uint32_t per_word = 2;
+};
+template <>
+struct Packed<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static constexpr uint32_t per_word = 2;
+};
+
+// Tile order: columns of `kPairGroup` row tiles, so that the tiles under way
+// at any time span about as many rows of a as of b and both stay in L2.
+constexpr uint32_t kPairGroup = 8;
+
+__device__ __forceinline__ void pair_tile(uint32_t i, uint32_t n_mt, uint32_t n_nt, uint32_t& mt, uint32_t& nt) {
+    const uint32_t per = kPairGroup * n_nt, g = i / per, r = i % per;
+    const uint32_t rows = min(kPairGroup, n_mt - g * kPairGroup);
+    mt = g * kPairGroup + r % rows;
+    nt = r / rows;
+}
+
+// Roles as in the search kernel: warp 0 loads, warp 1 of rank 0 issues the
+// pair's MMAs, eight warps empty one accumulator while the other fills. A
+// thread of the epilogue owns a row of a and half of the tile's columns; its
+// results go through 128-byte rows of shared memory to TMA stores, which drop
+// what lies outside the matrix, or, where the output's rows are no multiple
+// of 16 bytes, to plain stores.
+template <class T>
+static __global__ void __launch_bounds__(kPairThreads, 1)
+    gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                          const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ GemmParams p,
+                          uint32_t n_mt, uint32_t n_nt, int tma_out) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t sbase = (raw + 1023u) & ~1023u;
+    uint8_t* smem = smem_raw + (sbase - raw);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t rank = cluster_ctarank(), pair = cluster_id_x(), pairs = cluster_count_x();
+    const bool leader = rank == 0;
+    const uint32_t tiles = n_mt * n_nt;
+    const uint32_t kblocks = (p.k + kGemmStageK - 1u) / kGemmStageK;
+
+    const uint32_t bar0 = sbase + kPairBarOffset;
+    auto full_bar = [&](uint32_t s) { return bar0 + 8u * s; };
+    auto empty_bar = [&](uint32_t s) { return bar0 + 8u * (kPairStages + s); };
+    auto tfull_bar = [&](uint32_t a) { return bar0 + 8u * (2 * kPairStages + a); };
+    auto tempty_bar = [&](uint32_t a) { return bar0 + 8u * (2 * kPairStages + 2 + a); };
+    const uint32_t mma_done_bar = bar0 + 8u * (2 * kPairStages + 4);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kPairBarOffset + 8 * (2 * kPairStages + 5));
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    auto a_addr = [&](uint32_t s) { return sbase + s * kPairStageBytes; };
+    auto b_addr = [&](uint32_t s) { return a_addr(s) + kPairM / 2 * kGemmStageK; };
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < kPairStages; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        for (uint32_t a = 0; a < 2; ++a) {
+            mbar_init(tfull_bar(a), 1);
+            mbar_init(tempty_bar(a), kPairEpilogueWarps * 2);
+        }
+        mbar_init(mma_done_bar, 1);
+        *abort_flag = 0;
+        fence_mbarrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32(tmem_slot), 2 * kPairN);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        if (elect_one_sync()) {
+            tma_prefetch_desc(&tm_a);
+            tma_prefetch_desc(&tm_b);
+            uint32_t stage = 0, phase = 0, issued_mask = 0, issued_parity = 0;
+            bool ok = true;
+            for (uint32_t i = pair; ok && i < tiles; i += pairs) {
+                uint32_t mt, nt;
+                pair_tile(i, n_mt, n_nt, mt, nt);
+                const int32_t a_row = static_cast<int32_t>(mt * kPairM + rank * (kPairM / 2));
+                const int32_t b_row = static_cast<int32_t>(nt * kPairN + rank * (kPairN / 2));
+                for (uint32_t kb = 0; kb < kblocks; ++kb) {
+                    if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    const int32_t x = static_cast<int32_t>(kb * kGemmStageK);
+                    if (leader) mbar_arrive_expect_tx(full_bar(stage), 2u * kPairStageBytes);
+                    const uint32_t fb = mapa_shared(full_bar(stage), 0);
+                    tma_load_2d_pair(a_addr(stage), &tm_a, fb, x, a_row);
+                    tma_load_2d_pair(b_addr(stage), &tm_b, fb, x, b_row);
+                    issued_mask |= 1u << stage;
+                    issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
+                    if (++stage == kPairStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            // Every load must land before the CTAs exit; rank 0's barriers
+            // count both CTAs' bytes, and the peer leaves only after the
+            // closing cluster barrier.
+            if (leader) land_loads(bar0, issued_mask, issued_parity);
+        }
+    } else if (warp == 1) {
+        if (leader && elect_one_sync()) {
+            constexpr uint32_t idesc = make_idesc(2, 1, kPairM, kPairN);
+            uint32_t stage = 0, phase = 0, iter = 0;
+            bool ok = true;
+            for (uint32_t i = pair; ok && i < tiles; i += pairs, ++iter) {
+                const uint32_t acc = iter & 1u;
+                if (!mbar_wait_cluster(tempty_bar(acc), ((iter >> 1) & 1u) ^ 1u, abort_flag)) break;
+                tc_fence_after();
+                const uint32_t d = tmem_base + acc * kPairN;
+                for (uint32_t kb = 0; kb < kblocks; ++kb) {
+                    if (!mbar_wait(full_bar(stage), phase, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k)
+                        tc_mma<MmaKind::I8, 2>(d, smem_desc_k128(a_addr(stage) + 32u * k),
+                                               smem_desc_k128(b_addr(stage) + 32u * k), idesc, kb == 0 && k == 0 ? 0u : 1u);
+                    tc_commit_pair_both(empty_bar(stage), 0x3);
+                    if (++stage == kPairStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                tc_commit_pair_both(tfull_bar(acc), 0x3);
+            }
+            tc_commit_pair(mma_done_bar);
+            finish_wait(mma_done_bar, 0);
+        }
+    } else {
+        const uint32_t ew = warp - 2u, quad = warp & 3u, half = ew >> 2;
+        constexpr uint32_t kHalf = kPairN / 2;
+        constexpr uint32_t kCols = 128 / sizeof(T);  // columns per store: 128 bytes of output
+        constexpr uint32_t kPer = Packed<T>::per_word;
+        const uint32_t store = sbase + kPairStoreOffset + ew * kPairStoreBytes;
+        uint8_t* const store_ptr = smem + kPairStoreOffset + ew * kPairStoreBytes;
+        float2* const cols = reinterpret_cast<float2*>(smem + kPairColsOffset) + ew * kHalf;
+        const uint32_t tempty0 = mapa_shared(tempty_bar(0), 0), tempty1 = mapa_shared(tempty_bar(1), 0);
+        uint32_t iter = 0;
+        for (uint32_t i = pair; i < tiles; i += pairs, ++iter) {
+            uint32_t mt, nt;
+            pair_tile(i, n_mt, n_nt, mt, nt);
+            const uint32_t acc = iter & 1u;
+            const uint32_t m_warp = mt * kPairM + rank * (kPairM / 2) + quad * 32u;
+            const uint32_t m = m_warp + lane;
+            const uint32_t n_half = nt * kPairN + half * kHalf;
+            const float sa = m < p.m ? p.a_scales[m] : 0.0f;
+            for (uint32_t j = lane; j < kHalf; j += 32) {
+                const uint32_t n = n_half + j;
+                float2 c = make_float2(0.0f, 0.0f);
+                if (n < p.n) {
+                    c.x = p.b_scales[n];
+                    if (p.bias != nullptr) c.y = bias_at(p.bias, p.bias_type, n);
+                }
+                cols[j] = c;
+            }
+            __syncwarp();
+            bool ok = mbar_wait(tfull_bar(acc), (iter >> 1) & 1u, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t taddr = tmem_base + ((quad * 32u) << 16) + acc * kPairN + half * kHalf;
+#pragma unroll 1
+            for (uint32_t c0 = 0; c0 < kHalf; c0 += kCols) {
+                if (lane == 0) tma_store_wait_read();  // the buffer's last store
+                __syncwarp();
+#pragma unroll
+                for (uint32_t h = 0; h < kCols; h += 32) {
+                    uint32_t v[32];
+                    tmem_ld_32x32b_x32(taddr + c0 + h, v);
+                    tmem_wait_ld();
+                    uint32_t w[32 / kPer];
+#pragma unroll
+                    for (uint32_t j = 0; j < 32; j += kPer) {
+                        const float2 s0 = cols[c0 + h + j], s1 = cols[c0 + h + j + (kPer - 1)];
+                        w[j / kPer] = Packed<T>::pack(scaled(static_cast<int32_t>(v[j]), sa, s0.x, s0.y),
+                                                      scaled(static_cast<int32_t>(v[j + kPer - 1]), sa, s1.x, s1.y));
+                    }
+                    // 128-byte rows with their 16-byte pieces swizzled as the
+                    // store's tensor map (or the plain reader) expects
+#pragma unroll
+                    for (uint32_t j = 0; j < 32 / kPer; j += 4) {
+                        const uint32_t piece = h * sizeof(T) / 16u + j / 4u;
+                        *reinterpret_cast<uint4*>(store_ptr + lane * 128u + ((piece ^ (lane & 7u)) * 16u)) =
+                            make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+                    }
+                }
+                if (c0 + kCols >= kHalf) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(acc ? tempty1 : tempty0);
+                }
+                const uint32_t n = n_half + c0;
+                if (n >= p.n || m_warp >= p.m) {
+                    __syncwarp();
+                    continue;
+                }
+                if (tma_out) {
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) tma_store_2d(&tm_out, store, static_cast<int32_t>(n), static_cast<int32_t>(m_warp));
+                } else {
+                    __syncwarp();
+                    T* const out = static_cast<T*>(p.out);
+                    const uint32_t rows = min(32u, p.m - m_warp);
+                    for (uint32_t r = 0; r < rows; ++r) {
+#pragma unroll
+                        for (uint32_t q = 0; q < kCols; q += 32) {
+                            const uint32_t byte = (q + lane) * sizeof(T), piece = (byte / 16u) ^ (r & 7u);
+                            if (n + q + lane < p.n)
+                                out[(m_warp + r) * p.out_pitch + n + q + lane] =
+                                    *reinterpret_cast<const T*>(store_ptr + r * 128u + piece * 16u + byte % 16u);
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        // The bulk stores have to be complete, not only read, before the CTA
+        // exits and its shared memory goes to another.
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 2 * kPairN);
+    }
+}
+
+// ------------------------------------------------- operands that TMA cannot read
+
+// Copies rows whose start or pitch is no multiple of 16 bytes to rows of
+// `pitch` bytes (a multiple of 16), zero past the width.
+static __global__ void __launch_bounds__(256) repack_codes_kernel(const int8_t* in, int64_t in_pitch, int8_t* out,
+                                                                  uint32_t pitch, uint32_t rows, uint32_t k) {
+    const uint32_t words = pitch / 4u;
+    const uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256u + threadIdx.x;
+    if (i >= static_cast<uint64_t>(words) * rows) return;
+    const uint32_t r = static_cast<uint32_t>(i / words), c = static_cast<uint32_t>(i % words) * 4u;
+    const int8_t* src = in + r * in_pitch;
+    uint32_t w = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j)
+        if (c + j < k) w |= static_cast<uint32_t>(static_cast<uint8_t>(src[c + j])) << (8u * j);
+    *reinterpret_cast<uint32_t*>(out + static_cast<uint64_t>(r) * pitch + c) = w;
+}
+
+}  // namespace eb

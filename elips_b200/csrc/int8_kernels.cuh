@@ -207,10 +207,7 @@ static __global__ void __launch_bounds__(256) cache_read_kernel(const ReadParams
     for (uint32_t j = lane; j < p.d; j += 32) out[j] = from_f32<T>(static_cast<float>(q[j]) * sc);
 }
 
-// The int8 product C[m][n] = (sum_k A[m][k] B[n][k]) * sa[m] * sb[n] + bias[n]:
-// the sum is exact in int32 (k < 2^17), then three fp32 roundings (the
-// conversion where the sum passes 2^24, and each scale), the bias, and one
-// rounding to the output type.
+// The int8 product's arguments (int8_gemm.cuh).
 struct GemmParams {
     const int8_t* a;
     const int8_t* b;
@@ -228,51 +225,6 @@ __device__ __forceinline__ float bias_at(const void* bias, int type, uint32_t n)
     if (type == 1) return __half2float(static_cast<const __half*>(bias)[n]);
     if (type == 4) return __bfloat162float(static_cast<const __nv_bfloat16*>(bias)[n]);
     return static_cast<const float*>(bias)[n];
-}
-
-// 64 x 64 outputs per CTA, 4 x 4 per thread, 64 bytes of k staged at a time.
-template <class T>
-static __global__ void __launch_bounds__(256) gemm_int8_tile_kernel(const GemmParams p) {
-    __shared__ __align__(16) int8_t as[64][68], bs[64][68];
-    const uint32_t tid = threadIdx.x, tx = tid & 15u, ty = tid >> 4;
-    const uint32_t m0 = blockIdx.y * 64u, n0 = blockIdx.x * 64u;
-    int acc[4][4] = {};
-    for (uint32_t k0 = 0; k0 < p.k; k0 += 64) {
-        for (uint32_t e = tid; e < 64 * 64; e += 256) {
-            const uint32_t r = e >> 6, c = e & 63u;
-            const bool kin = k0 + c < p.k;
-            as[r][c] = kin && m0 + r < p.m ? p.a[(m0 + r) * p.a_pitch + k0 + c] : 0;
-            bs[r][c] = kin && n0 + r < p.n ? p.b[(n0 + r) * p.b_pitch + k0 + c] : 0;
-        }
-        __syncthreads();
-#pragma unroll 4
-        for (uint32_t c = 0; c < 64; c += 4) {
-            int av[4], bv[4];
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                av[i] = *reinterpret_cast<const int*>(&as[ty + 16 * i][c]);
-                bv[i] = *reinterpret_cast<const int*>(&bs[tx + 16 * i][c]);
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i)
-#pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) acc[i][j] = __dp4a(av[i], bv[j], acc[i][j]);
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t m = m0 + ty + 16 * i;
-        if (m >= p.m) continue;
-#pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-            const uint32_t n = n0 + tx + 16 * j;
-            if (n >= p.n) continue;
-            float v = static_cast<float>(acc[i][j]) * p.a_scales[m] * p.b_scales[n];
-            if (p.bias != nullptr) v += bias_at(p.bias, p.bias_type, n);
-            static_cast<T*>(p.out)[m * p.out_pitch + n] = from_f32<T>(v);
-        }
-    }
 }
 
 }  // namespace eb
