@@ -27,6 +27,8 @@ uint32_t blocks_for(uint64_t items, uint32_t per_block) {
     return static_cast<uint32_t>(b);
 }
 
+uint32_t cdiv(uint64_t a, uint64_t b) { return static_cast<uint32_t>((a + b - 1) / b); }
+
 constexpr size_t kMaxDim = size_t{1} << 24;
 constexpr size_t kMaxRows = 0x7FFFFFF0ull;
 // Largest k whose sum of products of int8 values (at most 2^14 each) stays
@@ -55,10 +57,57 @@ void with_float_type(int type, Fn&& fn) {
     }
 }
 
-void launch_quantize(int type, const QuantParams& p, bool claimed, cudaStream_t stream) {
-    const uint64_t rows = static_cast<uint64_t>(p.t) * p.parts * p.heads;
+template <class T, int V, int G, int NV>
+void launch_rows(const QuantParams& p, cudaStream_t stream) {
+    quantize_rows_kernel<T, V, G, NV><<<blocks_for(p.groups, 256 / G), 256, 0, stream>>>(p);
+}
+
+// The narrowest set of threads that holds a row in registers, a few accesses
+// each; rows wider than any are looped over by a block.
+template <class T, int V>
+void launch_rows_of(const QuantParams& p, cudaStream_t stream) {
+    const uint32_t n = (p.d + V - 1) / V;  // accesses per row
+    if (n <= 8) launch_rows<T, V, 8, 1>(p, stream);
+    else if (n <= 16) launch_rows<T, V, 8, 2>(p, stream);
+    else if (n <= 32) launch_rows<T, V, 8, 4>(p, stream);
+    else if (n <= 64) launch_rows<T, V, 32, 2>(p, stream);
+    else if (n <= 128) launch_rows<T, V, 32, 4>(p, stream);
+    else if (n <= 512) launch_rows<T, V, 256, 2>(p, stream);
+    else launch_rows<T, V, 256, 4>(p, stream);
+}
+
+// fn(first row, groups) for runs of rows whose (part, head) groups are fewer
+// than 2^30, what one launch indexes.
+template <class Fn>
+void in_runs(size_t t, uint32_t per_t, Fn&& fn) {
+    const size_t step = std::max<size_t>(1, (size_t{1} << 30) / per_t);
+    for (size_t t0 = 0; t0 < t; t0 += step) fn(static_cast<uint32_t>(t0), static_cast<uint32_t>(std::min(step, t - t0) * per_t));
+}
+
+// Rows are read 16 bytes at a time where every row starts on 16 bytes, holds a
+// whole number of them, and its codes can be stored as many at a time.
+template <class T>
+bool whole_accesses(const QuantParams& p, uint32_t parts) {
+    constexpr uint32_t V = 16 / sizeof(T);
+    uint64_t bits = p.d % V;
+    for (uint32_t i = 0; i < parts; ++i) {
+        bits |= reinterpret_cast<uintptr_t>(p.x[i]) % 16;
+        bits |= (static_cast<uint64_t>(p.x_stride_t[i]) | static_cast<uint64_t>(p.x_stride_h[i])) % V;
+    }
+    bits |= (reinterpret_cast<uintptr_t>(p.codes) | static_cast<uint64_t>(p.code_part | p.code_page | p.code_row | p.code_head)) % V;
+    return bits == 0;
+}
+
+void launch_quantize(int type, QuantParams p, uint32_t parts, cudaStream_t stream) {
     with_float_type(type, [&](auto tag) {
-        quantize_rows_kernel<decltype(tag)><<<blocks_for(rows, 8), 256, 0, stream>>>(p, claimed ? 1 : 0);
+        using T = decltype(tag);
+        const bool whole = whole_accesses<T>(p, parts);
+        in_runs(p.t, p.per_t.d, [&](uint32_t t0, uint32_t groups) {
+            p.t0 = t0;
+            p.groups = groups;
+            if (whole) launch_rows_of<T, 16 / sizeof(T)>(p, stream);
+            else launch_rows_of<T, 1>(p, stream);
+        });
     });
     launch_ok("row quantisation launch");
 }
@@ -68,23 +117,25 @@ void quantize_rows(const void* x, int type, size_t n, size_t d, int64_t x_pitch,
     if (n == 0) return;
     QuantParams p{};
     p.x[0] = x;
-    p.x_stride_t[0] = x_pitch;
+    p.x_stride_t[0] = n > 1 ? x_pitch : 0;
     p.codes = codes;
     p.scales = scales;
-    p.code_page = static_cast<int64_t>(code_pitch);
+    p.code_page = static_cast<int64_t>(n > 1 ? code_pitch : 0);
     p.scale_page = 1;
     p.t = static_cast<uint32_t>(n);
-    p.parts = p.heads = p.page = 1;
+    p.heads = 1;
     p.d = static_cast<uint32_t>(d);
     p.num_slots = static_cast<int64_t>(n);
+    p.dup = kDupNone;
     Profiler::Scope prof("quantize_rows", stream, n);
-    launch_quantize(type, p, false, stream);
+    launch_quantize(type, p, 1, stream);
 }
 
 void check_cache(const elips_b200_cache& c) {
     if (c.parts < 1 || c.parts > 2) bad("a cache has one or two parts");
     if (c.pages < 0 || c.page_size < 1 || c.heads < 1 || c.dim < 1) bad("cache sizes must be positive");
-    if (c.dim > static_cast<int64_t>(kMaxDim) || c.heads > (1 << 20)) bad("cache rows too wide");
+    if (c.dim > static_cast<int64_t>(kMaxDim) || c.heads > (1 << 20) || c.parts * c.heads * c.dim > (1 << 30))
+        bad("cache rows too wide");
     if (c.page_size > 0x7FFFFFFFll || c.pages > 0x7FFFFFFFll || c.pages * c.page_size > 0x7FFFFFFFll)
         bad("a cache holds fewer than 2^31 slots");
     if (c.pages > 0 && (c.codes == nullptr || c.scales == nullptr)) bad("cache without storage");
@@ -95,6 +146,14 @@ void check_cache_rows(const elips_b200_cache& c, const elips_b200_rows* rows, in
     if (t > kMaxRows) bad("too many rows in one call");
     for (int64_t i = 0; t > 0 && i < c.parts; ++i)
         if (rows[i].data == nullptr) bad("rows missing");
+}
+
+// The cache with 0 for the strides of axes of one entry, which address nothing.
+elips_b200_cache plain_strides(elips_b200_cache c) {
+    const int64_t sizes[4] = {c.parts, c.pages, c.page_size, c.heads};
+    for (int i = 0; i < 4; ++i)
+        if (sizes[i] == 1) c.code_strides[i] = c.scale_strides[i] = 0;
+    return c;
 }
 
 template <class P>
@@ -109,49 +168,81 @@ void set_cache(P& p, const elips_b200_cache& c) {
     p.scale_page = c.scale_strides[1];
     p.scale_row = c.scale_strides[2];
     p.scale_head = c.scale_strides[3];
-    p.parts = static_cast<uint32_t>(c.parts);
-    p.heads = static_cast<uint32_t>(c.heads);
-    p.page = static_cast<uint32_t>(c.page_size);
-    p.d = static_cast<uint32_t>(c.dim);
+    p.by_heads = FastDiv(static_cast<uint32_t>(c.heads));
+    p.page = FastDiv(static_cast<uint32_t>(c.page_size));
 }
 
-void cache_write(const elips_b200_cache& c, const elips_b200_rows* rows, int type, size_t t, const void* slots,
+void cache_write(const elips_b200_cache& given, const elips_b200_rows* rows, int type, size_t t, const void* slots,
                  int slots64, cudaStream_t stream) {
+    const elips_b200_cache c = plain_strides(given);
     if (t == 0 || c.pages == 0) return;
     QuantParams p{};
     set_cache(p, c);
     for (int64_t i = 0; i < c.parts; ++i) {
         p.x[i] = rows[i].data;
-        p.x_stride_t[i] = rows[i].stride_row;
-        p.x_stride_h[i] = rows[i].stride_head;
+        p.x_stride_t[i] = t > 1 ? rows[i].stride_row : 0;
+        p.x_stride_h[i] = c.heads > 1 ? rows[i].stride_head : 0;
     }
     p.slots = slots;
     p.slots64 = slots64;
     p.t = static_cast<uint32_t>(t);
+    p.heads = static_cast<uint32_t>(c.heads);
+    p.d = static_cast<uint32_t>(c.dim);
     p.num_slots = c.pages * c.page_size;
-    const uint64_t groups = static_cast<uint64_t>(t) * p.parts * p.heads;
-    const bool claimed = t > 1;
-    if (claimed) {
-        for (int clear = 1; clear >= 0; --clear) {
-            Profiler::Scope prof("cache_claim", stream, groups);
+    const uint32_t parts = static_cast<uint32_t>(c.parts);
+    p.per_t = FastDiv(parts * p.heads);
+    p.dup = t == 1 ? kDupNone : t <= kDupScanRows ? kDupScan : kDupClaim;
+    const uint64_t items = static_cast<uint64_t>(t) * p.per_t.d;
+    for (int clear = 1; p.dup == kDupClaim && clear >= 0; --clear) {
+        Profiler::Scope prof("cache_claim", stream, items);
+        in_runs(t, p.per_t.d, [&](uint32_t t0, uint32_t groups) {
+            p.t0 = t0;
+            p.groups = groups;
             cache_claim_kernel<<<blocks_for(groups, 256), 256, 0, stream>>>(p, clear);
-            launch_ok("cache claim launch");
-        }
+        });
+        launch_ok("cache claim launch");
     }
-    Profiler::Scope prof("cache_write", stream, groups);
-    launch_quantize(type, p, claimed, stream);
+    Profiler::Scope prof("cache_write", stream, items);
+    launch_quantize(type, p, parts, stream);
 }
 
-void cache_read(const elips_b200_cache& c, const void* table, int table64, int64_t table_stride, size_t sequences,
+// The most codes per access (a power of two, at most 16 bytes of output) that
+// the sizes and strides of a read allow.
+template <class T>
+uint32_t read_width(const ReadParams& p, const elips_b200_cache& c) {
+    uint64_t bits = static_cast<uint64_t>(c.dim) | reinterpret_cast<uintptr_t>(c.codes);
+    for (int i = 0; i < 4; ++i) bits |= static_cast<uint64_t>(c.code_strides[i]);
+    for (int64_t i = 0; i < c.parts; ++i) {
+        bits |= static_cast<uint64_t>(p.out_stride_t[i] | p.out_stride_h[i]);
+        bits |= reinterpret_cast<uintptr_t>(p.out[i]) / sizeof(T);
+    }
+    uint32_t v = 16 / sizeof(T);
+    while (bits % v != 0) v /= 2;
+    return v;
+}
+
+template <class T, int V>
+void launch_read(ReadParams p, const elips_b200_cache& c, int num_sms, cudaStream_t stream) {
+    p.per_group = FastDiv(static_cast<uint32_t>(c.dim) / V);
+    p.per_row = FastDiv(static_cast<uint32_t>(c.parts * c.heads) * p.per_group.d);
+    // About eight accesses a thread, and at least two blocks an SM.
+    uint64_t rows = std::min<uint64_t>(kReadRows, std::max<uint64_t>(1, 2048 / p.per_row.d));
+    rows = std::min<uint64_t>(rows, cdiv(p.total, 2u * static_cast<uint32_t>(num_sms)));
+    p.rows = static_cast<uint32_t>(rows);
+    cache_read_kernel<T, V><<<blocks_for(p.total, p.rows), 256, 0, stream>>>(p);
+}
+
+void cache_read(int device, const elips_b200_cache& given, const void* table, int table64, int64_t table_stride, size_t sequences,
                 size_t table_width, const void* offsets, int offsets64, size_t total, const elips_b200_rows* out,
                 int type, int zero_behind, cudaStream_t stream) {
+    const elips_b200_cache c = plain_strides(given);
     if (total == 0) return;
     ReadParams p{};
     set_cache(p, c);
     for (int64_t i = 0; i < c.parts; ++i) {
         p.out[i] = const_cast<void*>(out[i].data);
-        p.out_stride_t[i] = out[i].stride_row;
-        p.out_stride_h[i] = out[i].stride_head;
+        p.out_stride_t[i] = total > 1 ? out[i].stride_row : 0;
+        p.out_stride_h[i] = c.heads > 1 ? out[i].stride_head : 0;
     }
     p.table = table;
     p.table64 = table64;
@@ -163,15 +254,20 @@ void cache_read(const elips_b200_cache& c, const void* table, int table64, int64
     p.pages = static_cast<uint32_t>(c.pages);
     p.total = static_cast<uint32_t>(total);
     p.zero_behind = zero_behind;
-    const uint64_t groups = static_cast<uint64_t>(total) * p.parts * p.heads;
-    Profiler::Scope prof("cache_read", stream, groups);
+    const int num_sms = device_props(device).num_sms;
+    Profiler::Scope prof("cache_read", stream, static_cast<uint64_t>(total) * static_cast<uint64_t>(c.parts * c.heads));
     with_float_type(type, [&](auto tag) {
-        cache_read_kernel<decltype(tag)><<<blocks_for(groups, 8), 256, 0, stream>>>(p);
+        using T = decltype(tag);
+        const uint32_t v = read_width<T>(p, c);
+        if constexpr (sizeof(T) == 2) {
+            if (v == 8) return launch_read<T, 8>(p, c, num_sms, stream);
+        }
+        if (v >= 4) launch_read<T, 4>(p, c, num_sms, stream);
+        else if (v == 2) launch_read<T, 2>(p, c, num_sms, stream);
+        else launch_read<T, 1>(p, c, num_sms, stream);
     });
     launch_ok("cache read launch");
 }
-
-uint32_t cdiv(uint64_t a, uint64_t b) { return static_cast<uint32_t>((a + b - 1) / b); }
 
 bool on_16(const void* ptr, int64_t pitch_bytes, uint32_t rows) {
     return reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && (rows <= 1 || pitch_bytes % 16 == 0);
@@ -444,7 +540,7 @@ int elips_b200_cache_read(int device, const elips_b200_cache* cache, const void*
         if (total > 0 && sequences > 0 && table_width > 0 && page_table == nullptr) eb::bad("page table missing");
         eb::DeviceGuard g(device);
         eb::device_props(device);
-        eb::cache_read(*cache, page_table, table_64bit, table_stride, sequences, table_width, offsets, offsets_64bit,
+        eb::cache_read(device, *cache, page_table, table_64bit, table_stride, sequences, table_width, offsets, offsets_64bit,
                        total, out, type, zero_behind, eb::as_stream(stream));
     });
 }

@@ -49,17 +49,69 @@ __device__ __forceinline__ float row_inverse(float s) {
     return s > 0.0f && s < __int_as_float(0x7f800000) ? __frcp_rn(s) : 0.0f;
 }
 
-// The integer nearest to x / s. t = x * inv is within 2^-16 of the quotient
-// (|t| <= 127.5, inv is 1/s to half an ulp), so rint(t) is the answer unless t
-// lies that near to a half; only there the quotient is taken in 64 bits, where
-// its distance from a half decides exactly (x - (q + 1/2) s is a multiple of
-// ulp(s)/2, so a quotient that is no tie is at least 2^-25 relative away).
-__device__ __forceinline__ int row_code(float x, float s, float inv) {
-    if (inv == 0.0f) return 0;
-    const float t = x * inv;
-    const float q = rintf(t);
-    if (fabsf(t - q) > 0.5f - 0x1p-15f) return static_cast<int>(rint(static_cast<double>(x) / static_cast<double>(s)));
-    return static_cast<int>(q);
+// The integer nearest to x / s by a 64-bit division. A quotient of two fp32
+// numbers that is no tie is at least 2^-25 (relative) away from one, because
+// x - (q + 1/2) s is a multiple of half an ulp of s: the division decides.
+__device__ __noinline__ int row_code_exact(float x, float s) {
+    return static_cast<int>(rint(static_cast<double>(x) / static_cast<double>(s)));
+}
+
+// Adding 1.5 * 2^23 to a number below 2^22 rounds it to the nearest integer,
+// ties to even, and leaves that integer in the low bits of the sum.
+constexpr float kRound = 12582912.0f;
+
+// V codes of one row, packed. inv is 1/s to half an ulp, so x * inv is within
+// 2^-17 of the quotient (|x / s| < 127.5): its nearest integer is the code
+// unless it lies that near to a half, and only then the exact division runs
+// (for values that are half steps by their making, and else 1 in 2^15).
+template <int V>
+__device__ __forceinline__ void row_codes(const float (&x)[V], float s, float inv, uint32_t (&w)[(V + 3) / 4]) {
+    uint32_t m[V];
+    float off = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const float r = fmaf(x[i], inv, kRound);
+        off = fmaxf(off, fabsf(fmaf(x[i], inv, kRound - r)));
+        m[i] = __float_as_uint(r);
+    }
+    if (off > 0.5f - 0x1p-16f) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) m[i] = static_cast<uint32_t>(row_code_exact(x[i], s));
+    }
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+        uint32_t lo = m[i], hi = 0;
+        if constexpr (V >= 2) lo = __byte_perm(m[i], m[i + 1], 0x0040);
+        if constexpr (V >= 4) hi = __byte_perm(m[i + 2], m[i + 3], 0x0040);
+        w[i / 4] = __byte_perm(lo, hi, 0x5410);
+    }
+}
+
+// Division of numbers below 2^31 by a fixed divisor: a multiply, an add and a
+// shift (mul = floor(2^32 (2^shift - d) / d) + 1 with 2^shift >= d).
+struct FastDiv {
+    uint32_t d = 1, mul = 1, shift = 0;
+    __host__ __device__ FastDiv() {}
+    __host__ explicit FastDiv(uint32_t divisor) : d(divisor) {
+        while (shift < 31 && (1u << shift) < d) ++shift;
+        mul = static_cast<uint32_t>((((uint64_t{1} << shift) - d) << 32) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+
+// V elements as fp32, from one access of V * sizeof(T) bytes.
+template <class T, int V>
+__device__ __forceinline__ void load_row(const T* src, float (&x)[V]) {
+    if constexpr (V == 1) {
+        x[0] = to_f32(src[0]);
+    } else if constexpr (sizeof(T) * V == 16) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(src);
+        const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = to_f32(e[i]);
+    } else {
+        static_assert(V == 1, "rows are read 16 bytes or one element at a time");
+    }
 }
 
 // Where rows come from and where their codes go: row (part, t, head) of the
@@ -75,9 +127,14 @@ struct QuantParams {
     int64_t scale_part, scale_page, scale_row, scale_head;  // elements
     const void* slots;  // [t], int32 or int64; null: row t goes to slot t
     int slots64;
-    uint32_t t, parts, heads, d, page;
+    uint32_t t, heads, d;
+    uint32_t t0, groups;  // this launch: rows of t0 on, (t, part, head) groups of them
+    FastDiv per_t, by_heads, page;
     int64_t num_slots;
+    int dup;  // a slot may come twice: kDupNone, kDupScan or kDupClaim
 };
+
+enum DupCheck : int { kDupNone = 0, kDupScan = 1, kDupClaim = 2 };
 
 __device__ __forceinline__ int64_t slot_of(const QuantParams& p, uint32_t t) {
     if (p.slots == nullptr) return t;
@@ -85,58 +142,135 @@ __device__ __forceinline__ int64_t slot_of(const QuantParams& p, uint32_t t) {
 }
 
 __device__ __forceinline__ float* scale_at(const QuantParams& p, uint32_t part, uint32_t slot, uint32_t head) {
-    return p.scales + part * p.scale_part + static_cast<int64_t>(slot / p.page) * p.scale_page +
-           static_cast<int64_t>(slot % p.page) * p.scale_row + head * p.scale_head;
+    const uint32_t pg = p.page.div(slot), at = slot - pg * p.page.d;
+    return p.scales + part * p.scale_part + pg * p.scale_page + at * p.scale_row + head * p.scale_head;
 }
 
-// A slot given twice in one call keeps the last of its rows. Who writes is
-// settled in the slot's own scale words before any row is written: one launch
-// zeroes them, the next leaves the largest claim 0x80000001 + t there, and the
-// row whose claim stands writes codes and scale. A scale is never negative, so
-// no scale written in between is taken for a claim.
+// The part, row and head of group g of this launch.
+__device__ __forceinline__ void group_at(const QuantParams& p, uint32_t g, uint32_t& t, uint32_t& part, uint32_t& head) {
+    const uint32_t i = p.per_t.div(g), r = g - i * p.per_t.d;
+    t = p.t0 + i;
+    part = p.by_heads.div(r);
+    head = r - part * p.heads;
+}
+
+// A slot given twice in one call keeps the last of its rows. Up to
+// kDupScanRows rows each row looks for its slot among the later ones (which
+// stay in L1). Longer calls settle it in the slot's own scale words before any
+// row is written: one launch zeroes them, the next leaves the largest claim
+// 0x80000001 + t there, and the row whose claim stands writes codes and scale.
+// A scale is never negative, so no scale written in between is taken for a
+// claim; what the words held before does not matter.
+constexpr uint32_t kDupScanRows = 256;
+
 __device__ __forceinline__ uint32_t claim_of(uint32_t t) { return 0x80000001u + t; }
 
-static __global__ void __launch_bounds__(256) cache_claim_kernel(const QuantParams p, int clear) {
-    const uint64_t per_t = static_cast<uint64_t>(p.parts) * p.heads;
-    const uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256u + threadIdx.x;
-    if (i >= per_t * p.t) return;
-    const uint32_t t = static_cast<uint32_t>(i / per_t), r = static_cast<uint32_t>(i % per_t);
+static __global__ void __launch_bounds__(256) cache_claim_kernel(const __grid_constant__ QuantParams p, int clear) {
+    const uint32_t g = blockIdx.x * 256u + threadIdx.x;
+    if (g >= p.groups) return;
+    uint32_t t, part, head;
+    group_at(p, g, t, part, head);
     const int64_t s = slot_of(p, t);
     if (s < 0 || s >= p.num_slots) return;
-    uint32_t* w = reinterpret_cast<uint32_t*>(scale_at(p, r / p.heads, static_cast<uint32_t>(s), r % p.heads));
+    uint32_t* w = reinterpret_cast<uint32_t*>(scale_at(p, part, static_cast<uint32_t>(s), head));
     if (clear) *w = 0u;
     else atomicMax(w, claim_of(t));
 }
 
-// One warp per row: the largest magnitude, then the codes from a second read.
-template <class T>
-static __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p, int claimed) {
-    const uint32_t lane = threadIdx.x & 31u;
-    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * 8u + (threadIdx.x >> 5);
-    const uint64_t per_t = static_cast<uint64_t>(p.parts) * p.heads;
-    if (row >= per_t * p.t) return;
-    const uint32_t t = static_cast<uint32_t>(row / per_t), r = static_cast<uint32_t>(row % per_t);
-    const uint32_t part = r / p.heads, head = r % p.heads;
-    const int64_t s = slot_of(p, t);
-    if (s < 0 || s >= p.num_slots) return;
-    const uint32_t slot = static_cast<uint32_t>(s);
-    float* const scale = scale_at(p, part, slot, head);
-    if (claimed) {
-        // Read by one lane, before any lane can write: the row's own claim
-        // stands until lane 0 stores the scale below.
-        uint32_t w = 0;
-        if (lane == 0) w = *reinterpret_cast<volatile uint32_t*>(scale);
-        if (__shfl_sync(0xffffffffu, w, 0) != claim_of(t)) return;
+// G threads per row (8, a warp, or the whole block), each holding NV accesses
+// of V values in registers: one read of the row, the largest magnitude over
+// its threads, the codes. Rows wider than G * NV * V (only where G is the
+// block) are read a second time for what did not fit.
+template <class T, int V, int G, int NV>
+static __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_constant__ QuantParams p) {
+    __shared__ uint32_t block_max[8];
+    constexpr uint32_t kPer = 256 / G;  // rows per block
+    constexpr uint32_t kHeld = G * NV * V;
+    const uint32_t gl = threadIdx.x % G;
+    const uint32_t g = blockIdx.x * kPer + threadIdx.x / G;
+    uint32_t t = 0, part = 0, head = 0;
+    int64_t s = -1;
+    if (g < p.groups) {
+        group_at(p, g, t, part, head);
+        s = slot_of(p, t);
     }
-    const T* x = static_cast<const T*>(p.x[part]) + t * p.x_stride_t[part] + head * p.x_stride_h[part];
+    // Rows of one warp stay together to the end: they share its votes.
+    bool keep = s >= 0 && s < p.num_slots;
+    const uint32_t slot = keep ? static_cast<uint32_t>(s) : 0u;
+    float* const scale = scale_at(p, part, slot, head);
+    const T* const x = static_cast<const T*>(p.x[part]) + t * p.x_stride_t[part] + head * p.x_stride_h[part];
+
+    float v[NV][V];
     uint32_t amax = 0;
-    for (uint32_t j = lane; j < p.d; j += 32) amax = max(amax, __float_as_uint(to_f32(x[j])) & 0x7FFFFFFFu);
-    amax = __reduce_max_sync(0xffffffffu, amax);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const uint32_t e = (j * G + gl) * V;
+        if (e < p.d && keep) {
+            load_row<T, V>(x + e, v[j]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[j][i] = 0.0f;
+        }
+    }
+    if (p.dup == kDupClaim) {
+        // The row's own claim stands until it stores its scale below.
+        if (keep) keep = *reinterpret_cast<volatile uint32_t*>(scale) == claim_of(t);
+    } else if (p.dup == kDupScan && keep) {
+        for (uint32_t i = t + 1u + gl; i < p.t; i += G) keep = keep && slot_of(p, i) != s;
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) amax = max(amax, __float_as_uint(v[j][i]) & 0x7FFFFFFFu);
+    if constexpr (G == 256) {
+        for (uint32_t e = kHeld + gl * V; e < p.d; e += G * V) {
+            float u[V];
+            load_row<T, V>(x + e, u);
+#pragma unroll
+            for (int i = 0; i < V; ++i) amax = max(amax, __float_as_uint(u[i]) & 0x7FFFFFFFu);
+        }
+        if (__syncthreads_or(!keep)) return;
+        amax = __reduce_max_sync(0xFFFFFFFFu, amax);
+        if ((threadIdx.x & 31u) == 0) block_max[threadIdx.x >> 5] = amax;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amax = max(amax, block_max[i]);
+    } else {
+        const uint32_t kept = __ballot_sync(0xFFFFFFFFu, keep);
+        if constexpr (G == 32) {
+            keep = kept == 0xFFFFFFFFu;
+            amax = __reduce_max_sync(0xFFFFFFFFu, amax);
+        } else {
+            constexpr uint32_t kPeers = (1u << (G % 32)) - 1u;
+            keep = ((kept >> (threadIdx.x & 31u & ~(G - 1u))) & kPeers) == kPeers;
+#pragma unroll
+            for (int o = G / 2; o > 0; o /= 2) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+        }
+        if (!keep) return;
+    }
     const float sc = row_scale(amax), inv = row_inverse(sc);
-    int8_t* out = p.codes + part * p.code_part + static_cast<int64_t>(slot / p.page) * p.code_page +
-                  static_cast<int64_t>(slot % p.page) * p.code_row + head * p.code_head;
-    for (uint32_t j = lane; j < p.d; j += 32) out[j] = static_cast<int8_t>(row_code(to_f32(x[j]), sc, inv));
-    if (lane == 0) *scale = sc;
+    const uint32_t pg = p.page.div(slot), at = slot - pg * p.page.d;
+    int8_t* const out = p.codes + part * p.code_part + pg * p.code_page + at * p.code_row + head * p.code_head;
+    auto put = [&](uint32_t e, const float (&u)[V]) {
+        uint32_t w[(V + 3) / 4] = {};
+        if (inv != 0.0f) row_codes<V>(u, sc, inv, w);
+        if constexpr (V == 8) *reinterpret_cast<uint2*>(out + e) = make_uint2(w[0], w[V / 4 - 1]);
+        else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(out + e) = w[0];
+        else out[e] = static_cast<int8_t>(w[0]);
+    };
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const uint32_t e = (j * G + gl) * V;
+        if (e < p.d) put(e, v[j]);
+    }
+    if constexpr (G == 256) {
+        for (uint32_t e = kHeld + gl * V; e < p.d; e += G * V) {
+            float u[V];
+            load_row<T, V>(x + e, u);
+            put(e, u);
+        }
+    }
+    if (gl == 0) *scale = sc;
 }
 
 // Reading pages back into packed rows. Sequence b owns the output rows
@@ -153,8 +287,9 @@ struct ReadParams {
     const void* offsets;
     int table64, offsets64;
     int64_t table_stride;
-    uint32_t sequences, table_width, pages, page, parts, heads, d;
-    uint32_t total;
+    uint32_t sequences, table_width, pages;
+    uint32_t total, rows;                           // output rows, and those of one block
+    FastDiv page, per_row, per_group, by_heads;     // accesses of V codes per output row and per (part, head)
     int zero_behind;  // rows past the last sequence: zeroed (a fresh output) or left as they are
 };
 
@@ -178,33 +313,89 @@ __device__ __forceinline__ int64_t read_slot(const ReadParams& p, uint32_t t) {
     const int64_t i = static_cast<int64_t>(t) - offset_of(p, lo);
     if (i < 0) return kRowNoPage;
     const uint32_t pos = static_cast<uint32_t>(i);  // i <= t
-    const uint32_t col = pos / p.page;
+    const uint32_t col = p.page.div(pos);
     if (col >= p.table_width) return kRowNoPage;
     const int64_t at = static_cast<int64_t>(lo) * p.table_stride + col;
     const int64_t pg = p.table64 ? static_cast<const int64_t*>(p.table)[at] : static_cast<const int32_t*>(p.table)[at];
     if (pg < 0 || pg >= static_cast<int64_t>(p.pages)) return kRowNoPage;
-    return pg * p.page + pos % p.page;
+    return pg * p.page.d + (pos - col * p.page.d);
 }
 
-template <class T>
-static __global__ void __launch_bounds__(256) cache_read_kernel(const ReadParams p) {
-    const uint32_t lane = threadIdx.x & 31u;
-    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * 8u + (threadIdx.x >> 5);
-    const uint64_t per_t = static_cast<uint64_t>(p.parts) * p.heads;
-    if (row >= per_t * p.total) return;
-    const uint32_t t = static_cast<uint32_t>(row / per_t), r = static_cast<uint32_t>(row % per_t);
-    const uint32_t part = r / p.heads, head = r % p.heads;
-    const int64_t s = read_slot(p, t);
-    if (s == kRowBehind && !p.zero_behind) return;
-    T* out = static_cast<T*>(p.out[part]) + t * p.out_stride_t[part] + head * p.out_stride_h[part];
-    if (s < 0) {
-        for (uint32_t j = lane; j < p.d; j += 32) out[j] = from_f32<T>(0.0f);
-        return;
+// int8 -> fp32 without the conversion unit: the byte with its sign bit turned
+// (0 .. 255) in the low bits of 2^23 is 2^23 + byte, exactly.
+__device__ __forceinline__ float code_f32(uint32_t turned, uint32_t byte) {
+    return __uint_as_float(__byte_perm(turned, 0x4B000000u, 0x7440u | byte)) - 8388736.0f;  // 2^23 + 128
+}
+
+constexpr uint32_t kReadRows = 64;  // most output rows per block
+constexpr int kReadBatch = 4;       // accesses a thread has under way
+
+// A block reads `rows` output rows: first their slots, one thread each, then
+// the codes, V at a time (16 bytes of output where everything is aligned so
+// far), neighbouring threads on neighbouring codes of a row. One pass, bound
+// by the bytes: 1 + sizeof(T) and 4 / dim per value.
+template <class T, int V>
+static __global__ void __launch_bounds__(256) cache_read_kernel(const __grid_constant__ ReadParams p) {
+    __shared__ int64_t code_at[kReadRows], scale_at[kReadRows];
+    const uint32_t t0 = blockIdx.x * p.rows, rows = min(p.rows, p.total - t0);
+    if (threadIdx.x < rows) {
+        const int64_t s = read_slot(p, t0 + threadIdx.x);
+        int64_t code = s, scale = s;
+        if (s >= 0) {
+            const uint32_t pg = p.page.div(static_cast<uint32_t>(s)), at = static_cast<uint32_t>(s) - pg * p.page.d;
+            code = pg * p.code_page + at * p.code_row;
+            scale = pg * p.scale_page + at * p.scale_row;
+        }
+        code_at[threadIdx.x] = code;
+        scale_at[threadIdx.x] = s < 0 ? s : scale;
     }
-    const int64_t pg = s / p.page, at = s % p.page;
-    const int8_t* q = p.codes + part * p.code_part + pg * p.code_page + at * p.code_row + head * p.code_head;
-    const float sc = p.scales[part * p.scale_part + pg * p.scale_page + at * p.scale_row + head * p.scale_head];
-    for (uint32_t j = lane; j < p.d; j += 32) out[j] = from_f32<T>(static_cast<float>(q[j]) * sc);
+    __syncthreads();
+    const uint32_t items = rows * p.per_row.d;
+    for (uint32_t i0 = threadIdx.x; i0 < items; i0 += 256u * kReadBatch) {
+        // The loads of a batch are issued before the first of its stores.
+        uint32_t w[kReadBatch][(V + 3) / 4];
+        float sc[kReadBatch];
+        T* out[kReadBatch];
+#pragma unroll
+        for (int b = 0; b < kReadBatch; ++b) {
+            const uint32_t i = i0 + 256u * b;
+            out[b] = nullptr;
+            if (i >= items) continue;
+            const uint32_t row = p.per_row.div(i), r = i - row * p.per_row.d;
+            const uint32_t group = p.per_group.div(r), e = (r - group * p.per_group.d) * V;
+            const uint32_t part = p.by_heads.div(group), head = group - part * p.by_heads.d;
+            const int64_t code = code_at[row];
+            if (code == kRowBehind && !p.zero_behind) continue;
+            out[b] = static_cast<T*>(p.out[part]) + (t0 + row) * p.out_stride_t[part] + head * p.out_stride_h[part] + e;
+            sc[b] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < (V + 3) / 4; ++j) w[b][j] = 0;
+            if (code < 0) continue;
+            const int8_t* q = p.codes + code + part * p.code_part + head * p.code_head + e;
+            if constexpr (V == 8) {
+                const uint2 u = __ldg(reinterpret_cast<const uint2*>(q));
+                w[b][0] = u.x, w[b][V / 4 - 1] = u.y;
+            } else if constexpr (V == 4) {
+                w[b][0] = __ldg(reinterpret_cast<const uint32_t*>(q));
+            } else if constexpr (V == 2) {
+                w[b][0] = __ldg(reinterpret_cast<const uint16_t*>(q));
+            } else {
+                w[b][0] = static_cast<uint8_t>(__ldg(q));
+            }
+            sc[b] = __ldg(p.scales + scale_at[row] + part * p.scale_part + head * p.scale_head);
+        }
+#pragma unroll
+        for (int b = 0; b < kReadBatch; ++b) {
+            if (out[b] == nullptr) continue;
+            alignas(16) T v[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = from_f32<T>(code_f32(w[b][j / 4] ^ 0x80808080u, j % 4) * sc[b]);
+            if constexpr (sizeof(T) * V == 16) *reinterpret_cast<uint4*>(out[b]) = *reinterpret_cast<const uint4*>(v);
+            else if constexpr (sizeof(T) * V == 8) *reinterpret_cast<uint2*>(out[b]) = *reinterpret_cast<const uint2*>(v);
+            else if constexpr (sizeof(T) * V == 4) *reinterpret_cast<uint32_t*>(out[b]) = *reinterpret_cast<const uint32_t*>(v);
+            else *out[b] = v[0];
+        }
+    }
 }
 
 // The int8 product's arguments (int8_gemm.cuh).
