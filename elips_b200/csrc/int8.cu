@@ -59,20 +59,25 @@ void with_float_type(int type, Fn&& fn) {
 
 template <class T, int V, int G, int NV>
 void launch_rows(const QuantParams& p, cudaStream_t stream) {
-    quantize_rows_kernel<T, V, G, NV><<<blocks_for(p.groups, 256 / G), 256, 0, stream>>>(p);
+    const uint32_t blocks = blocks_for(p.groups, 256 / G);
+    if (p.slots != nullptr) quantize_rows_kernel<T, V, G, NV, true><<<blocks, 256, 0, stream>>>(p);
+    else quantize_rows_kernel<T, V, G, NV, false><<<blocks, 256, 0, stream>>>(p);
 }
 
-// The narrowest set of threads that holds a row in registers, a few accesses
-// each; rows wider than any are looped over by a block.
+// Few threads with many accesses each: what a thread spends on finding its row
+// is shared by more values, and up to 512 accesses a row needs no more than a
+// warp. Wider rows take a block.
 template <class T, int V>
 void launch_rows_of(const QuantParams& p, cudaStream_t stream) {
     const uint32_t n = (p.d + V - 1) / V;  // accesses per row
-    if (n <= 8) launch_rows<T, V, 8, 1>(p, stream);
-    else if (n <= 16) launch_rows<T, V, 8, 2>(p, stream);
-    else if (n <= 32) launch_rows<T, V, 8, 4>(p, stream);
-    else if (n <= 64) launch_rows<T, V, 32, 2>(p, stream);
+    if constexpr (V > 1) {
+        if (n <= 8) return launch_rows<T, V, 4, 2>(p, stream);
+        if (n <= 16) return launch_rows<T, V, 4, 4>(p, stream);
+    }
+    if (n <= 32) launch_rows<T, V, 8, 4>(p, stream);
     else if (n <= 128) launch_rows<T, V, 32, 4>(p, stream);
-    else if (n <= 512) launch_rows<T, V, 256, 2>(p, stream);
+    else if (n <= 256) launch_rows<T, V, 32, 8>(p, stream);
+    else if (n <= 512) launch_rows<T, V, 32, 16>(p, stream);
     else launch_rows<T, V, 256, 4>(p, stream);
 }
 
@@ -224,12 +229,22 @@ uint32_t read_width(const ReadParams& p, const elips_b200_cache& c) {
 template <class T, int V>
 void launch_read(ReadParams p, const elips_b200_cache& c, int num_sms, cudaStream_t stream) {
     p.per_group = FastDiv(static_cast<uint32_t>(c.dim) / V);
-    p.per_row = FastDiv(static_cast<uint32_t>(c.parts * c.heads) * p.per_group.d);
-    // About eight accesses a thread, and at least two blocks an SM.
-    uint64_t rows = std::min<uint64_t>(kReadRows, std::max<uint64_t>(1, 2048 / p.per_row.d));
+    p.per_row = static_cast<uint32_t>(c.parts * c.heads) * p.per_group.d;
+    // A thread per access of a row, up to 256, and as many rows side by side as
+    // leave the fewest threads of the last warp idle.
+    p.nx = std::min(p.per_row, 256u);
+    p.ny = 1;
+    uint32_t threads = cdiv(p.nx, 32) * 32;
+    for (uint32_t ny = 2; ny * p.nx <= 288; ++ny) {
+        const uint32_t with = cdiv(ny * p.nx, 32) * 32;
+        if (with < 128 || static_cast<uint64_t>(ny * p.nx) * threads >= static_cast<uint64_t>(p.ny * p.nx) * with) p.ny = ny, threads = with;
+    }
+    // Two batches of accesses a thread, and at least two blocks an SM.
+    uint64_t rows = std::min<uint64_t>(kReadRows, 2u * kReadBatch * p.ny);
     rows = std::min<uint64_t>(rows, cdiv(p.total, 2u * static_cast<uint32_t>(num_sms)));
     p.rows = static_cast<uint32_t>(rows);
-    cache_read_kernel<T, V><<<blocks_for(p.total, p.rows), 256, 0, stream>>>(p);
+    threads = std::max(threads, cdiv(p.rows, 32) * 32);
+    cache_read_kernel<T, V><<<blocks_for(p.total, p.rows), threads, 0, stream>>>(p);
 }
 
 void cache_read(int device, const elips_b200_cache& given, const void* table, int table64, int64_t table_stride, size_t sequences,

@@ -299,7 +299,8 @@ def cache_read(codes, scales, page_table, offsets, total: int, dtype=torch.bfloa
     ascending, one more entry than there are sequences, int32 or int64);
     position i of it is read from row i % page of page page_table[b, i // page]
     (int32 or int64 [sequences, width]). An entry that is no page of the cache,
-    or lies past the table's width, reads as zeros. `total` is the number of
+    or lies past the table's width, reads as zeros, as do rows in front of
+    offsets[0]. `total` is the number of
     output rows, offsets[-1] or more; rows behind the last sequence are zeros,
     or with `out` (a tuple of tensors like the result, of any strides but the
     last) stay as they are."""

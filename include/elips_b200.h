@@ -640,7 +640,8 @@ ELIPS_B200_API int elips_b200_cache_write(int device, const elips_b200_cache* ca
  * the sequence b with offsets[b] <= r < offsets[b + 1] (offsets ascending,
  * sequences + 1 entries) and is position i = r - offsets[b] of it, in page
  * page_table[b * table_stride + i / page_size]. A page that is no page of the
- * cache, or past the table's width, reads as zeros. Rows from
+ * cache, or past the table's width, reads as zeros, and so do rows in front
+ * of offsets[0]. Rows from
  * offsets[sequences] to `total` are zeroed where zero_behind, else left as
  * they are. */
 ELIPS_B200_API int elips_b200_cache_read(int device, const elips_b200_cache* cache, const void* page_table,

@@ -468,6 +468,34 @@ def test_cache_read_bad_pages_are_zeros(heads, dim):
     assert_read(got, codes, scales, table << 20, offsets, 50)
 
 
+@pytest.mark.parametrize("sequences", [255, 256, 257, 3000, 70000])
+def test_cache_read_many_sequences(sequences):
+    """More sequences than one step of the search looks at, many of them empty, the first not at row 0."""
+    from elips_b200 import int8
+    g = rng(sequences)
+    codes, scales = filled(g, 1, 40, 2, 1, 24)
+    offsets = 3 + np.concatenate([[0], np.cumsum(g.integers(0, 3, sequences))])
+    table = g.integers(0, 40, (sequences, 1))
+    total = int(offsets[-1]) + 5
+    got = int8.cache_read(codes, scales, torch.from_numpy(table).cuda().int(), torch.from_numpy(offsets).cuda(), total,
+                          torch.float32)[0].cpu()
+    seq = np.repeat(np.arange(sequences), np.diff(offsets))
+    pos = np.arange(3, offsets[-1]) - offsets[seq]
+    pg = torch.from_numpy(table[seq, 0])
+    want = codes[0].cpu()[pg, pos].float() * scales[0].cpu()[pg, pos][..., None]
+    assert torch.equal(got[3:-5], want) and (got[:3] == 0).all() and (got[-5:] == 0).all()
+
+
+@pytest.mark.parametrize("offsets", [[0, -5, 9], [7, 3, 1], [0, 1 << 40, 4], [-(1 << 40), 5, 9], [-(1 << 31) - 3, -7, 9]])
+def test_cache_read_offsets_that_do_not_ascend(offsets):
+    """Whatever they hold, every row read is a row of the cache or zeros."""
+    from elips_b200 import int8
+    codes, scales = new_cache(1, 3, 4, 1, 16, fill=1)
+    table = torch.tensor([[0, 1, 2], [2, 1, 0]], device="cuda")
+    got = int8.cache_read(codes, scales, table, torch.tensor(offsets, device="cuda"), 9, torch.float32)[0]
+    assert ((got == 1) | (got == 0)).all()
+
+
 def test_cache_read_nothing():
     from elips_b200 import int8
     codes, scales = filled(rng(1), 1, 2, 4, 1, 16)
