@@ -40,7 +40,7 @@ CODEC_SQ8 = 3
 
 
 class Cache(ctypes.Structure):
-    """elips_b200_cache."""
+    """elips_b200_cache (entry points take its address, or the same bytes packed)."""
     _fields_ = [("codes", c_void_p), ("scales", c_void_p), ("parts", c_int64), ("pages", c_int64),
                 ("page_size", c_int64), ("heads", c_int64), ("dim", c_int64), ("code_strides", c_int64 * 4),
                 ("scale_strides", c_int64 * 4)]
@@ -162,10 +162,10 @@ SIGNATURES = [
     ("elips_b200_linear_int8", c_int,
      [c_int, c_void_p, c_int, c_int64, c_void_p, c_size_t, c_void_p, c_void_p, c_int, c_size_t, c_size_t, c_size_t,
       c_void_p, c_int, c_size_t, c_void_p]),
-    ("elips_b200_cache_write", c_int, [c_int, POINTER(Cache), POINTER(Rows), c_int, c_size_t, c_void_p, c_int, c_void_p]),
+    ("elips_b200_cache_write", c_int, [c_int, c_void_p, c_void_p, c_int, c_size_t, c_void_p, c_int, c_void_p]),
     ("elips_b200_cache_read", c_int,
-     [c_int, POINTER(Cache), c_void_p, c_int, c_int64, c_size_t, c_size_t, c_void_p, c_int, c_size_t, POINTER(Rows),
-      c_int, c_int, c_void_p]),
+     [c_int, c_void_p, c_void_p, c_int, c_int64, c_size_t, c_size_t, c_void_p, c_int, c_size_t, c_void_p, c_int, c_int,
+      c_void_p]),
     ("elips_b200_profiler_enable", c_int, [c_int]),
     ("elips_b200_profiler_stats", c_int,
      [c_char_p, POINTER(ctypes.c_uint64), POINTER(ctypes.c_double), POINTER(ctypes.c_uint64)]),

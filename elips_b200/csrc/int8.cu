@@ -247,7 +247,7 @@ void launch_read(ReadParams p, const elips_b200_cache& c, int num_sms, cudaStrea
     cache_read_kernel<T, V><<<blocks_for(p.total, p.rows), threads, 0, stream>>>(p);
 }
 
-void cache_read(int device, const elips_b200_cache& given, const void* table, int table64, int64_t table_stride, size_t sequences,
+void cache_read(int num_sms, const elips_b200_cache& given, const void* table, int table64, int64_t table_stride, size_t sequences,
                 size_t table_width, const void* offsets, int offsets64, size_t total, const elips_b200_rows* out,
                 int type, int zero_behind, cudaStream_t stream) {
     const elips_b200_cache c = plain_strides(given);
@@ -269,7 +269,6 @@ void cache_read(int device, const elips_b200_cache& given, const void* table, in
     p.pages = static_cast<uint32_t>(c.pages);
     p.total = static_cast<uint32_t>(total);
     p.zero_behind = zero_behind;
-    const int num_sms = device_props(device).num_sms;
     Profiler::Scope prof("cache_read", stream, static_cast<uint64_t>(total) * static_cast<uint64_t>(c.parts * c.heads));
     with_float_type(type, [&](auto tag) {
         using T = decltype(tag);
@@ -311,45 +310,44 @@ void launch_dot(const GemmParams& p, int num_sms, cudaStream_t stream) {
     else gemm_int8_dot_kernel<8, T><<<blocks, 256, 0, stream>>>(p, wk);
 }
 
-template <int BT, class T>
-void launch_wide(const GemmParams& p, int num_sms, cudaStream_t stream) {
-    constexpr uint32_t stage_bytes = (kWideChannels + BT) * kGemmStageK;
+template <int BT, int S, class T>
+void launch_wide_split(const GemmParams& p, int num_sms, cudaStream_t stream) {
     const uint32_t n_ct = cdiv(p.n, kWideChannels), n_rt = cdiv(p.m, BT);
-    if (n_ct > 65535 || n_rt > 65535) bad("too many rows in one call");
-    const uint32_t kblocks = cdiv(p.k, kGemmStageK);
-    const uint64_t tiles = static_cast<uint64_t>(n_ct) * n_rt;
-    uint32_t splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= static_cast<uint64_t>(num_sms) * 2 && splits * 2 <= kblocks) splits *= 2;
-    const uint32_t per = std::max(1u, cdiv(kblocks, splits));
-    const uint32_t stages = std::min<uint32_t>(std::min<uint32_t>(kWideMaxStages, per), 196608u / stage_bytes);
-    const size_t smem = 1024 + std::max<size_t>(static_cast<size_t>(stages) * stage_bytes,
-                                                splits > 1 ? BT * kWideChannels * 4u : 0u);
+    constexpr uint32_t stage_bytes = (kWideChannels + BT) * kGemmStageK;
+    const uint32_t per = std::max(1u, cdiv(cdiv(p.k, kGemmStageK), S));
+    // All of k in flight where a CTA has an SM to itself. Several waves of CTAs
+    // run two or three to an SM, one's epilogue under another's loads (64 x
+    // 100,000 x 768: 29.6 us with six stages, 21.9 with three), and clusters of
+    // eight find room on every GPC only at two to an SM.
+    const bool shared = S == 8 || static_cast<uint64_t>(n_ct) * n_rt * S > static_cast<uint64_t>(num_sms);
+    uint32_t stages = std::min<uint32_t>(per, shared ? std::max(3u, 92160u / stage_bytes) : 196608u / stage_bytes);
+    stages = std::min<uint32_t>(stages, kWideMaxStages);
+    const size_t smem = 1024 + std::max<size_t>(static_cast<size_t>(stages) * stage_bytes, S > 1 ? BT * kWideChannels * 4u : 0u);
     const CUtensorMap mw = code_map(p.b, p.b_pitch, p.n, p.k, kWideChannels);
     const CUtensorMap mx = code_map(p.a, p.a_pitch, p.m, p.k, BT);
-    allow_dynamic_smem(reinterpret_cast<const void*>(gemm_int8_wide_kernel<BT, T>), smem);
+    allow_dynamic_smem(reinterpret_cast<const void*>(gemm_int8_wide_kernel<BT, S, T>), smem);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(splits, n_ct, n_rt);
+    cfg.gridDim = dim3(S, n_ct, n_rt);
     cfg.blockDim = dim3(kWideThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = splits;
+    attr[0].val.clusterDim.x = S;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = splits > 1 ? 1 : 0;
-    check_cuda(cudaLaunchKernelEx(&cfg, gemm_int8_wide_kernel<BT, T>, mw, mx, p, stages, splits),
+    cfg.numAttrs = S > 1 ? 1 : 0;
+    check_cuda(cudaLaunchKernelEx(&cfg, gemm_int8_wide_kernel<BT, S, T>, mw, mx, p, stages),
                ELIPS_B200_KERNEL_LAUNCH_FAILED, "int8 product launch");
 }
 
-template <class T>
-CUtensorMapDataType map_type();
-template <>
-CUtensorMapDataType map_type<float>() { return CU_TENSOR_MAP_DATA_TYPE_FLOAT32; }
-template <>
-CUtensorMapDataType map_type<__half>() { return CU_TENSOR_MAP_DATA_TYPE_FLOAT16; }
-template <>
-CUtensorMapDataType map_type<__nv_bfloat16>() { return CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; }
+template <int BT, class T>
+void launch_wide(const GemmParams& p, int num_sms, uint32_t splits, cudaStream_t stream) {
+    if (splits == 1) launch_wide_split<BT, 1, T>(p, num_sms, stream);
+    else if (splits == 2) launch_wide_split<BT, 2, T>(p, num_sms, stream);
+    else if (splits == 4) launch_wide_split<BT, 4, T>(p, num_sms, stream);
+    else launch_wide_split<BT, 8, T>(p, num_sms, stream);
+}
 
 template <class T>
 void launch_pair(const GemmParams& p, int num_sms, cudaStream_t stream) {
@@ -357,18 +355,13 @@ void launch_pair(const GemmParams& p, int num_sms, cudaStream_t stream) {
     if (static_cast<uint64_t>(n_mt) * n_nt > 0x7FFFFFFFull) bad("too many rows in one call");
     const CUtensorMap ma = code_map(p.a, p.a_pitch, p.m, p.k, kPairM / 2);
     const CUtensorMap mb = code_map(p.b, p.b_pitch, p.n, p.k, kPairN / 2);
-    const int64_t out_bytes = p.out_pitch * static_cast<int64_t>(sizeof(T));
-    const bool tma_out = on_16(p.out, out_bytes, p.m);
-    CUtensorMap mo{};
-    if (tma_out)
-        mo = make_operand_map(p.out, map_type<T>(), sizeof(T), p.n, p.m, 32,
-                              map_pitch(out_bytes, static_cast<uint64_t>(p.n) * sizeof(T), p.m));
-    allow_dynamic_smem(reinterpret_cast<const void*>(gemm_int8_pair_kernel<T>), kPairSmemBytes);
+    constexpr uint32_t smem = kPairSmemBytes;
+    allow_dynamic_smem(reinterpret_cast<const void*>(gemm_int8_pair_kernel<T>), smem);
     const uint32_t pairs = std::min<uint32_t>(n_mt * n_nt, static_cast<uint32_t>(num_sms) / 2);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(pairs * 2);
     cfg.blockDim = dim3(kPairThreads);
-    cfg.dynamicSmemBytes = kPairSmemBytes;
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -376,24 +369,69 @@ void launch_pair(const GemmParams& p, int num_sms, cudaStream_t stream) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    check_cuda(cudaLaunchKernelEx(&cfg, gemm_int8_pair_kernel<T>, ma, mb, mo, p, n_mt, n_nt, tma_out ? 1 : 0),
+    check_cuda(cudaLaunchKernelEx(&cfg, gemm_int8_pair_kernel<T>, ma, mb, p, n_mt, n_nt),
                ELIPS_B200_KERNEL_LAUNCH_FAILED, "int8 product launch");
+}
+
+// The form a product takes: rows per tile of the wide kernel (0: the pair
+// kernel, 1: the dot kernel) and how many CTAs split k.
+struct GemmForm {
+    uint32_t rows = 0, splits = 1;
+};
+
+// The dot kernel is for single tokens: its dp4a takes over from the loads at
+// about 2^25 products (device times, bf16 out: 1 x 4096 x 4096 5.3 us and wide
+// 7.0, 4 x 2048 x 2048 3.1 and 4.6, 4 x 4096 x 4096 8.5 and 7.1). Between the
+// others the least time that a simple model gives, in us, from what was
+// measured over sizes from 16 x 1024 x 1024 to 8192^3:
+//  * wide: 4 for the launch and its ends; a CTA loads 127 KB/us, four fifths
+//    of that when all SMs do; a cluster's summing costs 0.35 and 0.0145 a row;
+//    and each further tile that an SM gets after its first 2 more.
+//  * pair: 4.5 for the launch and its ends, then waves of tiles at 0.36 per
+//    128 of k (1670 T products/s, the tensor cores' pace at this power) + 1.2.
+// E.g. 512 x 4096 x 4096: wide of 128 rows 13.0 us, pair 16.6; 1024 x 4096 x
+// 4096: 23.4 and 17.2; 64 x 100,000 x 384 to fp32: 16.4 (64 rows) and 22.8.
+GemmForm gemm_form(uint32_t m, uint32_t n, uint32_t k, int num_sms) {
+    if (k > 0 && (m <= 2 || (m <= 8 && static_cast<uint64_t>(m) * n * k <= (1u << 25)))) return {1, 1};
+    const uint32_t kb = cdiv(k, kGemmStageK);
+    const double sms = num_sms;
+    GemmForm best{0, 1};
+    double least = 1e30;
+    if (kb > 0) {
+        const uint64_t tiles = static_cast<uint64_t>(cdiv(m, kPairM)) * cdiv(n, kPairN);
+        least = 4.5 + static_cast<double>((tiles + num_sms / 2 - 1) / (num_sms / 2)) * (kb * 0.36 + 1.2);
+    }
+    for (uint32_t rows = 16; rows <= 128; rows *= 2) {
+        const uint64_t tiles = static_cast<uint64_t>(cdiv(n, kWideChannels)) * cdiv(m, rows);
+        if (cdiv(n, kWideChannels) > 65535 || cdiv(m, rows) > 65535) continue;
+        const double per_kb = (kWideChannels + rows) * kGemmStageK / 127e3;
+        for (uint32_t splits = 1; splits <= 8; splits *= 2) {
+            if (splits > 1 && (tiles * splits > static_cast<uint64_t>(num_sms) || splits > kb)) break;
+            const double each = cdiv(kb, splits) * per_kb;
+            const double us = tiles <= static_cast<uint64_t>(num_sms)
+                                  ? 4 + each + (splits > 1 ? 0.35 + 0.0145 * rows : 0)
+                                  : 2 + tiles / sms * (1.25 * each + 2);
+            if (us < least) least = us, best = {rows, splits};
+        }
+        if (rows >= m) break;
+    }
+    return best;
 }
 
 template <class T>
 void launch_gemm(const GemmParams& p, int num_sms, cudaStream_t stream) {
-    if (p.m <= 2 && p.k > 0) launch_dot<T>(p, num_sms, stream);
-    else if (p.m > 256 && p.k > 0) launch_pair<T>(p, num_sms, stream);
-    else if (p.m <= 16) launch_wide<16, T>(p, num_sms, stream);
-    else if (p.m <= 32) launch_wide<32, T>(p, num_sms, stream);
-    else if (p.m <= 64) launch_wide<64, T>(p, num_sms, stream);
-    else launch_wide<128, T>(p, num_sms, stream);
+    GemmForm f = gemm_form(p.m, p.n, p.k, num_sms);
+    if (f.rows == 0) launch_pair<T>(p, num_sms, stream);
+    else if (f.rows == 1) launch_dot<T>(p, num_sms, stream);
+    else if (f.rows == 16) launch_wide<16, T>(p, num_sms, f.splits, stream);
+    else if (f.rows == 32) launch_wide<32, T>(p, num_sms, f.splits, stream);
+    else if (f.rows == 64) launch_wide<64, T>(p, num_sms, f.splits, stream);
+    else launch_wide<128, T>(p, num_sms, f.splits, stream);
     launch_ok("int8 product launch");
 }
 
-void gemm_int8(int device, GemmParams p, int out_type, cudaStream_t stream) {
+void gemm_int8(int num_sms, GemmParams p, int out_type, cudaStream_t stream) {
     if (p.m == 0 || p.n == 0) return;
-    const int num_sms = device_props(device).num_sms;
     // Operands whose rows do not start on 16 bytes are copied to rows that do:
     // one more pass over them.
     const bool a_ok = on_16(p.a, p.a_pitch, p.m), b_ok = on_16(p.b, p.b_pitch, p.n);
@@ -432,7 +470,7 @@ void check_gemm(size_t m, size_t n, size_t k, size_t b_pitch, const void* bias, 
 
 GemmParams gemm_params(const int8_t* a, size_t a_pitch, const float* a_scales, const int8_t* b, size_t b_pitch,
                        const float* b_scales, const void* bias, int bias_type, size_t m, size_t n, size_t k, void* out,
-                       size_t out_pitch) {
+                       int out_type, size_t out_pitch) {
     GemmParams p{};
     p.a = a;
     p.b = b;
@@ -447,10 +485,13 @@ GemmParams gemm_params(const int8_t* a, size_t a_pitch, const float* a_scales, c
     p.m = static_cast<uint32_t>(m);
     p.n = static_cast<uint32_t>(n);
     p.k = static_cast<uint32_t>(k);
+    const size_t size = out_type == ELIPS_B200_PRECISION_FP32 ? 4 : 2;
+    p.out_vec4 = reinterpret_cast<uintptr_t>(out) % (4 * size) == 0 && (m <= 1 || out_pitch % 4 == 0);
+    p.out_vec16 = on_16(out, static_cast<int64_t>(out_pitch * size), p.m);
     return p;
 }
 
-void linear_int8(int device, const void* x, int x_type, int64_t x_pitch, const int8_t* b, size_t b_pitch, const float* b_scales,
+void linear_int8(int num_sms, const void* x, int x_type, int64_t x_pitch, const int8_t* b, size_t b_pitch, const float* b_scales,
                  const void* bias, int bias_type, size_t m, size_t n, size_t k, void* out, int out_type,
                  size_t out_pitch, cudaStream_t stream) {
     if (m == 0 || n == 0) return;
@@ -460,7 +501,7 @@ void linear_int8(int device, const void* x, int x_type, int64_t x_pitch, const i
     int8_t* codes = reinterpret_cast<int8_t*>(s.get());
     float* scales = reinterpret_cast<float*>(s.get() + code_bytes);
     quantize_rows(x, x_type, m, k, x_pitch, codes, pitch, scales, stream);
-    gemm_int8(device, gemm_params(codes, pitch, scales, b, b_pitch, b_scales, bias, bias_type, m, n, k, out, out_pitch),
+    gemm_int8(num_sms, gemm_params(codes, pitch, scales, b, b_pitch, b_scales, bias, bias_type, m, n, k, out, out_type, out_pitch),
               out_type, stream);
 }
 
@@ -507,9 +548,8 @@ int elips_b200_gemm_int8(int device, const int8_t* a, size_t a_stride, const flo
         eb::check_gemm(m, n, k, b_stride, bias, bias_type, out_type, out_stride);
         if (a_stride < k) eb::bad("neighbouring matrix rows overlap");
         eb::DeviceGuard g(device);
-        eb::device_props(device);
-        eb::gemm_int8(device, eb::gemm_params(a, a_stride, a_scales, b, b_stride, b_scales, bias, bias_type, m, n, k, out,
-                                      out_stride),
+        eb::gemm_int8(eb::device_props(device).num_sms, eb::gemm_params(a, a_stride, a_scales, b, b_stride, b_scales, bias, bias_type, m, n, k, out,
+                                      out_type, out_stride),
                       out_type, eb::as_stream(stream));
     });
 }
@@ -523,8 +563,7 @@ int elips_b200_linear_int8(int device, const void* x, int x_type, int64_t x_stri
         eb::check_gemm(m, n, k, w_stride, bias, bias_type, out_type, out_stride);
         eb::check_rows(m, k, x_type);
         eb::DeviceGuard g(device);
-        eb::device_props(device);
-        eb::linear_int8(device, x, x_type, x_stride, w, w_stride, w_scales, bias, bias_type, m, n, k, out, out_type,
+        eb::linear_int8(eb::device_props(device).num_sms, x, x_type, x_stride, w, w_stride, w_scales, bias, bias_type, m, n, k, out, out_type,
                         out_stride, eb::as_stream(stream));
     });
 }
@@ -554,8 +593,7 @@ int elips_b200_cache_read(int device, const elips_b200_cache* cache, const void*
         if (total > 0 && sequences > 0 && offsets == nullptr) eb::bad("offsets missing");
         if (total > 0 && sequences > 0 && table_width > 0 && page_table == nullptr) eb::bad("page table missing");
         eb::DeviceGuard g(device);
-        eb::device_props(device);
-        eb::cache_read(device, *cache, page_table, table_64bit, table_stride, sequences, table_width, offsets, offsets_64bit,
+        eb::cache_read(eb::device_props(device).num_sms, *cache, page_table, table_64bit, table_stride, sequences, table_width, offsets, offsets_64bit,
                        total, out, type, zero_behind, eb::as_stream(stream));
     });
 }

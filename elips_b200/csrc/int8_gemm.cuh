@@ -124,24 +124,28 @@ __device__ __forceinline__ void land_loads(uint32_t full0, uint32_t issued_mask,
     }
 }
 
-__device__ __forceinline__ int32_t ld_cluster(uint32_t addr) {
-    int32_t v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ int4 ld_cluster(uint32_t addr) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr)
+                 : "memory");
     return v;
 }
 
-// One output tile of 128 channels x BT rows per cluster of `splits` CTAs
-// (grid: splits x channel tiles x row tiles). Each CTA sums its share of k in
-// TMEM. With one split a thread owns a channel and stores its column of the
-// tile straight from TMEM (a warp's stores of one row are neighbours); with
-// more, every CTA leaves its int32 tile in shared memory (over the pipeline's
-// buffers, which are done) and sums BT / splits rows over the cluster.
-template <int BT, class T>
+// One output tile of 128 channels x BT rows per cluster of S CTAs (grid: S x
+// channel tiles x row tiles). Each CTA sums its share of k in TMEM. With S = 1
+// a thread owns a channel and stores its column of the tile straight from TMEM
+// (a warp's stores of one row are neighbours); with more, every CTA leaves its
+// int32 tile in shared memory (over the pipeline's buffers, which are done) and
+// sums BT / S of the rows over the cluster, four channels a lane.
+template <int BT, int S, class T>
 static __global__ void __launch_bounds__(kWideThreads)
     gemm_int8_wide_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
-                          const __grid_constant__ GemmParams p, uint32_t stages, uint32_t splits) {
+                          const __grid_constant__ GemmParams p, uint32_t stages) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[2 * kWideMaxStages + 1];
+    __shared__ float row_scales[BT];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     volatile int* const abort_flag = &abort_word;
@@ -151,17 +155,19 @@ static __global__ void __launch_bounds__(kWideThreads)
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t sbase = (raw + 1023u) & ~1023u;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    const uint32_t split = blockIdx.x;  // = rank in the cluster
+    const uint32_t split = S == 1 ? 0u : blockIdx.x;  // = rank in the cluster
     const uint32_t n0 = blockIdx.y * kWideChannels, m0 = blockIdx.z * BT;
     const uint32_t kblocks = (p.k + kGemmStageK - 1u) / kGemmStageK;
-    const uint32_t kb0 = static_cast<uint32_t>(static_cast<uint64_t>(kblocks) * split / splits);
-    const uint32_t kb1 = static_cast<uint32_t>(static_cast<uint64_t>(kblocks) * (split + 1u) / splits);
+    const uint32_t kb0 = static_cast<uint32_t>(static_cast<uint64_t>(kblocks) * split / S);
+    const uint32_t kb1 = static_cast<uint32_t>(static_cast<uint64_t>(kblocks) * (split + 1u) / S);
     const uint32_t bar0 = smem_u32(bars);
     auto full = [&](uint32_t s) { return bar0 + 8u * s; };
     auto empty = [&](uint32_t s) { return bar0 + 8u * (kWideMaxStages + s); };
     const uint32_t done = bar0 + 8u * (2 * kWideMaxStages);
 
     if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tm_w);
+        tma_prefetch_desc(&tm_x);
         for (uint32_t s = 0; s < stages; ++s) {
             mbar_init(full(s), 1);
             mbar_init(empty(s), 1);
@@ -178,6 +184,21 @@ static __global__ void __launch_bounds__(kWideThreads)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+
+    // The scales and the bias arrive while the sums are made.
+    constexpr int kOwn = S == 1 ? 1 : 4;  // channels of a thread
+    const uint32_t row = (warp & 3u) * 32u + lane;  // TMEM lane = channel of the tile
+    const uint32_t n = n0 + (S == 1 ? row : lane * 4u);
+    float sb[kOwn], bias[kOwn];
+    if (warp >= 2) {
+        for (uint32_t r = threadIdx.x - 64u; r < BT; r += kWideThreads - 64u)
+            row_scales[r] = m0 + r < p.m ? p.a_scales[m0 + r] : 0.0f;
+    }
+#pragma unroll
+    for (int c = 0; c < kOwn; ++c) {
+        sb[c] = n + c < p.n ? p.b_scales[n + c] : 0.0f;
+        bias[c] = n + c < p.n && p.bias != nullptr ? bias_at(p.bias, p.bias_type, n + c) : 0.0f;
+    }
 
     if (warp == 0) {
         if (elect_one_sync()) {
@@ -222,18 +243,13 @@ static __global__ void __launch_bounds__(kWideThreads)
     // Every warp waits for the sums: after this no load and no MMA is under
     // way and the pipeline's buffers are free.
     const bool ok = finish_wait(done, 0) && *abort_flag == 0;
+    __syncthreads();  // row_scales
     tc_fence_after();
     T* const out = static_cast<T*>(p.out);
     if (warp >= 2) {
-        const uint32_t row = (warp & 3u) * 32u + lane;  // TMEM lane = channel of the tile
-        const uint32_t n = n0 + row;
         const uint32_t taddr = tmem + (((warp & 3u) * 32u) << 16);
-        const bool valid = n < p.n;
-        float sb = 0.0f, bias = 0.0f;
-        if (splits == 1 && valid) {
-            sb = p.b_scales[n];
-            if (p.bias != nullptr) bias = bias_at(p.bias, p.bias_type, n);
-        }
+        const uint32_t rows = ok && m0 < p.m && n < p.n ? min(static_cast<uint32_t>(BT), p.m - m0) : 0u;
+        T* dst = out + static_cast<int64_t>(m0) * p.out_pitch + n;
 #pragma unroll 1
         for (uint32_t c = 0; c < BT; c += 32) {
             uint32_t v[32];
@@ -244,19 +260,15 @@ static __global__ void __launch_bounds__(kWideThreads)
 #pragma unroll
                 for (uint32_t i = 0; i < 32; ++i) v[i] = 0;
             }
-            if (splits == 1) {
-                if (!ok) continue;
 #pragma unroll
-                for (uint32_t i = 0; i < 32; ++i) {
-                    const uint32_t m = m0 + c + i;
-                    if (c + i < BT && m < p.m && valid)
-                        out[m * p.out_pitch + n] = from_f32<T>(scaled(static_cast<int32_t>(v[i]), __ldg(p.a_scales + m), sb, bias));
+            for (uint32_t i = 0; i < (BT < 32 ? BT : 32); ++i) {
+                if constexpr (S == 1) {
+                    const T o = from_f32<T>(scaled(static_cast<int32_t>(v[i]), row_scales[c + i], sb[0], bias[0]));
+                    if (c + i < rows) *dst = o;
+                    dst += p.out_pitch;
+                } else {
+                    *reinterpret_cast<uint32_t*>(smem_raw + (sbase - raw) + ((c + i) * kWideChannels + row) * 4u) = v[i];
                 }
-            } else {
-#pragma unroll
-                for (uint32_t i = 0; i < 32; ++i)
-                    if (c + i < BT)
-                        *reinterpret_cast<uint32_t*>(smem_raw + (sbase - raw) + ((c + i) * kWideChannels + row) * 4u) = v[i];
             }
         }
     }
@@ -269,23 +281,34 @@ static __global__ void __launch_bounds__(kWideThreads)
         tc_fence_after();
         tmem_dealloc(tmem, kTmemCols);
     }
-    if (splits > 1) {
+    if constexpr (S > 1) {
         __syncwarp();
         cluster_sync();
-        // Rows r of the tile with r % splits == split, one warp per row and
-        // step, a lane on every 32nd channel.
-        for (uint32_t r = split + splits * warp; r < BT && m0 + r < p.m; r += splits * (kWideThreads / 32)) {
-            const float sa = p.a_scales[m0 + r];
+        // Rows r of the tile with r % S == split, one warp per row and step.
+        for (uint32_t r = split + S * warp; r < BT && m0 + r < p.m; r += S * (kWideThreads / 32)) {
+            const uint32_t at = sbase + (r * kWideChannels + lane * 4u) * 4u;
+            int4 part[S];
 #pragma unroll
-            for (uint32_t q = 0; q < kWideChannels / 32u; ++q) {
-                const uint32_t ch = q * 32u + lane, n = n0 + ch;
-                int32_t sum = 0;
-                for (uint32_t j = 0; j < splits; ++j)
-                    sum += ld_cluster(mapa_shared(sbase + (r * kWideChannels + ch) * 4u, j));
-                if (n < p.n) {
-                    const float bias = p.bias == nullptr ? 0.0f : bias_at(p.bias, p.bias_type, n);
-                    out[(m0 + r) * p.out_pitch + n] = from_f32<T>(scaled(sum, sa, p.b_scales[n], bias));
-                }
+            for (int j = 0; j < S; ++j) part[j] = ld_cluster(mapa_shared(at, j));
+            int32_t sum[4] = {};
+#pragma unroll
+            for (int j = 0; j < S; ++j) {
+                sum[0] += part[j].x;
+                sum[1] += part[j].y;
+                sum[2] += part[j].z;
+                sum[3] += part[j].w;
+            }
+            T o[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[c] = from_f32<T>(scaled(sum[c], row_scales[r], sb[c], bias[c]));
+            T* dst = out + static_cast<int64_t>(m0 + r) * p.out_pitch + n;
+            if (p.out_vec4 && n + 4u <= p.n) {
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(o);
+                else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (n + c < p.n) dst[c] = o[c];
             }
         }
         cluster_sync();  // the others may still read this CTA's sums
@@ -295,7 +318,7 @@ static __global__ void __launch_bounds__(kWideThreads)
 // ------------------------------------------------------------- pair kernel
 
 constexpr uint32_t kPairM = 256, kPairN = 256;
-constexpr uint32_t kPairStages = 5;
+constexpr uint32_t kPairStages = 5;  // four lose 5 % on 8192^3, six gain nothing
 constexpr uint32_t kPairEpilogueWarps = 8;
 constexpr int kPairThreads = 32 * (2 + kPairEpilogueWarps);
 constexpr uint32_t kPairStageBytes = (kPairM / 2 + kPairN / 2) * kGemmStageK;
@@ -305,19 +328,7 @@ constexpr uint32_t kPairColsOffset = kPairStoreOffset + kPairEpilogueWarps * kPa
 constexpr uint32_t kPairBarOffset = kPairColsOffset + kPairEpilogueWarps * (kPairN / 2) * 8;
 constexpr uint32_t kPairSmemBytes = 1024 + kPairBarOffset + 256;
 static_assert(8 * (2 * kPairStages + 5) + 16 <= 256, "barrier area");
-
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int32_t x, int32_t y) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
-                     reinterpret_cast<uint64_t>(map)),
-                 "r"(src), "r"(x), "r"(y)
-                 : "memory");
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-}
-
-// Until this thread's bulk stores have read their shared memory.
-__device__ __forceinline__ void tma_store_wait_read() {
-    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-}
+static_assert(kPairSmemBytes <= 232448, "shared memory");
 
 template <class T>
 struct Packed;
@@ -357,14 +368,13 @@ __device__ __forceinline__ void pair_tile(uint32_t i, uint32_t n_mt, uint32_t n_
 // Roles as in the search kernel: warp 0 loads, warp 1 of rank 0 issues the
 // pair's MMAs, eight warps empty one accumulator while the other fills. A
 // thread of the epilogue owns a row of a and half of the tile's columns; its
-// results go through 128-byte rows of shared memory to TMA stores, which drop
-// what lies outside the matrix, or, where the output's rows are no multiple
-// of 16 bytes, to plain stores.
+// results go through 128-byte rows of shared memory, so that a warp stores
+// whole lines, 16 bytes a lane (one element where the output's rows start
+// anywhere). The scales of the next tile are fetched under the current one.
 template <class T>
 static __global__ void __launch_bounds__(kPairThreads, 1)
     gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                          const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ GemmParams p,
-                          uint32_t n_mt, uint32_t n_nt, int tma_out) {
+                          const __grid_constant__ GemmParams p, uint32_t n_mt, uint32_t n_nt) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t sbase = (raw + 1023u) & ~1023u;
@@ -478,40 +488,51 @@ static __global__ void __launch_bounds__(kPairThreads, 1)
     } else {
         const uint32_t ew = warp - 2u, quad = warp & 3u, half = ew >> 2;
         constexpr uint32_t kHalf = kPairN / 2;
-        constexpr uint32_t kCols = 128 / sizeof(T);  // columns per store: 128 bytes of output
+        constexpr uint32_t kOwn = kHalf / 32;        // columns whose scales a lane fetches
+        constexpr uint32_t kCols = 128 / sizeof(T);  // columns per 128 bytes of output
         constexpr uint32_t kPer = Packed<T>::per_word;
-        const uint32_t store = sbase + kPairStoreOffset + ew * kPairStoreBytes;
-        uint8_t* const store_ptr = smem + kPairStoreOffset + ew * kPairStoreBytes;
+        uint8_t* const store = smem + kPairStoreOffset + ew * kPairStoreBytes;
         float2* const cols = reinterpret_cast<float2*>(smem + kPairColsOffset) + ew * kHalf;
         const uint32_t tempty0 = mapa_shared(tempty_bar(0), 0), tempty1 = mapa_shared(tempty_bar(1), 0);
+        T* const out = static_cast<T*>(p.out);
+        float sa = 0.0f;
+        float2 sb[kOwn];  // scale and bias
+        auto fetch = [&](uint32_t i) {
+            uint32_t mt, nt;
+            pair_tile(i, n_mt, n_nt, mt, nt);
+            const uint32_t m = mt * kPairM + rank * (kPairM / 2) + quad * 32u + lane;
+            sa = m < p.m ? __ldg(p.a_scales + m) : 0.0f;
+#pragma unroll
+            for (uint32_t j = 0; j < kOwn; ++j) {
+                const uint32_t n = nt * kPairN + half * kHalf + j * 32u + lane;
+                sb[j] = make_float2(0.0f, 0.0f);
+                if (n < p.n) {
+                    sb[j].x = __ldg(p.b_scales + n);
+                    if (p.bias != nullptr) sb[j].y = bias_at(p.bias, p.bias_type, n);
+                }
+            }
+        };
+        if (pair < tiles) fetch(pair);
         uint32_t iter = 0;
         for (uint32_t i = pair; i < tiles; i += pairs, ++iter) {
             uint32_t mt, nt;
             pair_tile(i, n_mt, n_nt, mt, nt);
             const uint32_t acc = iter & 1u;
             const uint32_t m_warp = mt * kPairM + rank * (kPairM / 2) + quad * 32u;
-            const uint32_t m = m_warp + lane;
             const uint32_t n_half = nt * kPairN + half * kHalf;
-            const float sa = m < p.m ? p.a_scales[m] : 0.0f;
-            for (uint32_t j = lane; j < kHalf; j += 32) {
-                const uint32_t n = n_half + j;
-                float2 c = make_float2(0.0f, 0.0f);
-                if (n < p.n) {
-                    c.x = p.b_scales[n];
-                    if (p.bias != nullptr) c.y = bias_at(p.bias, p.bias_type, n);
-                }
-                cols[j] = c;
-            }
+            const float row_scale = sa;
+#pragma unroll
+            for (uint32_t j = 0; j < kOwn; ++j) cols[j * 32u + lane] = sb[j];
+            if (i + pairs < tiles) fetch(i + pairs);
             __syncwarp();
             bool ok = mbar_wait(tfull_bar(acc), (iter >> 1) & 1u, abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
             const uint32_t taddr = tmem_base + ((quad * 32u) << 16) + acc * kPairN + half * kHalf;
+            const uint32_t rows = m_warp < p.m ? min(32u, p.m - m_warp) : 0u;
 #pragma unroll 1
             for (uint32_t c0 = 0; c0 < kHalf; c0 += kCols) {
-                if (lane == 0) tma_store_wait_read();  // the buffer's last store
-                __syncwarp();
 #pragma unroll
                 for (uint32_t h = 0; h < kCols; h += 32) {
                     uint32_t v[32];
@@ -521,53 +542,45 @@ static __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
                     for (uint32_t j = 0; j < 32; j += kPer) {
                         const float2 s0 = cols[c0 + h + j], s1 = cols[c0 + h + j + (kPer - 1)];
-                        w[j / kPer] = Packed<T>::pack(scaled(static_cast<int32_t>(v[j]), sa, s0.x, s0.y),
-                                                      scaled(static_cast<int32_t>(v[j + kPer - 1]), sa, s1.x, s1.y));
+                        w[j / kPer] = Packed<T>::pack(scaled(static_cast<int32_t>(v[j]), row_scale, s0.x, s0.y),
+                                                      scaled(static_cast<int32_t>(v[j + kPer - 1]), row_scale, s1.x, s1.y));
                     }
-                    // 128-byte rows with their 16-byte pieces swizzled as the
-                    // store's tensor map (or the plain reader) expects
+                    // 16-byte pieces of the 128-byte rows change places with
+                    // the row, so that neither side meets a bank conflict.
 #pragma unroll
                     for (uint32_t j = 0; j < 32 / kPer; j += 4) {
                         const uint32_t piece = h * sizeof(T) / 16u + j / 4u;
-                        *reinterpret_cast<uint4*>(store_ptr + lane * 128u + ((piece ^ (lane & 7u)) * 16u)) =
+                        *reinterpret_cast<uint4*>(store + lane * 128u + ((piece ^ (lane & 7u)) * 16u)) =
                             make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
                     }
                 }
-                if (c0 + kCols >= kHalf) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(acc ? tempty1 : tempty0);
-                }
+                if (c0 + kCols >= kHalf) tc_fence_before();
+                __syncwarp();
+                if (c0 + kCols >= kHalf && lane == 0) mbar_arrive_cluster(acc ? tempty1 : tempty0);
                 const uint32_t n = n_half + c0;
-                if (n >= p.n || m_warp >= p.m) {
-                    __syncwarp();
-                    continue;
-                }
-                if (tma_out) {
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) tma_store_2d(&tm_out, store, static_cast<int32_t>(n), static_cast<int32_t>(m_warp));
-                } else {
-                    __syncwarp();
-                    T* const out = static_cast<T*>(p.out);
-                    const uint32_t rows = min(32u, p.m - m_warp);
+                if (p.out_vec16 && n + kCols <= p.n) {
+                    T* dst = out + static_cast<int64_t>(m_warp + lane / 8u) * p.out_pitch + n + (lane & 7u) * (16u / sizeof(T));
+#pragma unroll
+                    for (uint32_t r = 0; r < 32; r += 4) {
+                        const uint32_t row = r + lane / 8u;
+                        const uint4 x = *reinterpret_cast<const uint4*>(store + row * 128u + (((lane & 7u) ^ (row & 7u)) * 16u));
+                        if (row < rows) *reinterpret_cast<uint4*>(dst) = x;
+                        dst += 4 * p.out_pitch;
+                    }
+                } else if (n < p.n) {
                     for (uint32_t r = 0; r < rows; ++r) {
 #pragma unroll
                         for (uint32_t q = 0; q < kCols; q += 32) {
                             const uint32_t byte = (q + lane) * sizeof(T), piece = (byte / 16u) ^ (r & 7u);
                             if (n + q + lane < p.n)
                                 out[(m_warp + r) * p.out_pitch + n + q + lane] =
-                                    *reinterpret_cast<const T*>(store_ptr + r * 128u + piece * 16u + byte % 16u);
+                                    *reinterpret_cast<const T*>(store + r * 128u + piece * 16u + byte % 16u);
                         }
                     }
-                    __syncwarp();
                 }
+                __syncwarp();
             }
         }
-        // The bulk stores have to be complete, not only read, before the CTA
-        // exits and its shared memory goes to another.
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        __syncwarp();
     }
 
     tc_fence_before();

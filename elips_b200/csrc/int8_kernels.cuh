@@ -530,6 +530,7 @@ struct GemmParams {
     void* out;
     int64_t out_pitch;  // elements
     uint32_t m, n, k;
+    int out_vec4, out_vec16;  // rows of out start on four elements, on 16 bytes
 };
 
 __device__ __forceinline__ float bias_at(const void* bias, int type, uint32_t n) {

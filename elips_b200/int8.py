@@ -31,7 +31,7 @@ touching any other row.
 from __future__ import annotations
 
 import contextlib
-import ctypes
+import struct
 
 import torch
 
@@ -41,48 +41,47 @@ from .exact import DimensionMismatch
 _LIB = capi.LIB
 _TYPES = {torch.float32: capi.PRECISION_FP32, torch.float16: capi.PRECISION_FP16,
           torch.bfloat16: capi.PRECISION_BF16}
-_INTS = (torch.int32, torch.int64)
+# elips_b200_cache and elips_b200_rows, packed: a call costs little more on the
+# host than its launch, and building ctypes structures would double that.
+_CACHE = struct.Struct("15q")
+_ROWS = (None, struct.Struct("3q"), struct.Struct("6q"))
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _device(first, *others) -> int:
-    """The CUDA device all tensors are on."""
-    dev = first.device
-    if dev.type != "cuda":
-        raise ValueError("tensors must be on a CUDA device")
-    for t in others:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
-    return dev.index
+def _refuse_grad() -> None:
+    raise ValueError("8-bit operators have no gradient: detach the inputs or use torch.no_grad()")
 
 
-def _no_grad(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("8-bit operators have no gradient: detach the inputs or use torch.no_grad()")
+def _refuse_devices(*tensors) -> None:
+    where = sorted({str(t.device) for t in tensors if t is not None})
+    raise ValueError("tensors must be on one CUDA device, not on " + " and ".join(where))
 
 
 def _float_type(dtype, what: str) -> int:
-    if dtype not in _TYPES:
+    kind = _TYPES.get(dtype)
+    if kind is None:
         raise ValueError(f"{what} must be float32, float16 or bfloat16, not {dtype}")
-    return _TYPES[dtype]
+    return kind
 
 
-def _matrix(t, dtype, what: str) -> None:
+def _pitch(t, what: str, apart: bool = True) -> int:
+    """Checks a matrix with contiguous rows; elements from one row to the next
+    (the width where there is no next). apart: rows must not overlap."""
     if t.dim() != 2:
         raise DimensionMismatch(f"{what} must have two axes")
-    if dtype is not None and t.dtype != dtype:
-        raise ValueError(f"{what} must be {dtype}, not {t.dtype}")
-    if t.stride(1) != 1 and t.shape[1] > 1:
-        raise ValueError(f"{what} must have its last axis contiguous")
+    rows, width = t.shape
+    pitch, step = t.stride()
+    if step != 1 and width > 1:
+        raise ValueError(f"{what} must have contiguous rows")
+    if rows < 2:
+        return width or 1
+    if apart and pitch < width:
+        raise ValueError(f"rows of {what} overlap")
+    return pitch
 
 
-def _pitch(t) -> int:
-    """Elements from one row to the next; the width where there is no next."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
-
-
-def _scales(t, n: int, what: str) -> None:
-    if t.dtype != torch.float32:
-        raise ValueError(f"{what} must be float32, not {t.dtype}")
+def _vector(t, n: int, what: str) -> None:
     if t.dim() != 1 or t.shape[0] != n:
         raise DimensionMismatch(f"{what} must have {n} entries")
     if n > 1 and t.stride(0) != 1:
@@ -105,61 +104,84 @@ def _using(stream, device: int, *tensors):
             t.record_stream(s)
 
 
-def _run(fn, stream, device: int, *tensors):
-    """fn(stream handle) on the caller's stream."""
-    if stream is None:
-        return fn(torch.cuda.current_stream(device).cuda_stream)
-    with _using(stream, device, *tensors):
-        return fn(_handle(stream))
-
-
 def quantize_rows(x, stream=None):
     """(codes int8 [n, d], scales float32 [n]) of float rows x [n, d]. The rows
     of codes start on multiples of 16 bytes (codes is a view of wider rows
     where d is no such multiple): gemm_int8 reads them as they are."""
-    _no_grad(x)
+    if x.requires_grad and torch.is_grad_enabled():
+        _refuse_grad()
     kind = _float_type(x.dtype, "rows")
-    _matrix(x, None, "rows")
+    pitch = _pitch(x, "rows", apart=False)
     n, d = x.shape
     if d == 0:
         raise DimensionMismatch("rows must have at least one value")
-    device = _device(x)
-
-    def go(s):
-        wide = -(-d // 16) * 16
-        codes = torch.empty((n, wide), dtype=torch.int8, device=x.device)
-        scales = torch.empty(n, dtype=torch.float32, device=x.device)
-        capi.check(_LIB.elips_b200_quantize_rows(device, x.data_ptr(), kind, n, d, _pitch(x), codes.data_ptr(), wide,
-                                                 scales.data_ptr(), s), "elips_b200_quantize_rows")
-        return codes[:, :d], scales
-
-    return _run(go, stream, device, x)
-
-
-def _target(out, m: int, n: int) -> None:
-    _matrix(out, None, "out")
-    if out.shape != (m, n):
-        raise DimensionMismatch(f"out must be {m} x {n}")
-    if m > 1 and out.stride(0) < n:
-        raise ValueError("rows of out overlap")
+    device = x.get_device()
+    if device < 0:
+        _refuse_devices(x)
+    if stream is not None:
+        with _using(stream, device, x):
+            return quantize_rows(x)
+    wide = -(-d // 16) * 16
+    codes = x.new_empty((n, wide), dtype=torch.int8)
+    scales = x.new_empty(n, dtype=torch.float32)
+    capi.check(_LIB.elips_b200_quantize_rows(device, x.data_ptr(), kind, n, d, pitch, codes.data_ptr(), wide,
+                                             scales.data_ptr(), _raw_stream(device)), "elips_b200_quantize_rows")
+    return (codes if wide == d else codes[:, :d]), scales
 
 
-def _weight(b, b_scales, bias, k: int) -> int:
-    """Checks the n x k operand, its scales and the bias; the bias type."""
-    _matrix(b, torch.int8, "weight codes")
+def _product(entry, name, x, x_kind, x_scales, b, b_scales, bias, dtype, out, stream):
+    """What gemm_int8 (x_kind None) and linear_int8 share: the checks of the
+    n x k operand, its scales, the bias and the output, and the call."""
+    pitch = _pitch(x, "rows", apart=x_kind is None)
+    m, k = x.shape
+    if b.dtype is not torch.int8:
+        raise ValueError(f"weight codes must be int8, not {b.dtype}")
+    b_pitch = _pitch(b, "weight codes")
+    n = b.shape[0]
     if b.shape[1] != k:
         raise DimensionMismatch(f"rows of {k} and of {b.shape[1]} values")
-    if b.shape[0] > 1 and b.stride(0) < k:
-        raise ValueError("weight rows overlap")
-    _scales(b_scales, b.shape[0], "weight scales")
-    if bias is None:
-        return 0
-    kind = _float_type(bias.dtype, "bias")
-    if bias.dim() != 1 or bias.shape[0] != b.shape[0]:
-        raise DimensionMismatch(f"bias must have {b.shape[0]} entries")
-    if bias.shape[0] > 1 and bias.stride(0) != 1:
-        raise ValueError("bias must be contiguous")
-    return kind
+    if b_scales.dtype is not torch.float32:
+        raise ValueError(f"scales must be float32, not {b_scales.dtype}")
+    _vector(b_scales, n, "weight scales")
+    if x_kind is None:
+        if x_scales.dtype is not torch.float32:
+            raise ValueError(f"scales must be float32, not {x_scales.dtype}")
+        _vector(x_scales, m, "row scales")
+    bias_ptr, bias_kind = None, 0
+    if bias is not None:
+        bias_kind = _float_type(bias.dtype, "bias")
+        _vector(bias, n, "bias")
+        bias_ptr = bias.data_ptr()
+    if out is not None:
+        dtype = out.dtype
+        if out.dim() != 2 or out.shape[0] != m or out.shape[1] != n:
+            raise DimensionMismatch(f"out must be {m} x {n}")
+        out_pitch = _pitch(out, "out")
+    kind = _float_type(dtype, "out")
+    if torch.is_grad_enabled() and (b_scales.requires_grad or x.requires_grad or
+                                    (x_scales is not None and x_scales.requires_grad) or
+                                    (bias is not None and bias.requires_grad) or (out is not None and out.requires_grad)):
+        _refuse_grad()
+    device = x.get_device()
+    if device < 0 or b.get_device() != device or b_scales.get_device() != device or \
+            (x_scales is not None and x_scales.get_device() != device) or \
+            (bias is not None and bias.get_device() != device) or (out is not None and out.get_device() != device):
+        _refuse_devices(x, b, x_scales, b_scales, bias, out)
+    if stream is not None:
+        with _using(stream, device, x, b, x_scales, b_scales, bias, out):
+            return _product(entry, name, x, x_kind, x_scales, b, b_scales, bias, dtype, out, None)
+    if out is None:
+        out = x.new_empty((m, n), dtype=dtype)
+        out_pitch = n or 1
+    if x_kind is None:
+        status = entry(device, x.data_ptr(), pitch, x_scales.data_ptr(), b.data_ptr(), b_pitch, b_scales.data_ptr(),
+                       bias_ptr, bias_kind, m, n, k, out.data_ptr(), kind, out_pitch, _raw_stream(device))
+    else:
+        status = entry(device, x.data_ptr(), x_kind, pitch, b.data_ptr(), b_pitch, b_scales.data_ptr(),
+                       bias_ptr, bias_kind, m, n, k, out.data_ptr(), kind, out_pitch, _raw_stream(device))
+    if status:
+        capi.check(status, name)
+    return out
 
 
 def gemm_int8(a, b, a_scales, b_scales, bias=None, out_dtype=torch.bfloat16, out=None, stream=None):
@@ -171,91 +193,76 @@ def gemm_int8(a, b, a_scales, b_scales, bias=None, out_dtype=torch.bfloat16, out
     queries and b stored rows. Operands whose rows start on multiples of 16
     bytes are read as they are, others are copied to such rows first. bias
     [n] may have another float type than out."""
-    _no_grad(a_scales, b_scales, bias, out)
-    kind = _float_type(out_dtype if out is None else out.dtype, "out")
-    _matrix(a, torch.int8, "row codes")
-    m, k = a.shape
-    if m > 1 and a.stride(0) < k:
-        raise ValueError("rows of codes overlap")
-    _scales(a_scales, m, "row scales")
-    bias_kind = _weight(b, b_scales, bias, k)
-    n = b.shape[0]
-    if out is not None:
-        _target(out, m, n)
-    device = _device(a, b, a_scales, b_scales, bias, out)
-
-    def go(s):
-        c = out if out is not None else torch.empty((m, n), dtype=out_dtype, device=a.device)
-        capi.check(_LIB.elips_b200_gemm_int8(
-            device, a.data_ptr(), _pitch(a), a_scales.data_ptr(), b.data_ptr(), _pitch(b), b_scales.data_ptr(),
-            None if bias is None else bias.data_ptr(), bias_kind, m, n, k, c.data_ptr(), kind, _pitch(c), s),
-            "elips_b200_gemm_int8")
-        return c
-
-    return _run(go, stream, device, a, b, a_scales, b_scales, bias, out)
+    if a.dtype is not torch.int8:
+        raise ValueError(f"row codes must be int8, not {a.dtype}")
+    return _product(_LIB.elips_b200_gemm_int8, "elips_b200_gemm_int8", a, None, a_scales, b, b_scales, bias, out_dtype,
+                    out, stream)
 
 
 def linear_int8(x, weight, weight_scales, bias=None, out_dtype=None, out=None, stream=None):
     """gemm_int8 over the rows of x [m, k], quantised on the way as
     quantize_rows quantises them; out_dtype defaults to x's type."""
-    _no_grad(x, weight_scales, bias, out)
     kind = _float_type(x.dtype, "rows")
-    _matrix(x, None, "rows")
-    m, k = x.shape
-    if k == 0:
+    if x.shape[-1:] == (0,):
         raise DimensionMismatch("rows must have at least one value")
-    bias_kind = _weight(weight, weight_scales, bias, k)
-    dtype = out.dtype if out is not None else out_dtype if out_dtype is not None else x.dtype
-    out_kind = _float_type(dtype, "out")
-    n = weight.shape[0]
-    if out is not None:
-        _target(out, m, n)
-    device = _device(x, weight, weight_scales, bias, out)
-
-    def go(s):
-        c = out if out is not None else torch.empty((m, n), dtype=dtype, device=x.device)
-        capi.check(_LIB.elips_b200_linear_int8(
-            device, x.data_ptr(), kind, _pitch(x), weight.data_ptr(), _pitch(weight), weight_scales.data_ptr(),
-            None if bias is None else bias.data_ptr(), bias_kind, m, n, k, c.data_ptr(), out_kind, _pitch(c), s),
-            "elips_b200_linear_int8")
-        return c
-
-    return _run(go, stream, device, x, weight, weight_scales, bias, out)
+    return _product(_LIB.elips_b200_linear_int8, "elips_b200_linear_int8", x, kind, None, weight, weight_scales, bias,
+                    x.dtype if out_dtype is None else out_dtype, out, stream)
 
 
-def _cache(codes, scales):
-    """The C description of a cache's two tensors."""
-    if codes.dtype != torch.int8 or scales.dtype != torch.float32:
+def _distinct(strides, shape, what: str) -> None:
+    """Refuses a tensor to be written whose elements share memory by a stride of 0."""
+    if 0 in strides and any(st == 0 and n > 1 for st, n in zip(strides, shape)):
+        raise ValueError(f"{what} must not be an expanded tensor")
+
+
+def _cache(codes, scales, written: bool):
+    """The packed elips_b200_cache of a cache's two tensors, and its shape."""
+    if codes.dtype is not torch.int8 or scales.dtype is not torch.float32:
         raise ValueError("a cache has int8 codes and float32 scales")
-    if codes.dim() != 5 or scales.shape != codes.shape[:4]:
+    shape, held = codes.shape, scales.shape
+    if len(shape) != 5 or held != shape[:4]:
         raise DimensionMismatch("codes must be [parts, pages, page, heads, dim] and scales [parts, pages, page, heads]")
-    parts, pages, page, heads, dim = codes.shape
+    parts, pages, page, heads, dim = shape
     if not 1 <= parts <= 2:
         raise DimensionMismatch("a cache has one or two parts")
     if page < 1 or heads < 1 or dim < 1:
         raise DimensionMismatch("pages, heads and rows must not be empty")
-    st = codes.stride()
-    if st[4] != 1 and dim > 1:
+    s0, s1, s2, s3, s4 = strides = codes.stride()
+    if s4 != 1 and dim > 1:
         raise ValueError("rows of codes must be contiguous")
-    return capi.Cache(codes.data_ptr(), scales.data_ptr(), parts, pages, page, heads, dim, st[:4], scales.stride())
+    t0, t1, t2, t3 = scale_strides = scales.stride()
+    if written:
+        _distinct(strides, shape, "codes")
+        _distinct(scale_strides, held, "scales")
+    return _CACHE.pack(codes.data_ptr(), scales.data_ptr(), parts, pages, page, heads, dim, s0, s1, s2, s3, t0, t1, t2,
+                       t3), parts, heads, dim
 
 
-def _distinct(t, what: str) -> None:
-    """Refuses a tensor to be written whose elements share memory by a stride of 0."""
-    if 0 in t.stride() and any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
-        raise ValueError(f"{what} must not be an expanded tensor")
-
-
-def _rows(tensors, count, heads: int, dim: int, dtype, what: str):
-    """The C description of a part's rows [count, heads, dim], for each part."""
+def _rows(tensors, count: int, heads: int, dim: int, dtype, what: str, written: bool):
+    """The packed elips_b200_rows of a part's rows [count, heads, dim], for each part."""
+    packed = []
     for x in tensors:
-        if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != dim or x.shape[0] != count:
-            raise DimensionMismatch(f"{what} must be [{count}, {heads}, {dim}], not {list(x.shape)}")
-        if x.dtype != dtype:
+        shape = x.shape
+        if len(shape) != 3 or shape[0] != count or shape[1] != heads or shape[2] != dim:
+            raise DimensionMismatch(f"{what} must be [{count}, {heads}, {dim}], not {list(shape)}")
+        if x.dtype is not dtype:
             raise ValueError(f"{what} must be {dtype}, not {x.dtype}")
-        if x.stride(2) != 1 and dim > 1:
+        s0, s1, s2 = strides = x.stride()
+        if s2 != 1 and dim > 1:
             raise ValueError(f"{what} must have their last axis contiguous")
-    return (capi.Rows * len(tensors))(*[(x.data_ptr(), x.stride(0), x.stride(1)) for x in tensors])
+        if written:
+            _distinct(strides, shape, what)
+        packed += (x.data_ptr(), s0, s1)
+    return _ROWS[len(tensors)].pack(*packed)
+
+
+def _indexes(t, what: str) -> int:
+    """1 for int64, 0 for int32."""
+    if t.dtype is torch.int64:
+        return 1
+    if t.dtype is not torch.int32:
+        raise ValueError(f"{what} must be int32 or int64, not {t.dtype}")
+    return 0
 
 
 def cache_write(codes, scales, rows, slots, stream=None) -> None:
@@ -268,27 +275,28 @@ def cache_write(codes, scales, rows, slots, stream=None) -> None:
     (int32 or int64): row s % page of page s // page. A slot below 0 or past
     the last one is skipped (padding); of a slot given twice the last row is
     kept. Slots that are not named stay as they are."""
-    rows = tuple(rows)
-    _no_grad(scales, *rows)
-    c = _cache(codes, scales)
-    _distinct(codes, "codes")
-    _distinct(scales, "scales")
-    if len(rows) != c.parts:
-        raise DimensionMismatch(f"{len(rows)} tensors of rows for a cache of {c.parts} parts")
-    if slots.dtype not in _INTS:
-        raise ValueError(f"slots must be int32 or int64, not {slots.dtype}")
+    cache, parts, heads, dim = _cache(codes, scales, True)
+    if len(rows) != parts:
+        raise DimensionMismatch(f"{len(rows)} tensors of rows for a cache of {parts} parts")
+    wide = _indexes(slots, "slots")
     if slots.dim() != 1 or (slots.shape[0] > 1 and slots.stride(0) != 1):
         raise DimensionMismatch("slots must be one contiguous axis")
     t = slots.shape[0]
-    kind = _float_type(rows[0].dtype, "rows")
-    r = _rows(rows, t, c.heads, c.dim, rows[0].dtype, "rows")
-    device = _device(codes, scales, slots, *rows)
-
-    def go(s):
-        capi.check(_LIB.elips_b200_cache_write(device, ctypes.byref(c), r, kind, t, slots.data_ptr(),
-                                               slots.dtype == torch.int64, s), "elips_b200_cache_write")
-
-    _run(go, stream, device, codes, scales, slots, *rows)
+    dtype = rows[0].dtype
+    kind = _float_type(dtype, "rows")
+    packed = _rows(rows, t, heads, dim, dtype, "rows", False)
+    if torch.is_grad_enabled() and (scales.requires_grad or rows[0].requires_grad or rows[-1].requires_grad):
+        _refuse_grad()
+    device = codes.get_device()
+    if device < 0 or scales.get_device() != device or slots.get_device() != device or \
+            rows[0].get_device() != device or rows[-1].get_device() != device:
+        _refuse_devices(codes, scales, slots, *rows)
+    if stream is not None:
+        with _using(stream, device, codes, scales, slots, *rows):
+            return cache_write(codes, scales, rows, slots)
+    status = _LIB.elips_b200_cache_write(device, cache, packed, kind, t, slots.data_ptr(), wide, _raw_stream(device))
+    if status:
+        capi.check(status, "elips_b200_cache_write")
 
 
 def cache_read(codes, scales, page_table, offsets, total: int, dtype=torch.bfloat16, out=None, stream=None):
@@ -300,42 +308,44 @@ def cache_read(codes, scales, page_table, offsets, total: int, dtype=torch.bfloa
     position i of it is read from row i % page of page page_table[b, i // page]
     (int32 or int64 [sequences, width]). An entry that is no page of the cache,
     or lies past the table's width, reads as zeros, as do rows in front of
-    offsets[0]. `total` is the number of
-    output rows, offsets[-1] or more; rows behind the last sequence are zeros,
-    or with `out` (a tuple of tensors like the result, of any strides but the
-    last) stay as they are."""
-    out = None if out is None else tuple(out)
-    _no_grad(scales, *(out or ()))
-    c = _cache(codes, scales)
-    if page_table.dtype not in _INTS or offsets.dtype not in _INTS:
-        raise ValueError("page_table and offsets must be int32 or int64")
+    offsets[0]. `total` is the number of output rows, offsets[-1] or more; rows
+    behind the last sequence are zeros, or with `out` (a tuple of tensors like
+    the result, of any strides but the last) stay as they are."""
+    cache, parts, heads, dim = _cache(codes, scales, False)
+    table_wide, offsets_wide = _indexes(page_table, "page_table"), _indexes(offsets, "offsets")
     if page_table.dim() != 2 or offsets.dim() != 1 or offsets.shape[0] != page_table.shape[0] + 1:
         raise DimensionMismatch("offsets must have one entry more than page_table has rows")
-    if (page_table.shape[1] > 1 and page_table.stride(1) != 1) or (offsets.shape[0] > 1 and offsets.stride(0) != 1):
+    sequences, width = page_table.shape
+    table_stride, step = page_table.stride()
+    if (width > 1 and step != 1) or (sequences > 0 and offsets.stride(0) != 1):
         raise ValueError("page_table rows and offsets must be contiguous")
     total = int(total)
     if total < 0:
         raise DimensionMismatch("total must not be negative")
-    if out is not None:
-        if len(out) != c.parts:
-            raise DimensionMismatch(f"{len(out)} outputs for a cache of {c.parts} parts")
+    fresh = out is None
+    if not fresh:
+        out = tuple(out)
+        if len(out) != parts:
+            raise DimensionMismatch(f"{len(out)} outputs for a cache of {parts} parts")
         dtype = out[0].dtype
-        for x in out:
-            _distinct(x, "out")
-        given = _rows(out, total, c.heads, c.dim, dtype, "out")
+        packed = _rows(out, total, heads, dim, dtype, "out", True)
     kind = _float_type(dtype, "out")
-    device = _device(codes, scales, page_table, offsets, *(out or ()))
-
-    def go(s):
-        if out is not None:
-            res, r = out, given
-        else:
-            res = tuple(torch.empty((total, c.heads, c.dim), dtype=dtype, device=codes.device) for _ in range(c.parts))
-            r = _rows(res, total, c.heads, c.dim, dtype, "out")
-        capi.check(_LIB.elips_b200_cache_read(
-            device, ctypes.byref(c), page_table.data_ptr(), page_table.dtype == torch.int64, page_table.stride(0),
-            page_table.shape[0], page_table.shape[1], offsets.data_ptr(), offsets.dtype == torch.int64, total, r,
-            kind, out is None, s), "elips_b200_cache_read")
-        return res
-
-    return _run(go, stream, device, codes, scales, page_table, offsets, *(out or ()))
+    if torch.is_grad_enabled() and (scales.requires_grad or (not fresh and any(x.requires_grad for x in out))):
+        _refuse_grad()
+    device = codes.get_device()
+    if device < 0 or scales.get_device() != device or page_table.get_device() != device or \
+            offsets.get_device() != device or (not fresh and any(x.get_device() != device for x in out)):
+        _refuse_devices(codes, scales, page_table, offsets, *(out or ()))
+    if stream is not None:
+        with _using(stream, device, codes, scales, page_table, offsets, *(out or ())):
+            return cache_read(codes, scales, page_table, offsets, total, dtype, out)
+    if fresh:
+        out = tuple(codes.new_empty((total, heads, dim), dtype=dtype) for _ in range(parts))
+        first = (heads * dim, dim)
+        packed = _ROWS[parts].pack(*(v for x in out for v in (x.data_ptr(), *first)))
+    status = _LIB.elips_b200_cache_read(device, cache, page_table.data_ptr(), table_wide, table_stride, sequences, width,
+                                        offsets.data_ptr(), offsets_wide, total, packed, kind, fresh,
+                                        _raw_stream(device))
+    if status:
+        capi.check(status, "elips_b200_cache_read")
+    return out
