@@ -59,6 +59,7 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
 
 const DeviceProps& device_props(int device) {
     std::lock_guard<std::mutex> lock(g_props_mu);
+    if (device >= 0 && static_cast<size_t>(device) < g_props.size() && g_props_ready[device]) return g_props[device];
     int count = 0;
     if (cudaGetDeviceCount(&count) != cudaSuccess || device < 0 || device >= count)
         fail(ELIPS_B200_DEVICE_NOT_FOUND, "no such CUDA device");

@@ -57,11 +57,45 @@ void with_float_type(int type, Fn&& fn) {
     }
 }
 
+// A launch with attributes.
+struct LaunchConfig {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[2];
+    LaunchConfig(dim3 grid, uint32_t threads, size_t smem, cudaStream_t stream) {
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        cfg.attrs = attr;
+    }
+    void clusters_of(uint32_t x) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = x;
+        attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
+    // The kernel waits for the previous one of the call itself (await_previous).
+    void after_previous() {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++cfg.numAttrs;
+    }
+    template <class... K, class... A>
+    void launch(void (*kernel)(K...), A&&... args) {
+        check_cuda(cudaLaunchKernelEx(&cfg, kernel, static_cast<K>(args)...), ELIPS_B200_KERNEL_LAUNCH_FAILED, "kernel launch");
+    }
+};
+
 template <class T, int V, int G, int NV>
 void launch_rows(const QuantParams& p, cudaStream_t stream) {
     const uint32_t blocks = blocks_for(p.groups, 256 / G);
-    if (p.slots != nullptr) quantize_rows_kernel<T, V, G, NV, true><<<blocks, 256, 0, stream>>>(p);
-    else quantize_rows_kernel<T, V, G, NV, false><<<blocks, 256, 0, stream>>>(p);
+    if (p.slots == nullptr) {
+        quantize_rows_kernel<T, V, G, NV, false><<<blocks, 256, 0, stream>>>(p);
+        return;
+    }
+    LaunchConfig cfg(dim3(blocks), 256, 0, stream);
+    if (p.dup == kDupClaim && p.t0 == 0) cfg.after_previous();
+    cfg.launch(quantize_rows_kernel<T, V, G, NV, true>, p);
 }
 
 // Few threads with many accesses each: what a thread spends on finding its row
@@ -198,12 +232,12 @@ void cache_write(const elips_b200_cache& given, const elips_b200_rows* rows, int
     p.per_t = FastDiv(parts * p.heads);
     p.dup = t == 1 ? kDupNone : t <= kDupScanRows ? kDupScan : kDupClaim;
     const uint64_t items = static_cast<uint64_t>(t) * p.per_t.d;
-    for (int clear = 1; p.dup == kDupClaim && clear >= 0; --clear) {
+    if (p.dup == kDupClaim) {
         Profiler::Scope prof("cache_claim", stream, items);
         in_runs(t, p.per_t.d, [&](uint32_t t0, uint32_t groups) {
             p.t0 = t0;
             p.groups = groups;
-            cache_claim_kernel<<<blocks_for(groups, 256), 256, 0, stream>>>(p, clear);
+            cache_claim_kernel<<<blocks_for(groups, 256), 256, 0, stream>>>(p);
         });
         launch_ok("cache claim launch");
     }
@@ -297,17 +331,23 @@ CUtensorMap code_map(const int8_t* codes, int64_t pitch, uint32_t rows, uint32_t
     return make_operand_map(codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, k, rows, box_rows, map_pitch(pitch, k, rows));
 }
 
-template <class T>
-void launch_dot(const GemmParams& p, int num_sms, cudaStream_t stream) {
+template <int MR, class X, class T>
+void launch_dot_rows(const GemmParams& p, int num_sms, cudaStream_t stream) {
     // Warps that split k between them until every SM has sixteen.
     const uint64_t groups = cdiv(p.n, kDotChannels);
     uint32_t wk = 1;
     while (wk < 8 && groups * wk < static_cast<uint64_t>(num_sms) * 16 && p.k > wk * 512u) wk *= 2;
-    const uint32_t blocks = blocks_for(groups * wk, 8);
-    if (p.m == 1) gemm_int8_dot_kernel<1, T><<<blocks, 256, 0, stream>>>(p, wk);
-    else if (p.m == 2) gemm_int8_dot_kernel<2, T><<<blocks, 256, 0, stream>>>(p, wk);
-    else if (p.m <= 4) gemm_int8_dot_kernel<4, T><<<blocks, 256, 0, stream>>>(p, wk);
-    else gemm_int8_dot_kernel<8, T><<<blocks, 256, 0, stream>>>(p, wk);
+    const size_t smem = std::is_same<X, int8_t>::value ? 0 : static_cast<size_t>(p.m) * ((p.k + 15u) / 16u * 16u);
+    gemm_int8_dot_kernel<MR, X, T><<<blocks_for(groups * wk, 8), 256, smem, stream>>>(p, wk);
+    launch_ok("int8 product launch");
+}
+
+template <class X, class T>
+void launch_dot(const GemmParams& p, int num_sms, cudaStream_t stream) {
+    if (p.m == 1) launch_dot_rows<1, X, T>(p, num_sms, stream);
+    else if (p.m == 2) launch_dot_rows<2, X, T>(p, num_sms, stream);
+    else if (p.m <= 4) launch_dot_rows<4, X, T>(p, num_sms, stream);
+    else launch_dot_rows<8, X, T>(p, num_sms, stream);
 }
 
 template <int BT, int S, class T>
@@ -326,19 +366,10 @@ void launch_wide_split(const GemmParams& p, int num_sms, cudaStream_t stream) {
     const CUtensorMap mw = code_map(p.b, p.b_pitch, p.n, p.k, kWideChannels);
     const CUtensorMap mx = code_map(p.a, p.a_pitch, p.m, p.k, BT);
     allow_dynamic_smem(reinterpret_cast<const void*>(gemm_int8_wide_kernel<BT, S, T>), smem);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(S, n_ct, n_rt);
-    cfg.blockDim = dim3(kWideThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = S;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = S > 1 ? 1 : 0;
-    check_cuda(cudaLaunchKernelEx(&cfg, gemm_int8_wide_kernel<BT, S, T>, mw, mx, p, stages),
-               ELIPS_B200_KERNEL_LAUNCH_FAILED, "int8 product launch");
+    LaunchConfig cfg(dim3(S, n_ct, n_rt), kWideThreads, smem, stream);
+    if (S > 1) cfg.clusters_of(S);
+    if (p.after_previous) cfg.after_previous();
+    cfg.launch(gemm_int8_wide_kernel<BT, S, T>, mw, mx, p, stages);
 }
 
 template <int BT, class T>
@@ -358,19 +389,10 @@ void launch_pair(const GemmParams& p, int num_sms, cudaStream_t stream) {
     constexpr uint32_t smem = kPairSmemBytes;
     allow_dynamic_smem(reinterpret_cast<const void*>(gemm_int8_pair_kernel<T>), smem);
     const uint32_t pairs = std::min<uint32_t>(n_mt * n_nt, static_cast<uint32_t>(num_sms) / 2);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(pairs * 2);
-    cfg.blockDim = dim3(kPairThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    check_cuda(cudaLaunchKernelEx(&cfg, gemm_int8_pair_kernel<T>, ma, mb, p, n_mt, n_nt),
-               ELIPS_B200_KERNEL_LAUNCH_FAILED, "int8 product launch");
+    LaunchConfig cfg(dim3(pairs * 2), kPairThreads, smem, stream);
+    cfg.clusters_of(2);
+    if (p.after_previous) cfg.after_previous();
+    cfg.launch(gemm_int8_pair_kernel<T>, ma, mb, p, n_mt, n_nt);
 }
 
 // The form a product takes: rows per tile of the wide kernel (0: the pair
@@ -422,7 +444,7 @@ template <class T>
 void launch_gemm(const GemmParams& p, int num_sms, cudaStream_t stream) {
     GemmForm f = gemm_form(p.m, p.n, p.k, num_sms);
     if (f.rows == 0) launch_pair<T>(p, num_sms, stream);
-    else if (f.rows == 1) launch_dot<T>(p, num_sms, stream);
+    else if (f.rows == 1) launch_dot<int8_t, T>(p, num_sms, stream);
     else if (f.rows == 16) launch_wide<16, T>(p, num_sms, f.splits, stream);
     else if (f.rows == 32) launch_wide<32, T>(p, num_sms, f.splits, stream);
     else if (f.rows == 64) launch_wide<64, T>(p, num_sms, f.splits, stream);
@@ -446,16 +468,29 @@ void gemm_int8(int num_sms, GemmParams p, int out_type, cudaStream_t stream) {
         return;
     }
     StreamScratch s(a_bytes + b_bytes, stream);
-    auto repack = [&](const int8_t*& codes, int64_t& from, uint32_t rows, uint8_t* to) {
-        Profiler::Scope prof("repack_codes", stream, rows);
-        repack_codes_kernel<<<blocks_for(static_cast<uint64_t>(rows) * (pitch / 4), 256), 256, 0, stream>>>(
-            codes, from, reinterpret_cast<int8_t*>(to), static_cast<uint32_t>(pitch), rows, p.k);
+    {
+        Profiler::Scope prof("repack_codes", stream, (a_ok ? 0u : p.m) + static_cast<uint64_t>(b_ok ? 0u : p.n));
+        RepackParams r{};
+        r.k = p.k;
+        r.words = FastDiv(static_cast<uint32_t>(pitch / 4));
+        uint32_t count = 0;
+        uint64_t most = 0;
+        auto add = [&](const int8_t*& codes, int64_t& from, uint32_t rows, uint8_t* to) {
+            r.in[count] = codes;
+            r.in_pitch[count] = from;
+            r.rows[count] = rows;
+            r.out[count] = reinterpret_cast<int8_t*>(to);
+            most = std::max<uint64_t>(most, rows * (pitch / 4));
+            codes = r.out[count++];
+            from = static_cast<int64_t>(pitch);
+        };
+        if (!a_ok) add(p.a, p.a_pitch, p.m, s.get());
+        if (!b_ok) add(p.b, p.b_pitch, p.n, s.get() + a_bytes);
+        const uint32_t blocks = static_cast<uint32_t>(std::min<uint64_t>((most + 255) / 256, 1u << 20));
+        repack_codes_kernel<<<dim3(blocks, count), 256, 0, stream>>>(r);
         launch_ok("operand copy launch");
-        codes = reinterpret_cast<const int8_t*>(to);
-        from = static_cast<int64_t>(pitch);
-    };
-    if (!a_ok) repack(p.a, p.a_pitch, p.m, s.get());
-    if (!b_ok) repack(p.b, p.b_pitch, p.n, s.get() + a_bytes);
+    }
+    p.after_previous = 1;
     product();
 }
 
@@ -496,13 +531,29 @@ void linear_int8(int num_sms, const void* x, int x_type, int64_t x_pitch, const 
                  size_t out_pitch, cudaStream_t stream) {
     if (m == 0 || n == 0) return;
     const size_t pitch = (k + 15) / 16 * 16;
+    // Few values: the dot kernel quantises them itself.
+    if (gemm_form(static_cast<uint32_t>(m), static_cast<uint32_t>(n), static_cast<uint32_t>(k), num_sms).rows == 1 &&
+        m * pitch <= kDotCodeBytes && on_16(b, static_cast<int64_t>(b_pitch), static_cast<uint32_t>(n))) {
+        GemmParams p = gemm_params(nullptr, pitch, nullptr, b, b_pitch, b_scales, bias, bias_type, m, n, k, out, out_type,
+                                   out_pitch);
+        p.x = x;
+        p.x_pitch = m > 1 ? x_pitch : 0;
+        Profiler::Scope prof("linear_int8", stream, static_cast<uint64_t>(m) * n);
+        with_float_type(x_type, [&](auto xt) {
+            using X = decltype(xt);
+            p.x_vec16 = on_16(x, x_pitch * static_cast<int64_t>(sizeof(X)), p.m) && k % (16 / sizeof(X)) == 0;
+            with_float_type(out_type, [&](auto tag) { launch_dot<X, decltype(tag)>(p, num_sms, stream); });
+        });
+        return;
+    }
     const size_t code_bytes = (m * pitch + 255) / 256 * 256;
     StreamScratch s(code_bytes + m * sizeof(float), stream);
     int8_t* codes = reinterpret_cast<int8_t*>(s.get());
     float* scales = reinterpret_cast<float*>(s.get() + code_bytes);
     quantize_rows(x, x_type, m, k, x_pitch, codes, pitch, scales, stream);
-    gemm_int8(num_sms, gemm_params(codes, pitch, scales, b, b_pitch, b_scales, bias, bias_type, m, n, k, out, out_type, out_pitch),
-              out_type, stream);
+    GemmParams p = gemm_params(codes, pitch, scales, b, b_pitch, b_scales, bias, bias_type, m, n, k, out, out_type, out_pitch);
+    p.after_previous = 1;
+    gemm_int8(num_sms, p, out_type, stream);
 }
 
 cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }

@@ -31,22 +31,78 @@ __device__ __forceinline__ float scaled(int32_t acc, float sa, float sb, float b
 // -------------------------------------------------------------- a few rows
 
 constexpr int kDotChannels = 4;  // weight rows per warp and step
+constexpr uint32_t kDotCodeBytes = 32768;  // most codes of quantised rows in shared memory
+
+// The block's quantisation of MR rows (m of them there) to codes in shared
+// memory, padded with zeros to `pitch` bytes: 8 / MR warps a row.
+template <int MR, class X, int V>
+__device__ __forceinline__ void dot_quantize(const GemmParams& p, int8_t* codes, uint32_t pitch, uint32_t* warp_max,
+                                             float* scales) {
+    constexpr uint32_t kWarps = 8 / MR, kThreads = kWarps * 32;
+    const uint32_t row = threadIdx.x / kThreads, tid = threadIdx.x % kThreads;
+    const bool there = row < p.m;
+    const X* x = static_cast<const X*>(p.x) + (there ? row : 0u) * p.x_pitch;
+    uint32_t top = 0;
+    for (uint32_t e = tid * V; e < p.k; e += kThreads * V) {
+        Access<X, V> u;
+        u.load(x + e);
+        top = u.top(top);
+    }
+    const uint32_t top32 = __reduce_max_sync(0xFFFFFFFFu, Access<X, V>::bits32(top));
+    if ((threadIdx.x & 31u) == 0) warp_max[threadIdx.x >> 5] = top32;
+    __syncthreads();
+    uint32_t amax = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kWarps; ++i) amax = max(amax, warp_max[row * kWarps + i]);
+    const RowScale rs = make_scale<X>(amax);
+    if (tid == 0) scales[row] = rs.s;
+    for (uint32_t e = tid * V; there && e < pitch; e += kThreads * V) {
+        uint32_t w[(V + 3) / 4] = {};
+        if (e < p.k && rs.inv != 0.0f) {
+            Access<X, V> u;
+            u.load(x + e);
+            float f[V];
+            u.values(f);
+            row_codes<V>(f, rs, w);
+        }
+        int8_t* out = codes + row * pitch + e;
+        if constexpr (V == 8) *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[V / 4 - 1]);
+        else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(out) = w[0];
+        else *out = static_cast<int8_t>(w[0]);
+    }
+    __syncthreads();
+}
 
 // MR rows of a against every row of b. A block's warps form groups of `wk`
-// that split k between them; a group takes kDotChannels rows of b. Rows of a
-// and b start on 16 bytes and their last 16 bytes may be read whole (the
-// bytes past k are masked out of a).
-template <int MR, class T>
-static __global__ void __launch_bounds__(256) gemm_int8_dot_kernel(const GemmParams p, uint32_t wk) {
+// that split k between them; a group takes kDotChannels rows of b. Rows of b
+// start on 16 bytes and their last 16 bytes may be read whole. X is int8 (rows
+// of codes that start on 16 bytes too, the bytes past k masked out) or a float
+// type: each block then quantises the rows itself, a few thousand values that
+// stay in L2, which costs about 1 us and saves a launch and the codes' memory.
+template <int MR, class X, class T>
+static __global__ void __launch_bounds__(256) gemm_int8_dot_kernel(const __grid_constant__ GemmParams p, uint32_t wk) {
     __shared__ int32_t part[8][MR * kDotChannels];
+    extern __shared__ __align__(16) int8_t row_codes_smem[];
+    constexpr bool kFloat = !std::is_same<X, int8_t>::value;
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t group = (blockIdx.x * 8u + warp) / wk, kw = warp % wk;
     const uint32_t n0 = group * kDotChannels;
     const uint32_t chunks = (p.k + 15u) / 16u;
-    int32_t acc[MR][kDotChannels] = {};
     const int8_t* br[kDotChannels];
 #pragma unroll
     for (int c = 0; c < kDotChannels; ++c) br[c] = p.b + static_cast<int64_t>(min(n0 + c, p.n - 1u)) * p.b_pitch;
+    __shared__ float row_scales[kFloat ? MR : 1];
+    if constexpr (kFloat) {
+        __shared__ uint32_t warp_max[8];
+        // The first weights are on their way while the rows are quantised.
+#pragma unroll
+        for (int c = 0; c < kDotChannels; ++c)
+            if (kw * 32u + lane < chunks)
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(br[c] + (kw * 32u + lane) * 16u));
+        if (p.x_vec16) dot_quantize<MR, X, 16 / static_cast<int>(sizeof(X))>(p, row_codes_smem, chunks * 16u, warp_max, row_scales);
+        else dot_quantize<MR, X, 1>(p, row_codes_smem, chunks * 16u, warp_max, row_scales);
+    }
+    int32_t acc[MR][kDotChannels] = {};
     const uint32_t tail = p.k & 15u;
 #pragma unroll 4
     for (uint32_t i = kw * 32u + lane; i < chunks; i += wk * 32u) {
@@ -55,13 +111,19 @@ static __global__ void __launch_bounds__(256) gemm_int8_dot_kernel(const GemmPar
         for (int c = 0; c < kDotChannels; ++c) w[c] = __ldg(reinterpret_cast<const int4*>(br[c]) + i);
 #pragma unroll
         for (int m = 0; m < MR; ++m) {
-            int4 x = __ldg(reinterpret_cast<const int4*>(p.a + static_cast<int64_t>(min(static_cast<uint32_t>(m), p.m - 1u)) * p.a_pitch) + i);
-            if (tail != 0u && i == chunks - 1u) {
-                int* xw = reinterpret_cast<int*>(&x);
+            int4 x;
+            const uint32_t mm = min(static_cast<uint32_t>(m), p.m - 1u);
+            if constexpr (kFloat) {
+                x = *reinterpret_cast<const int4*>(row_codes_smem + (mm * chunks + i) * 16u);
+            } else {
+                x = __ldg(reinterpret_cast<const int4*>(p.a + static_cast<int64_t>(mm) * p.a_pitch) + i);
+                if (tail != 0u && i == chunks - 1u) {
+                    int* xw = reinterpret_cast<int*>(&x);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int keep = static_cast<int>(tail) - 4 * j;
-                    xw[j] = keep >= 4 ? xw[j] : keep <= 0 ? 0 : xw[j] & ((1 << (8 * keep)) - 1);
+                    for (int j = 0; j < 4; ++j) {
+                        const int keep = static_cast<int>(tail) - 4 * j;
+                        xw[j] = keep >= 4 ? xw[j] : keep <= 0 ? 0 : xw[j] & ((1 << (8 * keep)) - 1);
+                    }
                 }
             }
 #pragma unroll
@@ -91,8 +153,9 @@ static __global__ void __launch_bounds__(256) gemm_int8_dot_kernel(const GemmPar
     }
     const uint32_t m = lane / kDotChannels, n = n0 + lane % kDotChannels;
     if (lane >= MR * kDotChannels || m >= p.m || n >= p.n) return;
+    const float scale = kFloat ? row_scales[kFloat ? m : 0u] : p.a_scales[m];
     const float bias = p.bias == nullptr ? 0.0f : bias_at(p.bias, p.bias_type, n);
-    static_cast<T*>(p.out)[m * p.out_pitch + n] = from_f32<T>(scaled(mine, p.a_scales[m], p.b_scales[n], bias));
+    static_cast<T*>(p.out)[m * p.out_pitch + n] = from_f32<T>(scaled(mine, scale, p.b_scales[n], bias));
 }
 
 // ------------------------------------------------------------- wide kernel
@@ -184,6 +247,7 @@ static __global__ void __launch_bounds__(kWideThreads)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    await_previous();
 
     // The scales and the bias arrive while the sums are made.
     constexpr int kOwn = S == 1 ? 1 : 4;  // channels of a thread
@@ -418,6 +482,7 @@ static __global__ void __launch_bounds__(kPairThreads, 1)
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    await_previous();
 
     if (warp == 0) {
         if (elect_one_sync()) {
@@ -595,19 +660,45 @@ static __global__ void __launch_bounds__(kPairThreads, 1)
 // ------------------------------------------------- operands that TMA cannot read
 
 // Copies rows whose start or pitch is no multiple of 16 bytes to rows of
-// `pitch` bytes (a multiple of 16), zero past the width.
-static __global__ void __launch_bounds__(256) repack_codes_kernel(const int8_t* in, int64_t in_pitch, int8_t* out,
-                                                                  uint32_t pitch, uint32_t rows, uint32_t k) {
-    const uint32_t words = pitch / 4u;
-    const uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256u + threadIdx.x;
-    if (i >= static_cast<uint64_t>(words) * rows) return;
-    const uint32_t r = static_cast<uint32_t>(i / words), c = static_cast<uint32_t>(i % words) * 4u;
-    const int8_t* src = in + r * in_pitch;
-    uint32_t w = 0;
-#pragma unroll
-    for (uint32_t j = 0; j < 4; ++j)
-        if (c + j < k) w |= static_cast<uint32_t>(static_cast<uint8_t>(src[c + j])) << (8u * j);
-    *reinterpret_cast<uint32_t*>(out + static_cast<uint64_t>(r) * pitch + c) = w;
+// `pitch` bytes (a multiple of 16), zero past the width: one launch for one or
+// both operands, four bytes a thread.
+struct RepackParams {
+    const int8_t* in[2];
+    int8_t* out[2];
+    int64_t in_pitch[2];
+    uint32_t rows[2], k;
+    FastDiv words;  // pitch / 4
+};
+
+static __global__ void __launch_bounds__(256) repack_codes_kernel(const __grid_constant__ RepackParams p) {
+    let_next_start();
+    const uint32_t which = blockIdx.y;
+    const uint32_t rows = which ? p.rows[1] : p.rows[0];
+    const int8_t* const in = which ? p.in[1] : p.in[0];
+    const int64_t in_pitch = which ? p.in_pitch[1] : p.in_pitch[0];
+    const uint64_t blocks_of = (static_cast<uint64_t>(rows) * p.words.d + 255u) / 256u;
+    for (uint64_t block = blockIdx.x; block < blocks_of; block += gridDim.x) {
+        // Row and word of a block's first thread by a long division, once.
+        const uint64_t i0 = block * 256u;
+        const uint32_t r0 = static_cast<uint32_t>(i0 / p.words.d);
+        const uint32_t c0 = static_cast<uint32_t>(i0 - static_cast<uint64_t>(r0) * p.words.d) + threadIdx.x;
+        const uint32_t dr = p.words.div(c0), r = r0 + dr, c = (c0 - dr * p.words.d) * 4u;
+        if (r >= rows) continue;
+        const int8_t* src = in + r * in_pitch + c;
+        uint32_t w = 0;
+        if (c + 4u <= p.k) {
+            // Four bytes from the two aligned words that hold them; the second
+            // is read only where it holds one of them.
+            const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src)) & 3u;
+            const uint32_t* at = reinterpret_cast<const uint32_t*>(src - off);
+            const uint32_t lo = __ldg(at), hi = off != 0u ? __ldg(at + 1) : 0u;
+            w = __funnelshift_r(lo, hi, 8u * off);
+        } else {
+            for (uint32_t j = 0; c + j < p.k; ++j) w |= static_cast<uint32_t>(static_cast<uint8_t>(src[j])) << (8u * j);
+        }
+        int8_t* out = which ? p.out[1] : p.out[0];
+        *reinterpret_cast<uint32_t*>(out + (static_cast<uint64_t>(r) * p.words.d * 4u + c)) = w;
+    }
 }
 
 }  // namespace eb

@@ -230,27 +230,45 @@ __device__ __forceinline__ void group_at(const QuantParams& p, uint32_t g, uint3
     head = r - part * p.heads;
 }
 
+// Programmatic dependent launch: a kernel of a call may start while the call's
+// previous kernel ends. await_previous() returns once that one is complete and
+// its writes are seen; everything it made is read, and everything it reads is
+// written, after that. The first kernel of a call is launched plainly, so
+// what other work left in the stream is complete before any of them starts.
+__device__ __forceinline__ void await_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // A slot given twice in one call keeps the last of its rows. Up to
 // kDupScanRows rows each row looks for its slot among the later ones (which
-// stay in L1). Longer calls settle it in the slot's own scale words before any
-// row is written: one launch zeroes them, the next leaves the largest claim
-// 0x80000001 + t there, and the row whose claim stands writes codes and scale.
-// A scale is never negative, so no scale written in between is taken for a
-// claim; what the words held before does not matter.
+// stay in L1). Longer calls settle it before any row is written: a launch of
+// its own leaves the largest claim 0x80000001 + t in the slot's scale words,
+// and the row whose claim stands writes codes and scale. A scale is never
+// negative, so neither one that is written in between nor one that was there
+// is taken for a claim; of whatever else the words held (memory that no write
+// has reached), a number that could be a claim is one only if its row has this
+// slot, and then it loses to a later row's like any other.
 constexpr uint32_t kDupScanRows = 256;
 
 __device__ __forceinline__ uint32_t claim_of(uint32_t t) { return 0x80000001u + t; }
 
-static __global__ void __launch_bounds__(256) cache_claim_kernel(const __grid_constant__ QuantParams p, int clear) {
+static __global__ void __launch_bounds__(256) cache_claim_kernel(const __grid_constant__ QuantParams p) {
+    let_next_start();
     const uint32_t g = blockIdx.x * 256u + threadIdx.x;
     if (g >= p.groups) return;
     uint32_t t, part, head;
     group_at(p, g, t, part, head);
     const int64_t s = slot_of(p, t);
     if (s < 0 || s >= p.num_slots) return;
-    uint32_t* w = reinterpret_cast<uint32_t*>(scale_at(p, part, static_cast<uint32_t>(s), head));
-    if (clear) *w = 0u;
-    else atomicMax(w, claim_of(t));
+    uint32_t* const w = reinterpret_cast<uint32_t*>(scale_at(p, part, static_cast<uint32_t>(s), head));
+    const uint32_t claim = claim_of(t);
+    uint32_t old = *reinterpret_cast<volatile uint32_t*>(w);
+    for (;;) {
+        const uint32_t other = old - claim_of(0);  // the row that `old` would be the claim of
+        if (other < p.t && other >= t && slot_of(p, other) == s) return;
+        const uint32_t seen = atomicCAS(w, old, claim);
+        if (seen == old) return;
+        old = seen;
+    }
 }
 
 // G threads per row (4, 8, a warp, or the whole block), each holding NV
@@ -296,9 +314,11 @@ static __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_
         if (e < p.d && keep) v[j].load(x + e);
         else v[j].zero();
     }
+    let_next_start();
     if constexpr (CACHE) {
         if (p.dup == kDupClaim) {
             // The row's own claim stands until it stores its scale below.
+            await_previous();
             if (keep) keep = *reinterpret_cast<volatile uint32_t*>(scale) == claim_of(t);
         } else if (p.dup == kDupScan && keep) {
             for (uint32_t i = t + 1u + gl; i < p.t; i += G) keep = keep && slot_of(p, i) != static_cast<int64_t>(slot);
@@ -531,6 +551,11 @@ struct GemmParams {
     int64_t out_pitch;  // elements
     uint32_t m, n, k;
     int out_vec4, out_vec16;  // rows of out start on four elements, on 16 bytes
+    int after_previous;       // a was made by the launch before (await_previous)
+    // Rows that the product quantises itself (the dot kernel), in place of a:
+    const void* x;
+    int64_t x_pitch;  // elements
+    int x_vec16;      // they start on 16 bytes and hold a whole number of them
 };
 
 __device__ __forceinline__ float bias_at(const void* bias, int type, uint32_t n) {
