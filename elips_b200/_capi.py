@@ -6,7 +6,7 @@ missing or fails to load, importing this module raises.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libelips_b200.so"
@@ -40,7 +40,7 @@ CODEC_SQ8 = 3
 
 
 class Cache(ctypes.Structure):
-    """elips_b200_cache (entry points take its address, or the same bytes packed)."""
+    """elips_b200_cache. Entry points take the address of these structures, or the same bytes packed."""
     _fields_ = [("codes", c_void_p), ("scales", c_void_p), ("parts", c_int64), ("pages", c_int64),
                 ("page_size", c_int64), ("heads", c_int64), ("dim", c_int64), ("code_strides", c_int64 * 4),
                 ("scale_strides", c_int64 * 4)]
@@ -49,6 +49,20 @@ class Cache(ctypes.Structure):
 class Rows(ctypes.Structure):
     """elips_b200_rows."""
     _fields_ = [("data", c_void_p), ("stride_row", c_int64), ("stride_head", c_int64)]
+
+
+class Gemm(ctypes.Structure):
+    """elips_b200_gemm."""
+    _fields_ = [("a", c_void_p), ("a_scales", c_void_p), ("b", c_void_p), ("b_scales", c_void_p), ("bias", c_void_p),
+                ("out", c_void_p), ("m", c_int64), ("n", c_int64), ("k", c_int64), ("a_stride", c_int64),
+                ("b_stride", c_int64), ("out_stride", c_int64), ("a_type", c_int32), ("bias_type", c_int32),
+                ("out_type", c_int32), ("reserved", c_int32)]
+
+
+class Sequences(ctypes.Structure):
+    """elips_b200_sequences."""
+    _fields_ = [("page_table", c_void_p), ("offsets", c_void_p), ("table_stride", c_int64), ("sequences", c_int64),
+                ("table_width", c_int64), ("total", c_int64), ("table_64bit", c_int32), ("offsets_64bit", c_int32)]
 
 
 # (name, restype, argtypes) for every entry point in include/elips_b200.h.
@@ -156,16 +170,9 @@ SIGNATURES = [
     ("elips_b200_ivfflat_destroy", c_int, [c_void_p]),
     ("elips_b200_quantize_rows", c_int,
      [c_int, c_void_p, c_int, c_size_t, c_size_t, c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
-    ("elips_b200_gemm_int8", c_int,
-     [c_int, c_void_p, c_size_t, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p, c_int, c_size_t, c_size_t,
-      c_size_t, c_void_p, c_int, c_size_t, c_void_p]),
-    ("elips_b200_linear_int8", c_int,
-     [c_int, c_void_p, c_int, c_int64, c_void_p, c_size_t, c_void_p, c_void_p, c_int, c_size_t, c_size_t, c_size_t,
-      c_void_p, c_int, c_size_t, c_void_p]),
+    ("elips_b200_gemm_int8", c_int, [c_int, c_void_p, c_void_p]),
     ("elips_b200_cache_write", c_int, [c_int, c_void_p, c_void_p, c_int, c_size_t, c_void_p, c_int, c_void_p]),
-    ("elips_b200_cache_read", c_int,
-     [c_int, c_void_p, c_void_p, c_int, c_int64, c_size_t, c_size_t, c_void_p, c_int, c_size_t, c_void_p, c_int, c_int,
-      c_void_p]),
+    ("elips_b200_cache_read", c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     ("elips_b200_profiler_enable", c_int, [c_int]),
     ("elips_b200_profiler_stats", c_int,
      [c_char_p, POINTER(ctypes.c_uint64), POINTER(ctypes.c_double), POINTER(ctypes.c_uint64)]),

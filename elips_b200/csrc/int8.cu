@@ -281,11 +281,11 @@ void launch_read(ReadParams p, const elips_b200_cache& c, int num_sms, cudaStrea
     cache_read_kernel<T, V><<<blocks_for(p.total, p.rows), threads, 0, stream>>>(p);
 }
 
-void cache_read(int num_sms, const elips_b200_cache& given, const void* table, int table64, int64_t table_stride, size_t sequences,
-                size_t table_width, const void* offsets, int offsets64, size_t total, const elips_b200_rows* out,
+void cache_read(int num_sms, const elips_b200_cache& given, const elips_b200_sequences& q, const elips_b200_rows* out,
                 int type, int zero_behind, cudaStream_t stream) {
     const elips_b200_cache c = plain_strides(given);
-    if (total == 0) return;
+    if (q.total == 0) return;
+    const size_t total = static_cast<size_t>(q.total);
     ReadParams p{};
     set_cache(p, c);
     for (int64_t i = 0; i < c.parts; ++i) {
@@ -293,13 +293,13 @@ void cache_read(int num_sms, const elips_b200_cache& given, const void* table, i
         p.out_stride_t[i] = total > 1 ? out[i].stride_row : 0;
         p.out_stride_h[i] = c.heads > 1 ? out[i].stride_head : 0;
     }
-    p.table = table;
-    p.table64 = table64;
-    p.table_stride = table_stride;
-    p.offsets = offsets;
-    p.offsets64 = offsets64;
-    p.sequences = static_cast<uint32_t>(sequences);
-    p.table_width = static_cast<uint32_t>(table_width);
+    p.table = q.page_table;
+    p.table64 = q.table_64bit;
+    p.table_stride = q.table_stride;
+    p.offsets = q.offsets;
+    p.offsets64 = q.offsets_64bit;
+    p.sequences = static_cast<uint32_t>(q.sequences);
+    p.table_width = static_cast<uint32_t>(q.table_width);
     p.pages = static_cast<uint32_t>(c.pages);
     p.total = static_cast<uint32_t>(total);
     p.zero_behind = zero_behind;
@@ -494,66 +494,68 @@ void gemm_int8(int num_sms, GemmParams p, int out_type, cudaStream_t stream) {
     product();
 }
 
-void check_gemm(size_t m, size_t n, size_t k, size_t b_pitch, const void* bias, int bias_type, int out_type,
-                size_t out_pitch) {
-    check_float_type(out_type);
-    if (bias != nullptr) check_float_type(bias_type);
-    if (m > kMaxRows || n > kMaxRows) bad("matrix sizes must be below 2^31");
-    if (k > kMaxK) bad("k must be below 2^17: the int32 sum could overflow");
-    if (b_pitch < k || out_pitch < n) bad("neighbouring matrix rows overlap");
+void check_gemm(const elips_b200_gemm& g) {
+    check_float_type(g.out_type);
+    if (g.bias != nullptr) check_float_type(g.bias_type);
+    const bool codes = g.a_type == ELIPS_B200_PRECISION_INT8;
+    if (!codes) check_float_type(g.a_type);
+    if (g.m < 0 || g.n < 0 || g.k < 0 || g.m > static_cast<int64_t>(kMaxRows) || g.n > static_cast<int64_t>(kMaxRows))
+        bad("matrix sizes must be below 2^31");
+    if (g.k > static_cast<int64_t>(kMaxK)) bad("k must be below 2^17: the int32 sum could overflow");
+    if (!codes && g.k == 0) bad("rows to quantise must have a value");
+    if (g.b_stride < g.k || g.out_stride < g.n || (codes && g.a_stride < g.k)) bad("neighbouring matrix rows overlap");
+    if (g.m == 0 || g.n == 0) return;
+    if (g.b_scales == nullptr || g.out == nullptr || (codes && g.a_scales == nullptr)) bad("operand missing");
+    if (g.k > 0 && (g.a == nullptr || g.b == nullptr)) bad("operand missing");
 }
 
-GemmParams gemm_params(const int8_t* a, size_t a_pitch, const float* a_scales, const int8_t* b, size_t b_pitch,
-                       const float* b_scales, const void* bias, int bias_type, size_t m, size_t n, size_t k, void* out,
-                       int out_type, size_t out_pitch) {
+GemmParams gemm_params(const elips_b200_gemm& g) {
     GemmParams p{};
-    p.a = a;
-    p.b = b;
-    p.a_pitch = static_cast<int64_t>(a_pitch);
-    p.b_pitch = static_cast<int64_t>(b_pitch);
-    p.a_scales = a_scales;
-    p.b_scales = b_scales;
-    p.bias = bias;
-    p.bias_type = bias_type;
-    p.out = out;
-    p.out_pitch = static_cast<int64_t>(out_pitch);
-    p.m = static_cast<uint32_t>(m);
-    p.n = static_cast<uint32_t>(n);
-    p.k = static_cast<uint32_t>(k);
-    const size_t size = out_type == ELIPS_B200_PRECISION_FP32 ? 4 : 2;
-    p.out_vec4 = reinterpret_cast<uintptr_t>(out) % (4 * size) == 0 && (m <= 1 || out_pitch % 4 == 0);
-    p.out_vec16 = on_16(out, static_cast<int64_t>(out_pitch * size), p.m);
+    p.a = static_cast<const int8_t*>(g.a);
+    p.a_scales = g.a_scales;
+    p.a_pitch = g.a_stride;
+    p.b = g.b;
+    p.b_pitch = g.b_stride;
+    p.b_scales = g.b_scales;
+    p.bias = g.bias;
+    p.bias_type = g.bias_type;
+    p.out = g.out;
+    p.out_pitch = g.out_stride;
+    p.m = static_cast<uint32_t>(g.m);
+    p.n = static_cast<uint32_t>(g.n);
+    p.k = static_cast<uint32_t>(g.k);
+    const int64_t size = g.out_type == ELIPS_B200_PRECISION_FP32 ? 4 : 2;
+    p.out_vec4 = reinterpret_cast<uintptr_t>(g.out) % (4 * size) == 0 && (p.m <= 1 || g.out_stride % 4 == 0);
+    p.out_vec16 = on_16(g.out, g.out_stride * size, p.m);
     return p;
 }
 
-void linear_int8(int num_sms, const void* x, int x_type, int64_t x_pitch, const int8_t* b, size_t b_pitch, const float* b_scales,
-                 const void* bias, int bias_type, size_t m, size_t n, size_t k, void* out, int out_type,
-                 size_t out_pitch, cudaStream_t stream) {
-    if (m == 0 || n == 0) return;
-    const size_t pitch = (k + 15) / 16 * 16;
+// The product over rows that are not quantised yet.
+void linear_int8(int num_sms, const elips_b200_gemm& g, cudaStream_t stream) {
+    GemmParams p = gemm_params(g);
+    const size_t pitch = (static_cast<size_t>(p.k) + 15) / 16 * 16;
     // Few values: the dot kernel quantises them itself.
-    if (gemm_form(static_cast<uint32_t>(m), static_cast<uint32_t>(n), static_cast<uint32_t>(k), num_sms).rows == 1 &&
-        m * pitch <= kDotCodeBytes && on_16(b, static_cast<int64_t>(b_pitch), static_cast<uint32_t>(n))) {
-        GemmParams p = gemm_params(nullptr, pitch, nullptr, b, b_pitch, b_scales, bias, bias_type, m, n, k, out, out_type,
-                                   out_pitch);
-        p.x = x;
-        p.x_pitch = m > 1 ? x_pitch : 0;
-        Profiler::Scope prof("linear_int8", stream, static_cast<uint64_t>(m) * n);
-        with_float_type(x_type, [&](auto xt) {
+    if (gemm_form(p.m, p.n, p.k, num_sms).rows == 1 && p.m * pitch <= kDotCodeBytes && on_16(p.b, p.b_pitch, p.n)) {
+        p.x = g.a;
+        p.x_pitch = p.m > 1 ? g.a_stride : 0;
+        Profiler::Scope prof("linear_int8", stream, static_cast<uint64_t>(p.m) * p.n);
+        with_float_type(g.a_type, [&](auto xt) {
             using X = decltype(xt);
-            p.x_vec16 = on_16(x, x_pitch * static_cast<int64_t>(sizeof(X)), p.m) && k % (16 / sizeof(X)) == 0;
-            with_float_type(out_type, [&](auto tag) { launch_dot<X, decltype(tag)>(p, num_sms, stream); });
+            p.x_vec16 = on_16(g.a, g.a_stride * static_cast<int64_t>(sizeof(X)), p.m) && p.k % (16 / sizeof(X)) == 0;
+            with_float_type(g.out_type, [&](auto tag) { launch_dot<X, decltype(tag)>(p, num_sms, stream); });
         });
         return;
     }
-    const size_t code_bytes = (m * pitch + 255) / 256 * 256;
-    StreamScratch s(code_bytes + m * sizeof(float), stream);
+    const size_t code_bytes = (p.m * pitch + 255) / 256 * 256;
+    StreamScratch s(code_bytes + p.m * sizeof(float), stream);
     int8_t* codes = reinterpret_cast<int8_t*>(s.get());
     float* scales = reinterpret_cast<float*>(s.get() + code_bytes);
-    quantize_rows(x, x_type, m, k, x_pitch, codes, pitch, scales, stream);
-    GemmParams p = gemm_params(codes, pitch, scales, b, b_pitch, b_scales, bias, bias_type, m, n, k, out, out_type, out_pitch);
+    quantize_rows(g.a, g.a_type, p.m, p.k, g.a_stride, codes, pitch, scales, stream);
+    p.a = codes;
+    p.a_pitch = static_cast<int64_t>(pitch);
+    p.a_scales = scales;
     p.after_previous = 1;
-    gemm_int8(num_sms, p, out_type, stream);
+    gemm_int8(num_sms, p, g.out_type, stream);
 }
 
 cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
@@ -590,32 +592,17 @@ int elips_b200_quantize_rows(int device, const void* x, int type, size_t n, size
     });
 }
 
-int elips_b200_gemm_int8(int device, const int8_t* a, size_t a_stride, const float* a_scales, const int8_t* b,
-                         size_t b_stride, const float* b_scales, const void* bias, int bias_type, size_t m, size_t n,
-                         size_t k, void* out, int out_type, size_t out_stride, void* stream) {
-    if (m > 0 && n > 0 && ((k > 0 && (a == nullptr || b == nullptr)) || a_scales == nullptr || b_scales == nullptr || out == nullptr))
-        return ELIPS_B200_INVALID_ARGUMENT;
+int elips_b200_gemm_int8(int device, const elips_b200_gemm* args, void* stream) {
+    if (args == nullptr) return ELIPS_B200_INVALID_ARGUMENT;
     return guarded([&] {
-        eb::check_gemm(m, n, k, b_stride, bias, bias_type, out_type, out_stride);
-        if (a_stride < k) eb::bad("neighbouring matrix rows overlap");
+        eb::check_gemm(*args);
+        if (args->m == 0 || args->n == 0) return;
         eb::DeviceGuard g(device);
-        eb::gemm_int8(eb::device_props(device).num_sms, eb::gemm_params(a, a_stride, a_scales, b, b_stride, b_scales, bias, bias_type, m, n, k, out,
-                                      out_type, out_stride),
-                      out_type, eb::as_stream(stream));
-    });
-}
-
-int elips_b200_linear_int8(int device, const void* x, int x_type, int64_t x_stride, const int8_t* w, size_t w_stride,
-                           const float* w_scales, const void* bias, int bias_type, size_t m, size_t n, size_t k,
-                           void* out, int out_type, size_t out_stride, void* stream) {
-    if (m > 0 && n > 0 && (x == nullptr || w == nullptr || w_scales == nullptr || out == nullptr))
-        return ELIPS_B200_INVALID_ARGUMENT;
-    return guarded([&] {
-        eb::check_gemm(m, n, k, w_stride, bias, bias_type, out_type, out_stride);
-        eb::check_rows(m, k, x_type);
-        eb::DeviceGuard g(device);
-        eb::linear_int8(eb::device_props(device).num_sms, x, x_type, x_stride, w, w_stride, w_scales, bias, bias_type, m, n, k, out, out_type,
-                        out_stride, eb::as_stream(stream));
+        const int num_sms = eb::device_props(device).num_sms;
+        if (args->a_type == ELIPS_B200_PRECISION_INT8)
+            eb::gemm_int8(num_sms, eb::gemm_params(*args), args->out_type, eb::as_stream(stream));
+        else
+            eb::linear_int8(num_sms, *args, eb::as_stream(stream));
     });
 }
 
@@ -632,20 +619,21 @@ int elips_b200_cache_write(int device, const elips_b200_cache* cache, const elip
     });
 }
 
-int elips_b200_cache_read(int device, const elips_b200_cache* cache, const void* page_table, int table_64bit,
-                          int64_t table_stride, size_t sequences, size_t table_width, const void* offsets,
-                          int offsets_64bit, size_t total, const elips_b200_rows* out, int type, int zero_behind,
-                          void* stream) {
-    if (cache == nullptr || (total > 0 && out == nullptr)) return ELIPS_B200_INVALID_ARGUMENT;
+int elips_b200_cache_read(int device, const elips_b200_cache* cache, const elips_b200_sequences* sequences,
+                          const elips_b200_rows* out, int type, int zero_behind, void* stream) {
+    if (cache == nullptr || sequences == nullptr) return ELIPS_B200_INVALID_ARGUMENT;
+    const elips_b200_sequences& q = *sequences;
+    if (q.total < 0 || q.sequences < 0 || q.table_width < 0 || (q.total > 0 && out == nullptr))
+        return ELIPS_B200_INVALID_ARGUMENT;
     return guarded([&] {
         eb::check_cache(*cache);
-        eb::check_cache_rows(*cache, out, type, total);
-        if (sequences > eb::kMaxRows || table_width > eb::kMaxRows) eb::bad("page table too large");
-        if (total > 0 && sequences > 0 && offsets == nullptr) eb::bad("offsets missing");
-        if (total > 0 && sequences > 0 && table_width > 0 && page_table == nullptr) eb::bad("page table missing");
+        eb::check_cache_rows(*cache, out, type, static_cast<size_t>(q.total));
+        if (q.sequences > static_cast<int64_t>(eb::kMaxRows) || q.table_width > static_cast<int64_t>(eb::kMaxRows))
+            eb::bad("page table too large");
+        if (q.total > 0 && q.sequences > 0 && q.offsets == nullptr) eb::bad("offsets missing");
+        if (q.total > 0 && q.sequences > 0 && q.table_width > 0 && q.page_table == nullptr) eb::bad("page table missing");
         eb::DeviceGuard g(device);
-        eb::cache_read(eb::device_props(device).num_sms, *cache, page_table, table_64bit, table_stride, sequences, table_width, offsets, offsets_64bit,
-                       total, out, type, zero_behind, eb::as_stream(stream));
+        eb::cache_read(eb::device_props(device).num_sms, *cache, q, out, type, zero_behind, eb::as_stream(stream));
     });
 }
 

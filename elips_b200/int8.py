@@ -41,9 +41,11 @@ from .exact import DimensionMismatch
 _LIB = capi.LIB
 _TYPES = {torch.float32: capi.PRECISION_FP32, torch.float16: capi.PRECISION_FP16,
           torch.bfloat16: capi.PRECISION_BF16}
-# elips_b200_cache and elips_b200_rows, packed: a call costs little more on the
-# host than its launch, and building ctypes structures would double that.
+# The C structures, packed: on the host a small call costs little more than its
+# launch, and ctypes structures or a dozen ctypes arguments would add to that.
+_GEMM = struct.Struct("12q4i")
 _CACHE = struct.Struct("15q")
+_SEQUENCES = struct.Struct("6q2i")
 _ROWS = (None, struct.Struct("3q"), struct.Struct("6q"))
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda device: torch.cuda.current_stream(device).cuda_stream)
@@ -68,10 +70,11 @@ def _float_type(dtype, what: str) -> int:
 def _pitch(t, what: str, apart: bool = True) -> int:
     """Checks a matrix with contiguous rows; elements from one row to the next
     (the width where there is no next). apart: rows must not overlap."""
-    if t.dim() != 2:
+    strides = t.stride()
+    if len(strides) != 2:
         raise DimensionMismatch(f"{what} must have two axes")
     rows, width = t.shape
-    pitch, step = t.stride()
+    pitch, step = strides
     if step != 1 and width > 1:
         raise ValueError(f"{what} must have contiguous rows")
     if rows < 2:
@@ -81,11 +84,13 @@ def _pitch(t, what: str, apart: bool = True) -> int:
     return pitch
 
 
-def _vector(t, n: int, what: str) -> None:
-    if t.dim() != 1 or t.shape[0] != n:
+def _vector(t, n: int, what: str) -> int:
+    """Checks n contiguous values; their address."""
+    if t.shape != (n,):
         raise DimensionMismatch(f"{what} must have {n} entries")
-    if n > 1 and t.stride(0) != 1:
+    if not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous")
+    return t.data_ptr()
 
 
 def _handle(stream) -> int:
@@ -129,58 +134,52 @@ def quantize_rows(x, stream=None):
     return (codes if wide == d else codes[:, :d]), scales
 
 
-def _product(entry, name, x, x_kind, x_scales, b, b_scales, bias, dtype, out, stream):
-    """What gemm_int8 (x_kind None) and linear_int8 share: the checks of the
-    n x k operand, its scales, the bias and the output, and the call."""
-    pitch = _pitch(x, "rows", apart=x_kind is None)
+def _product(x, x_kind, x_scales, b, b_scales, bias, dtype, out, stream):
+    """The product of rows x (codes with x_scales, or floats with None) with the
+    n x k codes b: the checks, the output, the call."""
+    codes = x_scales is not None
+    pitch, b_pitch = _pitch(x, "rows", codes), _pitch(b, "weight codes")
     m, k = x.shape
+    n, width = b.shape
+    if width != k:
+        raise DimensionMismatch(f"rows of {k} and of {width} values")
     if b.dtype is not torch.int8:
         raise ValueError(f"weight codes must be int8, not {b.dtype}")
-    b_pitch = _pitch(b, "weight codes")
-    n = b.shape[0]
-    if b.shape[1] != k:
-        raise DimensionMismatch(f"rows of {k} and of {b.shape[1]} values")
-    if b_scales.dtype is not torch.float32:
-        raise ValueError(f"scales must be float32, not {b_scales.dtype}")
-    _vector(b_scales, n, "weight scales")
-    if x_kind is None:
-        if x_scales.dtype is not torch.float32:
-            raise ValueError(f"scales must be float32, not {x_scales.dtype}")
-        _vector(x_scales, m, "row scales")
-    bias_ptr, bias_kind = None, 0
+    if b_scales.dtype is not torch.float32 or (codes and x_scales.dtype is not torch.float32):
+        raise ValueError("scales must be float32")
+    x_scales_at = _vector(x_scales, m, "row scales") if codes else 0
+    b_scales_at = _vector(b_scales, n, "weight scales")
+    bias_at = bias_kind = 0
     if bias is not None:
         bias_kind = _float_type(bias.dtype, "bias")
-        _vector(bias, n, "bias")
-        bias_ptr = bias.data_ptr()
+        bias_at = _vector(bias, n, "bias")
     if out is not None:
         dtype = out.dtype
-        if out.dim() != 2 or out.shape[0] != m or out.shape[1] != n:
-            raise DimensionMismatch(f"out must be {m} x {n}")
         out_pitch = _pitch(out, "out")
-    kind = _float_type(dtype, "out")
-    if torch.is_grad_enabled() and (b_scales.requires_grad or x.requires_grad or
-                                    (x_scales is not None and x_scales.requires_grad) or
+        if out.shape != (m, n):
+            raise DimensionMismatch(f"out must be {m} x {n}")
+    kind = _TYPES.get(dtype)
+    if kind is None:
+        _float_type(dtype, "out")
+    if torch.is_grad_enabled() and (b_scales.requires_grad or x.requires_grad or (codes and x_scales.requires_grad) or
                                     (bias is not None and bias.requires_grad) or (out is not None and out.requires_grad)):
         _refuse_grad()
     device = x.get_device()
     if device < 0 or b.get_device() != device or b_scales.get_device() != device or \
-            (x_scales is not None and x_scales.get_device() != device) or \
+            (codes and x_scales.get_device() != device) or \
             (bias is not None and bias.get_device() != device) or (out is not None and out.get_device() != device):
         _refuse_devices(x, b, x_scales, b_scales, bias, out)
     if stream is not None:
         with _using(stream, device, x, b, x_scales, b_scales, bias, out):
-            return _product(entry, name, x, x_kind, x_scales, b, b_scales, bias, dtype, out, None)
+            return _product(x, x_kind, x_scales, b, b_scales, bias, dtype, out, None)
     if out is None:
         out = x.new_empty((m, n), dtype=dtype)
         out_pitch = n or 1
-    if x_kind is None:
-        status = entry(device, x.data_ptr(), pitch, x_scales.data_ptr(), b.data_ptr(), b_pitch, b_scales.data_ptr(),
-                       bias_ptr, bias_kind, m, n, k, out.data_ptr(), kind, out_pitch, _raw_stream(device))
-    else:
-        status = entry(device, x.data_ptr(), x_kind, pitch, b.data_ptr(), b_pitch, b_scales.data_ptr(),
-                       bias_ptr, bias_kind, m, n, k, out.data_ptr(), kind, out_pitch, _raw_stream(device))
+    status = _LIB.elips_b200_gemm_int8(
+        device, _GEMM.pack(x.data_ptr(), x_scales_at, b.data_ptr(), b_scales_at, bias_at, out.data_ptr(), m, n, k, pitch,
+                           b_pitch, out_pitch, x_kind, bias_kind, kind, 0), _raw_stream(device))
     if status:
-        capi.check(status, name)
+        capi.check(status, "elips_b200_gemm_int8")
     return out
 
 
@@ -195,18 +194,17 @@ def gemm_int8(a, b, a_scales, b_scales, bias=None, out_dtype=torch.bfloat16, out
     [n] may have another float type than out."""
     if a.dtype is not torch.int8:
         raise ValueError(f"row codes must be int8, not {a.dtype}")
-    return _product(_LIB.elips_b200_gemm_int8, "elips_b200_gemm_int8", a, None, a_scales, b, b_scales, bias, out_dtype,
-                    out, stream)
+    return _product(a, capi.PRECISION_INT8, a_scales, b, b_scales, bias, out_dtype, out, stream)
 
 
 def linear_int8(x, weight, weight_scales, bias=None, out_dtype=None, out=None, stream=None):
     """gemm_int8 over the rows of x [m, k], quantised on the way as
     quantize_rows quantises them; out_dtype defaults to x's type."""
-    kind = _float_type(x.dtype, "rows")
-    if x.shape[-1:] == (0,):
+    dtype = x.dtype
+    kind = _float_type(dtype, "rows")
+    if x.numel() == 0 and x.shape[-1:] == (0,):
         raise DimensionMismatch("rows must have at least one value")
-    return _product(_LIB.elips_b200_linear_int8, "elips_b200_linear_int8", x, kind, None, weight, weight_scales, bias,
-                    x.dtype if out_dtype is None else out_dtype, out, stream)
+    return _product(x, kind, None, weight, weight_scales, bias, dtype if out_dtype is None else out_dtype, out, stream)
 
 
 def _distinct(strides, shape, what: str) -> None:
@@ -343,9 +341,9 @@ def cache_read(codes, scales, page_table, offsets, total: int, dtype=torch.bfloa
         out = tuple(codes.new_empty((total, heads, dim), dtype=dtype) for _ in range(parts))
         first = (heads * dim, dim)
         packed = _ROWS[parts].pack(*(v for x in out for v in (x.data_ptr(), *first)))
-    status = _LIB.elips_b200_cache_read(device, cache, page_table.data_ptr(), table_wide, table_stride, sequences, width,
-                                        offsets.data_ptr(), offsets_wide, total, packed, kind, fresh,
-                                        _raw_stream(device))
+    seqs = _SEQUENCES.pack(page_table.data_ptr(), offsets.data_ptr(), table_stride, sequences, width, total, table_wide,
+                           offsets_wide)
+    status = _LIB.elips_b200_cache_read(device, cache, seqs, packed, kind, fresh, _raw_stream(device))
     if status:
         capi.check(status, "elips_b200_cache_read")
     return out

@@ -592,22 +592,27 @@ ELIPS_B200_API int elips_b200_ivfpq_train(int device, int metric, const float* r
 ELIPS_B200_API int elips_b200_quantize_rows(int device, const void* x, int type, size_t n, size_t d, int64_t x_stride,
                                             int8_t* codes, size_t code_stride, float* scales, void* stream);
 
-/* out[i][j] = (sum_l a[i][l] * b[j][l]) * a_scales[i] * b_scales[j] + bias[j],
- * rounded once to out_type: a is m x k, b is n x k (a layer's weight, or the
- * stored rows that queries are scored against), both int8 and row-major, the
- * sum exact in int32 (k < 2^17). bias may be NULL, its type is bias_type. */
-ELIPS_B200_API int elips_b200_gemm_int8(int device, const int8_t* a, size_t a_stride, const float* a_scales,
-                                        const int8_t* b, size_t b_stride, const float* b_scales, const void* bias,
-                                        int bias_type, size_t m, size_t n, size_t k, void* out, int out_type,
-                                        size_t out_stride, void* stream);
+/* A product of int8 matrices. a is m x k, b is n x k (a layer's weight with a
+ * scale per channel, or stored rows that queries are scored against), both
+ * row-major. a_type is ELIPS_B200_PRECISION_INT8 for codes with a_scales, or a
+ * float type for rows that are quantised on the way as
+ * elips_b200_quantize_rows does (a_scales is not read then, and k >= 1).
+ * bias may be NULL; its type is its own. */
+typedef struct {
+    const void* a;
+    const float* a_scales;
+    const int8_t* b;
+    const float* b_scales;
+    const void* bias;
+    void* out;
+    int64_t m, n, k;
+    int64_t a_stride, b_stride, out_stride;
+    int32_t a_type, bias_type, out_type, reserved;
+} elips_b200_gemm;
 
-/* elips_b200_gemm_int8 over rows of x quantised on the way (one scale per row
- * of x, as elips_b200_quantize_rows gives): a layer whose weight is int8.
- * k >= 1. */
-ELIPS_B200_API int elips_b200_linear_int8(int device, const void* x, int x_type, int64_t x_stride, const int8_t* w,
-                                          size_t w_stride, const float* w_scales, const void* bias, int bias_type,
-                                          size_t m, size_t n, size_t k, void* out, int out_type, size_t out_stride,
-                                          void* stream);
+/* out[i][j] = (sum_l a[i][l] * b[j][l]) * a_scales[i] * b_scales[j] + bias[j],
+ * rounded once to out_type; the sum is exact in int32 (k < 2^17). */
+ELIPS_B200_API int elips_b200_gemm_int8(int device, const elips_b200_gemm* args, void* stream);
 
 /* A paged cache of quantised rows: codes [parts][pages][page_size][heads][dim]
  * and scales [parts][pages][page_size][heads] with the given strides (the
@@ -636,18 +641,25 @@ typedef struct {
 ELIPS_B200_API int elips_b200_cache_write(int device, const elips_b200_cache* cache, const elips_b200_rows* rows,
                                           int type, size_t t, const void* slots, int slots_64bit, void* stream);
 
-/* Reads sequences back into packed rows: output row r of each part belongs to
- * the sequence b with offsets[b] <= r < offsets[b + 1] (offsets ascending,
- * sequences + 1 entries) and is position i = r - offsets[b] of it, in page
- * page_table[b * table_stride + i / page_size]. A page that is no page of the
- * cache, or past the table's width, reads as zeros, and so do rows in front
- * of offsets[0]. Rows from
- * offsets[sequences] to `total` are zeroed where zero_behind, else left as
- * they are. */
-ELIPS_B200_API int elips_b200_cache_read(int device, const elips_b200_cache* cache, const void* page_table,
-                                         int table_64bit, int64_t table_stride, size_t sequences, size_t table_width,
-                                         const void* offsets, int offsets_64bit, size_t total,
-                                         const elips_b200_rows* out, int type, int zero_behind, void* stream);
+/* Sequences over the pages of a cache: output row r belongs to the sequence b
+ * with offsets[b] <= r < offsets[b + 1] (offsets ascending, sequences + 1
+ * entries) and is position i = r - offsets[b] of it, in page page_table[b *
+ * table_stride + i / page_size]. Both are int32, or int64 where the flag says
+ * so. `total` is the number of output rows. */
+typedef struct {
+    const void* page_table;
+    const void* offsets;
+    int64_t table_stride, sequences, table_width, total;
+    int32_t table_64bit, offsets_64bit;
+} elips_b200_sequences;
+
+/* Reads sequences back into packed rows, one output per part. A page that is
+ * no page of the cache, or past the table's width, reads as zeros, and so do
+ * rows in front of offsets[0]. Rows from offsets[sequences] on are zeroed
+ * where zero_behind, else left as they are. */
+ELIPS_B200_API int elips_b200_cache_read(int device, const elips_b200_cache* cache,
+                                         const elips_b200_sequences* sequences, const elips_b200_rows* out, int type,
+                                         int zero_behind, void* stream);
 
 /* ------------------------------------------------------------ profiling */
 /* Device-side counterpart of GpuProfiler (src/gpu_engine/GpuProfiler.cpp:

@@ -98,29 +98,40 @@ def test_c_entry_points_refuse_before_the_device():
     assert lib.elips_b200_quantize_rows(0, p, f32, 1, (1 << 24) + 1, 8, p, 1 << 25, p, None) == bad
     assert lib.elips_b200_quantize_rows(0, p, f32, 2, 8, 8, p, 7, p, None) == bad
 
-    def gemm(a=p, a_stride=16, m=4, n=4, k=16, b_stride=16, bias=None, bias_type=0, out_type=f32, out_stride=4):
-        return lib.elips_b200_gemm_int8(0, a, a_stride, p, p, b_stride, p, bias, bias_type, m, n, k, p, out_type,
-                                        out_stride, None)
+    def gemm(**kw):
+        d = dict(a=p, a_scales=p, b=p, b_scales=p, bias=None, out=p, m=4, n=4, k=16, a_stride=16, b_stride=16, out_stride=4,
+                 a_type=int8, bias_type=0, out_type=f32, reserved=0) | kw
+        return lib.elips_b200_gemm_int8(0, ctypes.byref(_capi.Gemm(*d.values())), None)
+    assert lib.elips_b200_gemm_int8(0, None, None) == bad
     assert gemm(a=None) == bad
+    assert gemm(b_scales=None) == bad
+    assert gemm(a_scales=None) == bad
     assert gemm(a_stride=15) == bad
     assert gemm(b_stride=15) == bad
     assert gemm(out_stride=3) == bad
     assert gemm(out_type=int8) == bad
+    assert gemm(a_type=7) == bad
     assert gemm(bias=p, bias_type=9) == bad
     assert gemm(k=1 << 17, a_stride=1 << 17, b_stride=1 << 17) == bad   # the int32 sum could pass 2^31
     assert gemm(m=1 << 32) == bad
-    assert lib.elips_b200_linear_int8(0, p, int8, 16, p, 16, p, None, 0, 4, 4, 16, p, f32, 4, None) == bad
-    assert lib.elips_b200_linear_int8(0, p, f32, 16, p, 16, p, None, 0, 4, 4, 0, p, f32, 4, None) == bad
+    assert gemm(n=-1) == bad
+    assert gemm(a_type=bf16, k=0) == bad
+    assert gemm(m=0, a=None) == _capi.OK                                # nothing to do
 
     def described(**kw):
         d = dict(codes=p, scales=p, parts=1, pages=3, page_size=4, heads=2, dim=8) | kw
         return _capi.Cache(d["codes"], d["scales"], d["parts"], d["pages"], d["page_size"], d["heads"], d["dim"],
                            (0, 64, 16, 8), (0, 8, 2, 1))
     r = (_capi.Rows * 2)(_capi.Rows(p, 16, 8), _capi.Rows(None, 16, 8))
-    write = lambda c, t=2, type=bf16, slots=p: lib.elips_b200_cache_write(  # noqa: E731
-        0, None if c is None else ctypes.byref(c), r, type, t, slots, 1, None)
-    read = lambda c, total=2, type=bf16, table=p, offsets=p: lib.elips_b200_cache_read(  # noqa: E731
-        0, None if c is None else ctypes.byref(c), table, 0, 3, 2, 3, offsets, 0, total, r, type, 1, None)
+
+    def write(c, type=bf16, slots=p):
+        return lib.elips_b200_cache_write(0, None if c is None else ctypes.byref(c), r, type, 2, slots, 1, None)
+
+    def read(c, type=bf16, **kw):
+        d = dict(page_table=p, offsets=p, table_stride=3, sequences=2, table_width=3, total=2, table_64bit=0,
+                 offsets_64bit=0) | kw
+        return lib.elips_b200_cache_read(0, None if c is None else ctypes.byref(c),
+                                         ctypes.byref(_capi.Sequences(*d.values())), r, type, 1, None)
     for call in (write, read):
         assert call(None) == bad
         assert call(described(parts=3)) == bad
@@ -131,5 +142,8 @@ def test_c_entry_points_refuse_before_the_device():
         assert call(described(pages=1 << 30, page_size=2)) == bad
         assert call(described(), type=int8) == bad
     assert write(described(), slots=None) == bad
-    assert read(described(), table=None) == bad
+    assert read(described(), page_table=None) == bad
+    assert read(described(), total=-1) == bad
+    assert read(described(), sequences=1 << 40) == bad
+    assert lib.elips_b200_cache_read(0, ctypes.byref(described()), None, r, bf16, 1, None) == bad
     assert read(described(), offsets=None) == bad
