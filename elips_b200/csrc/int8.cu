@@ -352,24 +352,28 @@ void launch_dot(const GemmParams& p, int num_sms, cudaStream_t stream) {
 
 template <int BT, int S, class T>
 void launch_wide_split(const GemmParams& p, int num_sms, cudaStream_t stream) {
-    const uint32_t n_ct = cdiv(p.n, kWideChannels), n_rt = cdiv(p.m, BT);
     constexpr uint32_t stage_bytes = (kWideChannels + BT) * kGemmStageK;
-    const uint32_t per = std::max(1u, cdiv(cdiv(p.k, kGemmStageK), S));
-    // All of k in flight where a CTA has an SM to itself. Several waves of CTAs
-    // run two or three to an SM, one's epilogue under another's loads (64 x
-    // 100,000 x 768: 29.6 us with six stages, 21.9 with three), and clusters of
-    // eight find room on every GPC only at two to an SM.
-    const bool shared = S == 8 || static_cast<uint64_t>(n_ct) * n_rt * S > static_cast<uint64_t>(num_sms);
-    uint32_t stages = std::min<uint32_t>(per, shared ? std::max(3u, 92160u / stage_bytes) : 196608u / stage_bytes);
+    const uint32_t n_rt = cdiv(p.m, BT);
+    const uint64_t all = static_cast<uint64_t>(cdiv(p.n, kWideChannels)) * n_rt;
+    if (all > 0x7FFFFFFFull / S) bad("too many rows in one call");
+    const uint32_t tiles = static_cast<uint32_t>(all), kblocks = cdiv(p.k, kGemmStageK);
+    // A CTA has an SM to itself and keeps as much of k in flight as fits. Where
+    // there are more tiles than SMs two share one, for eight warps to store what
+    // the loads bring (64 x 100,000 x 384 to fp32: 17.8 us with one, 14.5 with
+    // two); clusters of eight find room on every GPC only at two to an SM.
+    const bool two = S == 8 || (S == 1 && tiles > static_cast<uint32_t>(num_sms));
+    uint32_t stages = (two ? 111000u : 196608u) / stage_bytes;
+    if (S > 1 || !two) stages = std::min(stages, std::max(1u, cdiv(kblocks, S)));
     stages = std::min<uint32_t>(stages, kWideMaxStages);
     const size_t smem = 1024 + std::max<size_t>(static_cast<size_t>(stages) * stage_bytes, S > 1 ? BT * kWideChannels * 4u : 0u);
     const CUtensorMap mw = code_map(p.b, p.b_pitch, p.n, p.k, kWideChannels);
     const CUtensorMap mx = code_map(p.a, p.a_pitch, p.m, p.k, BT);
     allow_dynamic_smem(reinterpret_cast<const void*>(gemm_int8_wide_kernel<BT, S, T>), smem);
-    LaunchConfig cfg(dim3(S, n_ct, n_rt), kWideThreads, smem, stream);
+    const uint32_t ctas = S == 1 ? std::min<uint32_t>(tiles, static_cast<uint32_t>(num_sms) * (two ? 2u : 1u)) : tiles * S;
+    LaunchConfig cfg(dim3(ctas), kWideThreads, smem, stream);
     if (S > 1) cfg.clusters_of(S);
     if (p.after_previous) cfg.after_previous();
-    cfg.launch(gemm_int8_wide_kernel<BT, S, T>, mw, mx, p, stages);
+    cfg.launch(gemm_int8_wide_kernel<BT, S, T>, mw, mx, p, stages, n_rt, tiles);
 }
 
 template <int BT, class T>
@@ -407,13 +411,16 @@ struct GemmForm {
 // others the least time that a simple model gives, in us, from what was
 // measured over sizes from 16 x 1024 x 1024 to 8192^3:
 //  * wide: 4 for the launch and its ends; a CTA loads 127 KB/us, four fifths
-//    of that when all SMs do; a cluster's summing costs 0.35 and 0.0145 a row;
-//    and each further tile that an SM gets after its first 2 more.
+//    of that when all SMs do; a cluster's summing costs 0.35 and 0.0145 a row.
+//    With more tiles than SMs, each takes 0.2 and its loads or, if longer, its
+//    stores (0.02 a row, a quarter more to fp32).
 //  * pair: 4.5 for the launch and its ends, then waves of tiles at 0.36 per
-//    128 of k (1670 T products/s, the tensor cores' pace at this power) + 1.2.
-// E.g. 512 x 4096 x 4096: wide of 128 rows 13.0 us, pair 16.6; 1024 x 4096 x
-// 4096: 23.4 and 17.2; 64 x 100,000 x 384 to fp32: 16.4 (64 rows) and 22.8.
-GemmForm gemm_form(uint32_t m, uint32_t n, uint32_t k, int num_sms) {
+//    128 of k (1670 T products/s, the tensor cores' pace at this power) + 1.2,
+//    2.4 at least, 0.8 more to fp32.
+// E.g. 512 x 4096 x 4096: wide of 128 rows 12.6 us, pair 16.3; 1024 x 4096 x
+// 4096: 19.1 and 16.9; 64 x 100,000 x 384 to fp32: 14.5 (64 rows) and 23.2;
+// 10,000 x 1536 x 768: 21.5 and 16.9.
+GemmForm gemm_form(uint32_t m, uint32_t n, uint32_t k, bool fp32, int num_sms) {
     if (k > 0 && (m <= 2 || (m <= 8 && static_cast<uint64_t>(m) * n * k <= (1u << 25)))) return {1, 1};
     const uint32_t kb = cdiv(k, kGemmStageK);
     const double sms = num_sms;
@@ -421,18 +428,18 @@ GemmForm gemm_form(uint32_t m, uint32_t n, uint32_t k, int num_sms) {
     double least = 1e30;
     if (kb > 0) {
         const uint64_t tiles = static_cast<uint64_t>(cdiv(m, kPairM)) * cdiv(n, kPairN);
-        least = 4.5 + static_cast<double>((tiles + num_sms / 2 - 1) / (num_sms / 2)) * (kb * 0.36 + 1.2);
+        const double each = std::max(kb * 0.36 + 1.2, 2.4) + (fp32 ? 0.8 : 0);
+        least = 4.5 + static_cast<double>((tiles + num_sms / 2 - 1) / (num_sms / 2)) * each;
     }
     for (uint32_t rows = 16; rows <= 128; rows *= 2) {
         const uint64_t tiles = static_cast<uint64_t>(cdiv(n, kWideChannels)) * cdiv(m, rows);
-        if (cdiv(n, kWideChannels) > 65535 || cdiv(m, rows) > 65535) continue;
         const double per_kb = (kWideChannels + rows) * kGemmStageK / 127e3;
         for (uint32_t splits = 1; splits <= 8; splits *= 2) {
             if (splits > 1 && (tiles * splits > static_cast<uint64_t>(num_sms) || splits > kb)) break;
             const double each = cdiv(kb, splits) * per_kb;
             const double us = tiles <= static_cast<uint64_t>(num_sms)
                                   ? 4 + each + (splits > 1 ? 0.35 + 0.0145 * rows : 0)
-                                  : 2 + tiles / sms * (1.25 * each + 2);
+                                  : 4 + tiles / sms * (0.2 + std::max(1.25 * each, (fp32 ? 0.025 : 0.02) * rows));
             if (us < least) least = us, best = {rows, splits};
         }
         if (rows >= m) break;
@@ -442,7 +449,7 @@ GemmForm gemm_form(uint32_t m, uint32_t n, uint32_t k, int num_sms) {
 
 template <class T>
 void launch_gemm(const GemmParams& p, int num_sms, cudaStream_t stream) {
-    GemmForm f = gemm_form(p.m, p.n, p.k, num_sms);
+    const GemmForm f = gemm_form(p.m, p.n, p.k, sizeof(T) == 4, num_sms);
     if (f.rows == 0) launch_pair<T>(p, num_sms, stream);
     else if (f.rows == 1) launch_dot<int8_t, T>(p, num_sms, stream);
     else if (f.rows == 16) launch_wide<16, T>(p, num_sms, f.splits, stream);
@@ -535,7 +542,7 @@ void linear_int8(int num_sms, const elips_b200_gemm& g, cudaStream_t stream) {
     GemmParams p = gemm_params(g);
     const size_t pitch = (static_cast<size_t>(p.k) + 15) / 16 * 16;
     // Few values: the dot kernel quantises them itself.
-    if (gemm_form(p.m, p.n, p.k, num_sms).rows == 1 && p.m * pitch <= kDotCodeBytes && on_16(p.b, p.b_pitch, p.n)) {
+    if (gemm_form(p.m, p.n, p.k, g.out_type == ELIPS_B200_PRECISION_FP32, num_sms).rows == 1 && p.m * pitch <= kDotCodeBytes && on_16(p.b, p.b_pitch, p.n)) {
         p.x = g.a;
         p.x_pitch = p.m > 1 ? g.a_stride : 0;
         Profiler::Scope prof("linear_int8", stream, static_cast<uint64_t>(p.m) * p.n);

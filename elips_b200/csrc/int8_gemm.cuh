@@ -196,37 +196,42 @@ __device__ __forceinline__ int4 ld_cluster(uint32_t addr) {
     return v;
 }
 
-// One output tile of 128 channels x BT rows per cluster of S CTAs (grid: S x
-// channel tiles x row tiles). Each CTA sums its share of k in TMEM. With S = 1
-// a thread owns a channel and stores its column of the tile straight from TMEM
-// (a warp's stores of one row are neighbours); with more, every CTA leaves its
-// int32 tile in shared memory (over the pipeline's buffers, which are done) and
-// sums BT / S of the rows over the cluster, four channels a lane.
+// Output tiles of 128 channels x BT rows. With S = 1 the CTAs are persistent:
+// each takes every gridDim.x-th tile, its loads running on into the next tile
+// while the epilogue empties the last one (two accumulators in TMEM). A thread
+// of the epilogue owns a channel and stores its column of the tile straight
+// from TMEM (a warp's stores of one row are neighbours). With S > 1 a cluster
+// of S CTAs makes one tile, each summing its share of k; every CTA leaves its
+// int32 tile in shared memory (over the pipeline's buffers, which are done)
+// and sums BT / S of the rows over the cluster, four channels a lane.
 template <int BT, int S, class T>
 static __global__ void __launch_bounds__(kWideThreads)
     gemm_int8_wide_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
-                          const __grid_constant__ GemmParams p, uint32_t stages) {
+                          const __grid_constant__ GemmParams p, uint32_t stages, uint32_t n_rt, uint32_t tiles) {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * kWideMaxStages + 1];
-    __shared__ float row_scales[BT];
+    // full and empty of every stage, then full and empty of both accumulators
+    __shared__ __align__(8) uint64_t bars[2 * kWideMaxStages + 4];
+    __shared__ float row_scales[4][BT];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     volatile int* const abort_flag = &abort_word;
     constexpr uint32_t kWBytes = kWideChannels * kGemmStageK;
     constexpr uint32_t kStageBytes = kWBytes + BT * kGemmStageK;
-    constexpr uint32_t kTmemCols = BT < 32 ? 32 : BT;
+    constexpr uint32_t kAccCols = BT < 32 ? 32 : BT;  // the epilogue reads 32 columns at a time
+    constexpr uint32_t kTmemCols = S == 1 ? 2 * kAccCols : kAccCols;
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t sbase = (raw + 1023u) & ~1023u;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    const uint32_t split = S == 1 ? 0u : blockIdx.x;  // = rank in the cluster
-    const uint32_t n0 = blockIdx.y * kWideChannels, m0 = blockIdx.z * BT;
+    const uint32_t split = S == 1 ? 0u : blockIdx.x % S;  // = rank in the cluster
+    const uint32_t tile0 = blockIdx.x / S, step = gridDim.x / S;
     const uint32_t kblocks = (p.k + kGemmStageK - 1u) / kGemmStageK;
     const uint32_t kb0 = static_cast<uint32_t>(static_cast<uint64_t>(kblocks) * split / S);
     const uint32_t kb1 = static_cast<uint32_t>(static_cast<uint64_t>(kblocks) * (split + 1u) / S);
     const uint32_t bar0 = smem_u32(bars);
     auto full = [&](uint32_t s) { return bar0 + 8u * s; };
     auto empty = [&](uint32_t s) { return bar0 + 8u * (kWideMaxStages + s); };
-    const uint32_t done = bar0 + 8u * (2 * kWideMaxStages);
+    auto tfull = [&](uint32_t a) { return bar0 + 8u * (2 * kWideMaxStages + a); };
+    auto tempty = [&](uint32_t a) { return bar0 + 8u * (2 * kWideMaxStages + 2 + a); };
 
     if (threadIdx.x == 0) {
         tma_prefetch_desc(&tm_w);
@@ -235,7 +240,10 @@ static __global__ void __launch_bounds__(kWideThreads)
             mbar_init(full(s), 1);
             mbar_init(empty(s), 1);
         }
-        mbar_init(done, 1);
+        for (uint32_t a = 0; a < 2; ++a) {
+            mbar_init(tfull(a), 1);
+            mbar_init(tempty(a), 4);
+        }
         abort_word = 0;
         fence_mbarrier_init();
     }
@@ -248,36 +256,40 @@ static __global__ void __launch_bounds__(kWideThreads)
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     await_previous();
-
-    // The scales and the bias arrive while the sums are made.
-    constexpr int kOwn = S == 1 ? 1 : 4;  // channels of a thread
-    const uint32_t row = (warp & 3u) * 32u + lane;  // TMEM lane = channel of the tile
-    const uint32_t n = n0 + (S == 1 ? row : lane * 4u);
-    float sb[kOwn], bias[kOwn];
-    if (warp >= 2) {
-        for (uint32_t r = threadIdx.x - 64u; r < BT; r += kWideThreads - 64u)
-            row_scales[r] = m0 + r < p.m ? p.a_scales[m0 + r] : 0.0f;
-    }
+    T* const out = static_cast<T*>(p.out);
+    // Of a cluster's sums, the four channels of a lane: fetched while they are made.
+    float sb4[4], bias4[4];
+    if constexpr (S > 1) {
+        const uint32_t n = tile0 / n_rt * kWideChannels + lane * 4u;
 #pragma unroll
-    for (int c = 0; c < kOwn; ++c) {
-        sb[c] = n + c < p.n ? p.b_scales[n + c] : 0.0f;
-        bias[c] = n + c < p.n && p.bias != nullptr ? bias_at(p.bias, p.bias_type, n + c) : 0.0f;
+        for (int c = 0; c < 4; ++c) {
+            sb4[c] = n + c < p.n ? p.b_scales[n + c] : 0.0f;
+            bias4[c] = n + c < p.n && p.bias != nullptr ? bias_at(p.bias, p.bias_type, n + c) : 0.0f;
+        }
     }
 
     if (warp == 0) {
         if (elect_one_sync()) {
             uint32_t stage = 0, phase = 0, issued_mask = 0, issued_parity = 0;
-            for (uint32_t kb = kb0; kb < kb1; ++kb) {
-                if (!mbar_wait(empty(stage), phase ^ 1u, abort_flag)) break;
-                mbar_arrive_expect_tx(full(stage), kStageBytes);
-                const uint32_t dst = sbase + stage * kStageBytes;
-                tma_load_2d(dst, &tm_w, full(stage), static_cast<int32_t>(kb * kGemmStageK), static_cast<int32_t>(n0));
-                tma_load_2d(dst + kWBytes, &tm_x, full(stage), static_cast<int32_t>(kb * kGemmStageK), static_cast<int32_t>(m0));
-                issued_mask |= 1u << stage;
-                issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
-                if (++stage == stages) {
-                    stage = 0;
-                    phase ^= 1u;
+            bool ok = true;
+            for (uint32_t t = tile0; ok && t < tiles; t += step) {
+                const int32_t n0 = static_cast<int32_t>(t / n_rt * kWideChannels), m0 = static_cast<int32_t>(t % n_rt * BT);
+                for (uint32_t kb = kb0; kb < kb1; ++kb) {
+                    if (!mbar_wait(empty(stage), phase ^ 1u, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    mbar_arrive_expect_tx(full(stage), kStageBytes);
+                    const uint32_t dst = sbase + stage * kStageBytes;
+                    const int32_t x = static_cast<int32_t>(kb * kGemmStageK);
+                    tma_load_2d(dst, &tm_w, full(stage), x, n0);
+                    tma_load_2d(dst + kWBytes, &tm_x, full(stage), x, m0);
+                    issued_mask |= 1u << stage;
+                    issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
+                    if (++stage == stages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
                 }
             }
             land_loads(bar0, issued_mask, issued_parity);
@@ -285,55 +297,82 @@ static __global__ void __launch_bounds__(kWideThreads)
     } else if (warp == 1) {
         if (elect_one_sync()) {
             constexpr uint32_t idesc = make_idesc(2, 1, kWideChannels, BT);
-            uint32_t stage = 0, phase = 0;
-            for (uint32_t kb = kb0; kb < kb1; ++kb) {
-                if (!mbar_wait(full(stage), phase, abort_flag)) break;
+            uint32_t stage = 0, phase = 0, iter = 0;
+            bool ok = true;
+            for (uint32_t t = tile0; ok && t < tiles; t += step, ++iter) {
+                const uint32_t acc = iter & 1u;
+                if (!mbar_wait(tempty(acc), ((iter >> 1) & 1u) ^ 1u, abort_flag)) break;
                 tc_fence_after();
-                const uint32_t w = sbase + stage * kStageBytes, x = w + kWBytes;
+                for (uint32_t kb = kb0; kb < kb1; ++kb) {
+                    if (!mbar_wait(full(stage), phase, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t w = sbase + stage * kStageBytes, x = w + kWBytes;
 #pragma unroll
-                for (uint32_t k = 0; k < 4; ++k)
-                    tc_mma<MmaKind::I8>(tmem, smem_desc_k128(w + 32u * k), smem_desc_k128(x + 32u * k), idesc,
-                                        kb == kb0 && k == 0 ? 0u : 1u);
-                tc_commit(empty(stage));
-                if (++stage == stages) {
-                    stage = 0;
-                    phase ^= 1u;
+                    for (uint32_t k = 0; k < 4; ++k)
+                        tc_mma<MmaKind::I8>(tmem + acc * kAccCols, smem_desc_k128(w + 32u * k), smem_desc_k128(x + 32u * k),
+                                            idesc, kb == kb0 && k == 0 ? 0u : 1u);
+                    tc_commit(empty(stage));
+                    if (++stage == stages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
                 }
+                // Also after an abort: the epilogue waits for what was issued.
+                tc_commit(tfull(acc));
             }
-            tc_commit(done);
         }
-    }
-    __syncwarp();
-    // Every warp waits for the sums: after this no load and no MMA is under
-    // way and the pipeline's buffers are free.
-    const bool ok = finish_wait(done, 0) && *abort_flag == 0;
-    __syncthreads();  // row_scales
-    tc_fence_after();
-    T* const out = static_cast<T*>(p.out);
-    if (warp >= 2) {
-        const uint32_t taddr = tmem + (((warp & 3u) * 32u) << 16);
-        const uint32_t rows = ok && m0 < p.m && n < p.n ? min(static_cast<uint32_t>(BT), p.m - m0) : 0u;
-        T* dst = out + static_cast<int64_t>(m0) * p.out_pitch + n;
-#pragma unroll 1
-        for (uint32_t c = 0; c < BT; c += 32) {
-            uint32_t v[32];
-            __syncwarp();
-            tmem_ld_32x32b_x32(taddr + c, v);
-            tmem_wait_ld();
-            if (kb0 == kb1) {
-#pragma unroll
-                for (uint32_t i = 0; i < 32; ++i) v[i] = 0;
+    } else {
+        const uint32_t quad = warp & 3u, row = quad * 32u + lane;  // TMEM lane = channel of the tile
+        float* const scales = row_scales[quad];
+        uint32_t iter = 0;
+        for (uint32_t t = tile0; t < tiles; t += step, ++iter) {
+            const uint32_t acc = iter & 1u;
+            const uint32_t m0 = t % n_rt * BT, n = t / n_rt * kWideChannels + row;
+            const uint32_t rows = m0 < p.m ? min(static_cast<uint32_t>(BT), p.m - m0) : 0u;
+            const bool valid = n < p.n;
+            for (uint32_t r = lane; r < BT; r += 32) scales[r] = r < rows ? p.a_scales[m0 + r] : 0.0f;
+            float sb = 0.0f, bias = 0.0f;
+            if (S == 1 && valid) {
+                sb = p.b_scales[n];
+                if (p.bias != nullptr) bias = bias_at(p.bias, p.bias_type, n);
             }
+            __syncwarp();
+            bool ok = mbar_wait(tfull(acc), (iter >> 1) & 1u, abort_flag);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t taddr = tmem + ((quad * 32u) << 16) + acc * kAccCols;
+            T* dst = out + static_cast<int64_t>(m0) * p.out_pitch + n;
+#pragma unroll 1
+            for (uint32_t c = 0; c < BT; c += 32) {
+                uint32_t v[32];
+                __syncwarp();
+                tmem_ld_32x32b_x32(taddr + c, v);
+                tmem_wait_ld();
+                if (S == 1 && c + 32 >= BT) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(tempty(acc));
+                }
+                if (kb0 == kb1) {
 #pragma unroll
-            for (uint32_t i = 0; i < (BT < 32 ? BT : 32); ++i) {
-                if constexpr (S == 1) {
-                    const T o = from_f32<T>(scaled(static_cast<int32_t>(v[i]), row_scales[c + i], sb[0], bias[0]));
-                    if (c + i < rows) *dst = o;
-                    dst += p.out_pitch;
-                } else {
-                    *reinterpret_cast<uint32_t*>(smem_raw + (sbase - raw) + ((c + i) * kWideChannels + row) * 4u) = v[i];
+                    for (uint32_t i = 0; i < 32; ++i) v[i] = 0;
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < (BT < 32 ? BT : 32); ++i) {
+                    if constexpr (S == 1) {
+                        const T o = from_f32<T>(scaled(static_cast<int32_t>(v[i]), scales[c + i], sb, bias));
+                        if (valid && c + i < rows) *dst = o;
+                        dst += p.out_pitch;
+                    } else {
+                        *reinterpret_cast<uint32_t*>(smem_raw + (sbase - raw) + ((c + i) * kWideChannels + row) * 4u) = v[i];
+                    }
                 }
             }
+            __syncwarp();
         }
     }
     // TMEM goes back before this CTA waits for the others of its cluster: a CTA
@@ -348,6 +387,7 @@ static __global__ void __launch_bounds__(kWideThreads)
     if constexpr (S > 1) {
         __syncwarp();
         cluster_sync();
+        const uint32_t m0 = tile0 % n_rt * BT, n = tile0 / n_rt * kWideChannels + lane * 4u;
         // Rows r of the tile with r % S == split, one warp per row and step.
         for (uint32_t r = split + S * warp; r < BT && m0 + r < p.m; r += S * (kWideThreads / 32)) {
             const uint32_t at = sbase + (r * kWideChannels + lane * 4u) * 4u;
@@ -364,7 +404,7 @@ static __global__ void __launch_bounds__(kWideThreads)
             }
             T o[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) o[c] = from_f32<T>(scaled(sum[c], row_scales[r], sb[c], bias[c]));
+            for (int c = 0; c < 4; ++c) o[c] = from_f32<T>(scaled(sum[c], row_scales[0][r], sb4[c], bias4[c]));
             T* dst = out + static_cast<int64_t>(m0 + r) * p.out_pitch + n;
             if (p.out_vec4 && n + 4u <= p.n) {
                 if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(o);
