@@ -387,16 +387,18 @@ void launch_wide(const GemmParams& p, int num_sms, uint32_t splits, cudaStream_t
 template <class T>
 void launch_pair(const GemmParams& p, int num_sms, cudaStream_t stream) {
     const uint32_t n_mt = cdiv(p.m, kPairM), n_nt = cdiv(p.n, kPairN);
-    if (static_cast<uint64_t>(n_mt) * n_nt > 0x7FFFFFFFull) bad("too many rows in one call");
+    if (static_cast<uint64_t>(n_mt) * n_nt > 0x3FFFFFFFull) bad("too many rows in one call");
     const CUtensorMap ma = code_map(p.a, p.a_pitch, p.m, p.k, kPairM / 2);
-    const CUtensorMap mb = code_map(p.b, p.b_pitch, p.n, p.k, kPairN / 2);
+    const CUtensorMap mb = code_map(p.b, p.b_pitch, p.n, p.k, kPairN / 4);
     constexpr uint32_t smem = kPairSmemBytes;
     allow_dynamic_smem(reinterpret_cast<const void*>(gemm_int8_pair_kernel<T>), smem);
-    const uint32_t pairs = std::min<uint32_t>(n_mt * n_nt, static_cast<uint32_t>(num_sms) / 2);
+    const uint32_t all = static_cast<uint32_t>(num_sms) / 2, tiles = n_mt * n_nt, last = tiles % all;
+    const uint32_t whole = 2 * last <= all ? tiles - last : tiles, units = whole + 2 * (tiles - whole);
+    const uint32_t pairs = std::min(units, all);
     LaunchConfig cfg(dim3(pairs * 2), kPairThreads, smem, stream);
     cfg.clusters_of(2);
     if (p.after_previous) cfg.after_previous();
-    cfg.launch(gemm_int8_pair_kernel<T>, ma, mb, p, n_mt, n_nt);
+    cfg.launch(gemm_int8_pair_kernel<T>, ma, mb, p, n_mt, n_nt, whole, units);
 }
 
 // The form a product takes: rows per tile of the wide kernel (0: the pair
@@ -416,7 +418,7 @@ struct GemmForm {
 //    stores (0.02 a row, a quarter more to fp32).
 //  * pair: 4.5 for the launch and its ends, then waves of tiles at 0.36 per
 //    128 of k (1670 T products/s, the tensor cores' pace at this power) + 1.2,
-//    2.4 at least, 0.8 more to fp32.
+//    2.4 at least, 0.8 more to fp32; 0.7 of that for a last wave of half tiles.
 // E.g. 512 x 4096 x 4096: wide of 128 rows 12.6 us, pair 16.3; 1024 x 4096 x
 // 4096: 19.1 and 16.9; 64 x 100,000 x 384 to fp32: 14.5 (64 rows) and 23.2;
 // 10,000 x 1536 x 768: 21.5 and 16.9.
@@ -427,9 +429,10 @@ GemmForm gemm_form(uint32_t m, uint32_t n, uint32_t k, bool fp32, int num_sms) {
     GemmForm best{0, 1};
     double least = 1e30;
     if (kb > 0) {
-        const uint64_t tiles = static_cast<uint64_t>(cdiv(m, kPairM)) * cdiv(n, kPairN);
+        const uint64_t pairs = num_sms / 2, tiles = static_cast<uint64_t>(cdiv(m, kPairM)) * cdiv(n, kPairN);
+        const double last = tiles % pairs == 0 ? 0 : 2 * (tiles % pairs) <= pairs ? 0.7 : 1;
         const double each = std::max(kb * 0.36 + 1.2, 2.4) + (fp32 ? 0.8 : 0);
-        least = 4.5 + static_cast<double>((tiles + num_sms / 2 - 1) / (num_sms / 2)) * each;
+        least = 4.5 + (static_cast<double>(tiles / pairs) + last) * each;
     }
     for (uint32_t rows = 16; rows <= 128; rows *= 2) {
         const uint64_t tiles = static_cast<uint64_t>(cdiv(n, kWideChannels)) * cdiv(m, rows);

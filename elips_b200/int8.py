@@ -238,18 +238,17 @@ def _cache(codes, scales, written: bool):
 
 def _rows(tensors, count: int, heads: int, dim: int, dtype, what: str, written: bool):
     """The packed elips_b200_rows of a part's rows [count, heads, dim], for each part."""
-    packed = []
+    want, packed = (count, heads, dim), []
     for x in tensors:
-        shape = x.shape
-        if len(shape) != 3 or shape[0] != count or shape[1] != heads or shape[2] != dim:
-            raise DimensionMismatch(f"{what} must be [{count}, {heads}, {dim}], not {list(shape)}")
+        if x.shape != want:
+            raise DimensionMismatch(f"{what} must be {list(want)}, not {list(x.shape)}")
         if x.dtype is not dtype:
             raise ValueError(f"{what} must be {dtype}, not {x.dtype}")
         s0, s1, s2 = strides = x.stride()
         if s2 != 1 and dim > 1:
             raise ValueError(f"{what} must have their last axis contiguous")
         if written:
-            _distinct(strides, shape, what)
+            _distinct(strides, want, what)
         packed += (x.data_ptr(), s0, s1)
     return _ROWS[len(tensors)].pack(*packed)
 
@@ -277,9 +276,9 @@ def cache_write(codes, scales, rows, slots, stream=None) -> None:
     if len(rows) != parts:
         raise DimensionMismatch(f"{len(rows)} tensors of rows for a cache of {parts} parts")
     wide = _indexes(slots, "slots")
-    if slots.dim() != 1 or (slots.shape[0] > 1 and slots.stride(0) != 1):
+    if slots.dim() != 1 or not slots.is_contiguous():
         raise DimensionMismatch("slots must be one contiguous axis")
-    t = slots.shape[0]
+    t = slots.numel()
     dtype = rows[0].dtype
     kind = _float_type(dtype, "rows")
     packed = _rows(rows, t, heads, dim, dtype, "rows", False)
@@ -311,11 +310,12 @@ def cache_read(codes, scales, page_table, offsets, total: int, dtype=torch.bfloa
     the result, of any strides but the last) stay as they are."""
     cache, parts, heads, dim = _cache(codes, scales, False)
     table_wide, offsets_wide = _indexes(page_table, "page_table"), _indexes(offsets, "offsets")
-    if page_table.dim() != 2 or offsets.dim() != 1 or offsets.shape[0] != page_table.shape[0] + 1:
+    shape = page_table.shape
+    if len(shape) != 2 or offsets.shape != (shape[0] + 1,):
         raise DimensionMismatch("offsets must have one entry more than page_table has rows")
-    sequences, width = page_table.shape
+    sequences, width = shape
     table_stride, step = page_table.stride()
-    if (width > 1 and step != 1) or (sequences > 0 and offsets.stride(0) != 1):
+    if (width > 1 and step != 1) or not offsets.is_contiguous():
         raise ValueError("page_table rows and offsets must be contiguous")
     total = int(total)
     if total < 0:
@@ -338,9 +338,15 @@ def cache_read(codes, scales, page_table, offsets, total: int, dtype=torch.bfloa
         with _using(stream, device, codes, scales, page_table, offsets, *(out or ())):
             return cache_read(codes, scales, page_table, offsets, total, dtype, out)
     if fresh:
-        out = tuple(codes.new_empty((total, heads, dim), dtype=dtype) for _ in range(parts))
-        first = (heads * dim, dim)
-        packed = _ROWS[parts].pack(*(v for x in out for v in (x.data_ptr(), *first)))
+        size, row = (total, heads, dim), heads * dim
+        first = codes.new_empty(size, dtype=dtype)
+        if parts == 1:
+            out = (first,)
+            packed = _ROWS[1].pack(first.data_ptr(), row, dim)
+        else:
+            second = codes.new_empty(size, dtype=dtype)
+            out = (first, second)
+            packed = _ROWS[2].pack(first.data_ptr(), row, dim, second.data_ptr(), row, dim)
     seqs = _SEQUENCES.pack(page_table.data_ptr(), offsets.data_ptr(), table_stride, sequences, width, total, table_wide,
                            offsets_wide)
     status = _LIB.elips_b200_cache_read(device, cache, seqs, packed, kind, fresh, _raw_stream(device))
