@@ -209,8 +209,8 @@ static __global__ void __launch_bounds__(kWideThreads)
     gemm_int8_wide_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
                           const __grid_constant__ GemmParams p, uint32_t stages, uint32_t n_rt, uint32_t tiles) {
     extern __shared__ uint8_t smem_raw[];
-    // full and empty of every stage, then full and empty of both accumulators
-    __shared__ __align__(8) uint64_t bars[2 * kWideMaxStages + 4];
+    // full and empty of every stage, full and empty of both accumulators, all MMAs done
+    __shared__ __align__(8) uint64_t bars[2 * kWideMaxStages + 5];
     __shared__ float row_scales[4][BT];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
@@ -232,6 +232,7 @@ static __global__ void __launch_bounds__(kWideThreads)
     auto empty = [&](uint32_t s) { return bar0 + 8u * (kWideMaxStages + s); };
     auto tfull = [&](uint32_t a) { return bar0 + 8u * (2 * kWideMaxStages + a); };
     auto tempty = [&](uint32_t a) { return bar0 + 8u * (2 * kWideMaxStages + 2 + a); };
+    const uint32_t done = bar0 + 8u * (2 * kWideMaxStages + 4);
 
     if (threadIdx.x == 0) {
         tma_prefetch_desc(&tm_w);
@@ -244,6 +245,7 @@ static __global__ void __launch_bounds__(kWideThreads)
             mbar_init(tfull(a), 1);
             mbar_init(tempty(a), 4);
         }
+        mbar_init(done, 1);
         abort_word = 0;
         fence_mbarrier_init();
     }
@@ -320,9 +322,12 @@ static __global__ void __launch_bounds__(kWideThreads)
                         phase ^= 1u;
                     }
                 }
-                // Also after an abort: the epilogue waits for what was issued.
+                if (!ok) break;
                 tc_commit(tfull(acc));
             }
+            // Nothing writes to TMEM once it is freed, whatever ended the loop.
+            tc_commit(done);
+            finish_wait(done, 0);
         }
     } else {
         const uint32_t quad = warp & 3u, row = quad * 32u + lane;  // TMEM lane = channel of the tile

@@ -611,7 +611,9 @@ typedef struct {
 } elips_b200_gemm;
 
 /* out[i][j] = (sum_l a[i][l] * b[j][l]) * a_scales[i] * b_scales[j] + bias[j],
- * rounded once to out_type; the sum is exact in int32 (k < 2^17). */
+ * the sum exact in int32 (k < 2^17), the rest in fp32 in this order, rounded
+ * once to out_type. The order of the sum does not matter, so the same inputs
+ * always give the same bits. */
 ELIPS_B200_API int elips_b200_gemm_int8(int device, const elips_b200_gemm* args, void* stream);
 
 /* A paged cache of quantised rows: codes [parts][pages][page_size][heads][dim]
