@@ -100,19 +100,27 @@ void launch_rows(const QuantParams& p, cudaStream_t stream) {
 
 // Few threads with many accesses each: what a thread spends on finding its row
 // is shared by more values, and up to 512 accesses a row needs no more than a
-// warp. Wider rows take a block.
+// warp. Wider rows take a block (1000 x 30,000 bf16: 26.2 us read twice with
+// four accesses a thread, 17.4 held in sixteen), and so do rows too few to
+// fill the SMs, whose time is that of one row (1 x 4096 bf16: 3.1 us with a
+// warp, 1.7 with a block).
 template <class T, int V>
 void launch_rows_of(const QuantParams& p, cudaStream_t stream) {
     const uint32_t n = (p.d + V - 1) / V;  // accesses per row
+    const bool few = p.groups <= 1024;
     if constexpr (V > 1) {
         if (n <= 8) return launch_rows<T, V, 4, 2>(p, stream);
         if (n <= 16) return launch_rows<T, V, 4, 4>(p, stream);
+    } else {
+        if (n > 512 && n <= 1024 && !few) return launch_rows<T, V, 32, 32>(p, stream);
     }
     if (n <= 32) launch_rows<T, V, 8, 4>(p, stream);
+    else if (n > 64 && n <= 512 && few) launch_rows<T, V, 256, 2>(p, stream);
     else if (n <= 128) launch_rows<T, V, 32, 4>(p, stream);
     else if (n <= 256) launch_rows<T, V, 32, 8>(p, stream);
     else if (n <= 512) launch_rows<T, V, 32, 16>(p, stream);
-    else launch_rows<T, V, 256, 4>(p, stream);
+    else if (n <= 1024) launch_rows<T, V, 256, 4>(p, stream);
+    else launch_rows<T, V, 256, 16>(p, stream);
 }
 
 // fn(first row, groups) for runs of rows whose (part, head) groups are fewer
