@@ -92,6 +92,8 @@ static __global__ void __launch_bounds__(256) gemm_int8_dot_kernel(const __grid_
 #pragma unroll
     for (int c = 0; c < kDotChannels; ++c) br[c] = p.b + static_cast<int64_t>(min(n0 + c, p.n - 1u)) * p.b_pitch;
     __shared__ float row_scales[kFloat ? MR : 1];
+    await_previous();
+    let_next_start();
     if constexpr (kFloat) {
         __shared__ uint32_t warp_max[8];
         // The first weights are on their way while the rows are quantised.
@@ -258,6 +260,7 @@ static __global__ void __launch_bounds__(kWideThreads)
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     await_previous();
+    let_next_start();
     T* const out = static_cast<T*>(p.out);
     // Of a cluster's sums, the four channels of a lane: fetched while they are made.
     float sb4[4], bias4[4];
@@ -543,6 +546,7 @@ static __global__ void __launch_bounds__(kPairThreads, 1)
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     await_previous();
+    let_next_start();
 
     if (warp == 0) {
         if (elect_one_sync()) {
@@ -742,6 +746,7 @@ struct RepackParams {
 };
 
 static __global__ void __launch_bounds__(256) repack_codes_kernel(const __grid_constant__ RepackParams p) {
+    await_previous();
     let_next_start();
     const uint32_t which = blockIdx.y;
     const uint32_t rows = which ? p.rows[1] : p.rows[0];

@@ -230,11 +230,13 @@ __device__ __forceinline__ void group_at(const QuantParams& p, uint32_t g, uint3
     head = r - part * p.heads;
 }
 
-// Programmatic dependent launch: a kernel of a call may start while the call's
-// previous kernel ends. await_previous() returns once that one is complete and
-// its writes are seen; everything it made is read, and everything it reads is
-// written, after that. The first kernel of a call is launched plainly, so
-// what other work left in the stream is complete before any of them starts.
+// Programmatic dependent launch: a kernel may start while the one before it in
+// the stream ends. Every kernel here waits with await_previous() until that one
+// is complete and its writes are seen before it reads or writes global memory,
+// and only then lets the next one start (let_next_start), so whatever a kernel
+// finds running has itself seen the end of all before it. The one exception:
+// a cache write after its claims reads rows and slots first, which nothing in
+// between writes.
 __device__ __forceinline__ void await_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -252,6 +254,7 @@ constexpr uint32_t kDupScanRows = 256;
 __device__ __forceinline__ uint32_t claim_of(uint32_t t) { return 0x80000001u + t; }
 
 static __global__ void __launch_bounds__(256) cache_claim_kernel(const __grid_constant__ QuantParams p) {
+    await_previous();
     let_next_start();
     const uint32_t g = blockIdx.x * 256u + threadIdx.x;
     if (g >= p.groups) return;
@@ -287,6 +290,7 @@ template <class T, int V, int G, int NV, bool CACHE>
 static __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_constant__ QuantParams p) {
     __shared__ uint32_t block_max[8];
     constexpr uint32_t kHeld = G * NV * V;
+    if (!CACHE || p.dup != kDupClaim) await_previous();
     const uint32_t gl = threadIdx.x % G;
     const uint32_t g = blockIdx.x * (256 / G) + threadIdx.x / G;
     uint32_t t = p.t0 + g, part = 0, head = 0, slot = t;
@@ -321,7 +325,6 @@ static __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_
         if (e < p.d && keep) v[j].load(x + e);
         else v[j].zero();
     }
-    let_next_start();
     if constexpr (CACHE) {
         if (p.dup == kDupClaim) {
             // The row's own claim stands until it stores its scale below.
@@ -331,6 +334,7 @@ static __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_
             for (uint32_t i = t + 1u + gl; i < p.t; i += G) keep = keep && slot_of(p, i) != static_cast<int64_t>(slot);
         }
     }
+    let_next_start();
     uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < NV; ++j) top = v[j].top(top);
@@ -492,6 +496,8 @@ constexpr int kReadBatch = 8;           // accesses a thread has under way
 template <class T, int V>
 static __global__ void __launch_bounds__(kReadThreads) cache_read_kernel(const __grid_constant__ ReadParams p) {
     __shared__ longlong2 row_at[kReadRows];  // where a row's codes and scales start; x below 0: it has none
+    await_previous();
+    let_next_start();
     const uint32_t t0 = blockIdx.x * p.rows, rows = min(p.rows, p.total - t0);
     if (threadIdx.x < rows) {
         const int64_t s = read_slot(p, t0 + threadIdx.x);
@@ -558,7 +564,6 @@ struct GemmParams {
     int64_t out_pitch;  // elements
     uint32_t m, n, k;
     int out_vec4, out_vec16;  // rows of out start on four elements, on 16 bytes
-    int after_previous;       // a was made by the launch before (await_previous)
     // Rows that the product quantises itself (the dot kernel), in place of a:
     const void* x;
     int64_t x_pitch;  // elements
