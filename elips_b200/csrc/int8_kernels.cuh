@@ -264,13 +264,14 @@ static __global__ void __launch_bounds__(256) cache_claim_kernel(const __grid_co
     if (s < 0 || s >= p.num_slots) return;
     uint32_t* const w = reinterpret_cast<uint32_t*>(scale_at(p, part, static_cast<uint32_t>(s), head));
     const uint32_t claim = claim_of(t);
-    uint32_t old = *reinterpret_cast<volatile uint32_t*>(w);
-    for (;;) {
+    uint32_t old = atomicMax(w, claim);
+    // Mostly done: the word held a scale or an earlier claim. Else a later
+    // row's claim, which stands, or a number that is none, which does not.
+    while (old > claim) {
         const uint32_t other = old - claim_of(0);  // the row that `old` would be the claim of
-        if (other < p.t && other >= t && slot_of(p, other) == s) return;
-        const uint32_t seen = atomicCAS(w, old, claim);
-        if (seen == old) return;
-        old = seen;
+        if (other < p.t && slot_of(p, other) == s) return;
+        if (atomicCAS(w, old, claim) == old) return;
+        old = atomicMax(w, claim);  // another row's claim came first
     }
 }
 
