@@ -57,20 +57,20 @@ void with_float_type(int type, Fn&& fn) {
     }
 }
 
-// A launch that may start while the kernel before it in the stream ends; it
-// waits for that one itself (await_previous). After another call of the same
-// kind: 64 x 100,000 x 384 scores 14.3 -> 12.0 us, prompts through a cache 45.7
-// -> 41.5, new tokens in a graph 5.4 -> 4.7.
+// A launch that may start while the kernel before it in the stream ends
+// (early); it waits for that one itself (await_previous). After another call of
+// the same kind: 64 x 100,000 x 384 scores 14.3 -> 12.0 us, prompts through a
+// cache 45.7 -> 41.5, new tokens in a graph 5.4 -> 4.7.
 struct LaunchConfig {
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[2];
-    LaunchConfig(dim3 grid, uint32_t threads, size_t smem, cudaStream_t stream) {
+    LaunchConfig(dim3 grid, uint32_t threads, size_t smem, cudaStream_t stream, bool early = true) {
         cfg.gridDim = grid;
         cfg.blockDim = dim3(threads);
         cfg.dynamicSmemBytes = smem;
         cfg.stream = stream;
         cfg.attrs = attr;
-        cfg.numAttrs = 1;
+        cfg.numAttrs = early ? 1 : 0;
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
     }
@@ -345,9 +345,12 @@ void launch_dot_rows(const GemmParams& p, int num_sms, cudaStream_t stream) {
     const uint64_t groups = cdiv(p.n, kDotChannels);
     uint32_t wk = 1;
     while (wk < 8 && groups * wk < static_cast<uint64_t>(num_sms) * 16 && p.k > wk * 512u) wk *= 2;
-    const size_t smem = std::is_same<X, int8_t>::value ? 0 : static_cast<size_t>(p.m) * ((p.k + 15u) / 16u * 16u);
+    // Blocks that quantise their rows are spread over the SMs only by a plain
+    // launch (1 x 4096 x 4096 after another, weights in L2: 4.4 us, early 5.3).
+    constexpr bool codes = std::is_same<X, int8_t>::value;
+    const size_t smem = codes ? 0 : static_cast<size_t>(p.m) * ((p.k + 15u) / 16u * 16u);
     const uint32_t blocks = blocks_for(groups * wk, 8);
-    LaunchConfig cfg(dim3(blocks), 256, smem, stream);
+    LaunchConfig cfg(dim3(blocks), 256, smem, stream, codes);
     cfg.launch(gemm_int8_dot_kernel<MR, X, T>, p, wk);
     launch_ok("int8 product launch");
 }
