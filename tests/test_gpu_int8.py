@@ -622,6 +622,43 @@ def test_captured_and_replayed(t):
         assert all(torch.equal(x, y) for x, y in zip(out, want))
 
 
+@pytest.mark.parametrize("t", [3, 300])
+def test_captured_over_two_streams(t):
+    """A graph whose calls fork to a second stream and meet again, with copies and fills between them."""
+    from elips_b200 import int8
+    st = state(t, 5)
+    w2 = operand(rng(t, 6), 200, 96, 16)
+    sw2 = torch.rand(200, device="cuda")
+
+    def step():
+        main, side = torch.cuda.current_stream(), torch.cuda.Stream()
+        x = st["x"].clone()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            right = int8.linear_int8(x, w2, sw2)
+            int8.cache_write(st["codes"], st["scales"], (right[:, :128].view(t, 2, 64), right[:, 64:192].view(t, 2, 64)),
+                             st["slots"])
+        codes, scales = int8.quantize_rows(x)
+        left = int8.gemm_int8(codes, w2, scales, sw2)
+        main.wait_stream(side)
+        keys, _ = int8.cache_read(st["codes"], st["scales"], st["table"], st["offsets"], t)
+        again, held = int8.quantize_rows(keys.view(t, 128))
+        out = torch.zeros((t, t), device="cuda")
+        return left, right, keys, int8.gemm_int8(again, again, held, held, out=out)
+
+    want = [y.clone() for y in step()]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    for _ in range(3):
+        for y in got:
+            y.fill_(1)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 @pytest.mark.parametrize("as_handle", [False, True])
 def test_on_another_stream(as_handle):
     """stream=: work is ordered on that stream, outputs belong to it, inputs may be dropped at once."""
@@ -639,10 +676,17 @@ def test_on_another_stream(as_handle):
     got = int8.linear_int8(y, w, sw, stream=handle)
     codes, held = int8.quantize_rows(y, stream=handle)
     scored = int8.gemm_int8(codes, w, held, sw, stream=handle)
-    del y
+    cache, scales = new_cache(1, 600, 1, 1, 512)
+    slots = torch.arange(600, device="cuda")
+    table, offsets = torch.arange(600, device="cuda")[None], torch.tensor([0, 600], device="cuda")
+    s.wait_stream(torch.cuda.current_stream())
+    int8.cache_write(cache, scales, (y[:, None],), slots, stream=handle)
+    back, = int8.cache_read(cache, scales, table, offsets, 600, torch.float32, stream=handle)
+    del y, slots, table, offsets
     noise = [torch.randn((600, 512), device="cuda").bfloat16() for _ in range(4)]
     s.synchronize()
     assert torch.equal(got, want) and torch.equal(scored, want) and len(noise) == 4
+    assert torch.equal(back[:, 0], codes.float() * held[:, None])
 
 
 def test_two_calls_at_once():
