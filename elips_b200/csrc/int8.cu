@@ -119,6 +119,31 @@ void launch_rows_of(const QuantParams& p, cudaStream_t stream) {
     else launch_rows<T, V, 256, 16>(p, stream);
 }
 
+template <class T, int G, int NV>
+void launch_shifted(const QuantParams& p, cudaStream_t stream) {
+    LaunchConfig cfg(dim3(blocks_for(p.groups, 256 / G)), 256, 0, stream);
+    cfg.launch(quantize_shifted_rows_kernel<T, 16 / static_cast<int>(sizeof(T)), G, NV>, p);
+}
+
+// Rows that start anywhere, by the accesses that one of them may span. False
+// where there are more than a block holds.
+template <class T>
+bool launch_shifted_of(const QuantParams& p, cudaStream_t stream) {
+    constexpr uint32_t V = 16 / sizeof(T);
+    const uint32_t n = (p.d + 2 * V - 2) / V;
+    const bool few = p.groups <= 1024;
+    if (n > 4096) return false;
+    if (n <= 16) launch_shifted<T, 4, 4>(p, stream);
+    else if (n <= 32) launch_shifted<T, 8, 4>(p, stream);
+    else if (n > 64 && n <= 512 && few) launch_shifted<T, 256, 2>(p, stream);
+    else if (n <= 128) launch_shifted<T, 32, 4>(p, stream);
+    else if (n <= 256) launch_shifted<T, 32, 8>(p, stream);
+    else if (n <= 512) launch_shifted<T, 32, 16>(p, stream);
+    else if (n <= 1024) launch_shifted<T, 256, 4>(p, stream);
+    else launch_shifted<T, 256, 16>(p, stream);
+    return true;
+}
+
 // fn(first row, groups) for runs of rows whose (part, head) groups are fewer
 // than 2^30, what one launch indexes.
 template <class Fn>
@@ -145,11 +170,13 @@ void launch_quantize(int type, QuantParams p, uint32_t parts, cudaStream_t strea
     with_float_type(type, [&](auto tag) {
         using T = decltype(tag);
         const bool whole = whole_accesses<T>(p, parts);
+        constexpr uint32_t V = 16 / sizeof(T);
+        const bool shifted = p.slots == nullptr && reinterpret_cast<uintptr_t>(p.codes) % V == 0 && p.code_page % V == 0;
         in_runs(p.t, p.per_t.d, [&](uint32_t t0, uint32_t groups) {
             p.t0 = t0;
             p.groups = groups;
             if (whole) launch_rows_of<T, 16 / sizeof(T)>(p, stream);
-            else launch_rows_of<T, 1>(p, stream);
+            else if (!shifted || !launch_shifted_of<T>(p, stream)) launch_rows_of<T, 1>(p, stream);
         });
     });
     launch_ok("row quantisation launch");
@@ -279,13 +306,16 @@ void launch_read(ReadParams p, const elips_b200_cache& c, int num_sms, cudaStrea
         const uint32_t with = cdiv(ny * p.nx, 32) * 32;
         if (with < 128 || static_cast<uint64_t>(ny * p.nx) * threads >= static_cast<uint64_t>(p.ny * p.nx) * with) p.ny = ny, threads = with;
     }
-    // Two batches of accesses a thread, and at least two blocks an SM.
-    uint64_t rows = std::min<uint64_t>(kReadRows, 2u * kReadBatch * p.ny);
-    rows = std::min<uint64_t>(rows, cdiv(p.total, 2u * static_cast<uint32_t>(num_sms)));
+    // Two batches of accesses a thread, the columns of wide rows in different
+    // blocks. Fewer rows make four blocks an SM as long as that leaves a thread
+    // three accesses, and one block an SM after that.
+    const uint32_t shares = std::min(cdiv(p.per_row, p.nx), 65535u);
+    const uint64_t work = static_cast<uint64_t>(p.total) * shares, sms = static_cast<uint32_t>(num_sms);
+    uint64_t rows = std::max(cdiv(work, 4 * sms), std::min(3u * p.ny, cdiv(work, sms)));
+    rows = std::min<uint64_t>(rows, std::min<uint64_t>(kReadRows, 2u * kReadBatch * p.ny));
     p.rows = static_cast<uint32_t>(rows);
     threads = std::max(threads, cdiv(p.rows, 32) * 32);
-    const uint32_t blocks = blocks_for(p.total, p.rows);
-    LaunchConfig cfg(dim3(blocks), threads, 0, stream);
+    LaunchConfig cfg(dim3(blocks_for(p.total, p.rows), shares), threads, 0, stream);
     cfg.launch(cache_read_kernel<T, V>, p);
 }
 

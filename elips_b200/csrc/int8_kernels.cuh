@@ -150,6 +150,20 @@ struct Access {
         if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
         else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
     }
+    // Zero for the elements outside [first, end).
+    __device__ __forceinline__ void keep_only(int first, int end) {
+        uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                if (i < first || i >= end) w[i] = 0;
+            } else {
+                if (2 * i < first || 2 * i >= end) w[i] &= 0xFFFF0000u;
+                if (2 * i + 1 < first || 2 * i + 1 >= end) w[i] &= 0x0000FFFFu;
+            }
+        }
+        raw = make_uint4(w[0], w[1], w[2], w[3]);
+    }
     // The larger of `top` (a magnitude, NaN above all) and those held.
     __device__ __forceinline__ uint32_t top(uint32_t top) const {
         if constexpr (sizeof(T) == 4) {
@@ -285,8 +299,7 @@ static __global__ void __launch_bounds__(256) cache_claim_kernel(const __grid_co
 // instructions: 16384 x 1024 bf16 takes 8.4 us (6.0 TB/s), 4096 x 4096 fp32
 // 13.6 us (6.2 TB/s), 10,000 x 768 fp32 7.6 us (5.0 TB/s, the launch a fourth
 // of it); with a check for halves in every 16-bit value and a block per wide
-// row the first took 13.2. Rows that start anywhere go value by value:
-// 10,000 x 767 bf16 11.3 us, 10,000 x 768 5.5.
+// row the first took 13.2.
 template <class T, int V, int G, int NV, bool CACHE>
 static __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_constant__ QuantParams p) {
     __shared__ uint32_t block_max[8];
@@ -405,6 +418,88 @@ static __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_
     if (gl == 0) *scale = rs.s;
 }
 
+// quantize_rows_kernel without a cache for rows that start anywhere: the 16-byte
+// accesses are those that hold the row (what they hold beside it is set to
+// zero; an access with one byte of the row is in memory wherever that byte
+// is), and the codes, which start `off` values into the first access, are
+// shifted into place through shared memory, so that they are stored V at a time
+// too. Codes start on V bytes. 10,000 x 767 bf16: 7.7 us, value by value 11.3
+// (10,000 x 768: 4.9); 60,000 x 67: 5.9 and 11.1.
+template <class T, int V, int G, int NV>
+static __global__ void __launch_bounds__(256) quantize_shifted_rows_kernel(const __grid_constant__ QuantParams p) {
+    using Word = typename std::conditional<V == 8, uint64_t, uint32_t>::type;  // V codes
+    __shared__ uint32_t block_max[8];
+    __shared__ Word words[256 * NV + 1];
+    await_previous();
+    let_next_start();
+    const uint32_t gl = threadIdx.x % G;
+    const uint32_t g = blockIdx.x * (256 / G) + threadIdx.x / G;
+    const bool there = g < p.groups;
+    const uint32_t t = p.t0 + g;
+    const T* const row = static_cast<const T*>(p.x[0]) + t * p.x_stride_t[0];
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) % 16u / sizeof(T));
+    const T* const x = row - off;
+    Word* const mine = words + threadIdx.x / G * (G * NV);
+
+    Access<T, V> v[NV];
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const uint32_t a = (j * G + gl) * V;  // its first element, counted from x
+        if (there && a < off + p.d) v[j].load(x + a);
+        else v[j].zero();
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int a = (j * G + gl) * V, first = static_cast<int>(off) - a, end = static_cast<int>(off + p.d) - a;
+        if (first > 0 || end < V) v[j].keep_only(first, end);
+        top = v[j].top(top);
+    }
+    uint32_t amax = Access<T, V>::bits32(top);
+    if constexpr (G == 256) {
+        amax = __reduce_max_sync(0xFFFFFFFFu, amax);
+        if ((threadIdx.x & 31u) == 0) block_max[threadIdx.x >> 5] = amax;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amax = max(amax, block_max[i]);
+    } else {
+#pragma unroll
+        for (int o = G / 2; o > 0; o /= 2) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+    }
+    const RowScale rs = make_scale<T>(amax);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        uint32_t w[V / 4] = {};
+        if (rs.inv != 0.0f) {
+            float f[V];
+            v[j].values(f);
+            row_codes<V>(f, rs, w);
+        }
+        if constexpr (V == 8) mine[j * G + gl] = static_cast<uint64_t>(w[V / 4 - 1]) << 32 | w[0];
+        else mine[j * G + gl] = w[0];
+    }
+    if constexpr (G == 256) __syncthreads();
+    else __syncwarp();
+    if (!there) return;
+    int8_t* const out = p.codes + t * p.code_page;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const uint32_t i = j * G + gl, e = i * V;
+        if (e >= p.d) continue;
+        // Where off is 0 the next word is not needed, and for a row's last word
+        // it holds nothing of the row: words[256 * NV] and the next row's are
+        // read for nothing.
+        Word w = mine[i] >> (8u * off);
+        if (off != 0u) w |= mine[i + 1] << (8u * (V - off));
+        if (e + V <= p.d) {
+            *reinterpret_cast<Word*>(out + e) = w;
+        } else {
+            for (uint32_t b = 0; e + b < p.d; ++b) out[e + b] = static_cast<int8_t>(w >> (8u * b));
+        }
+    }
+    if (gl == 0) p.scales[t] = rs.s;
+}
+
 // Reading pages back into packed rows. Sequence b owns the output rows
 // offsets[b] .. offsets[b + 1]; position i of it is slot page_table[b][i /
 // page] * page + i % page.
@@ -484,7 +579,8 @@ constexpr uint32_t kReadRows = 64;      // most output rows per block
 constexpr uint32_t kReadThreads = 512;  // most threads per block
 constexpr int kReadBatch = 8;           // accesses a thread has under way
 
-// A block reads `rows` output rows: first their slots, one thread each, then
+// A block reads `rows` output rows (a share of their columns, where they are
+// wide): first their slots, one thread each, then
 // the codes, V at a time (16 bytes of output where everything is aligned so
 // far). Its threads are `ny` times `nx`: neighbours on neighbouring codes of a
 // row, and each stays on its column (part, head and place in the row) while
@@ -513,7 +609,7 @@ static __global__ void __launch_bounds__(kReadThreads) cache_read_kernel(const _
     __syncthreads();
     const uint32_t ty = threadIdx.x / p.nx, tx = threadIdx.x - ty * p.nx;
     if (ty >= p.ny) return;
-    for (uint32_t c = tx; c < p.per_row; c += p.nx) {
+    for (uint32_t c = blockIdx.y * p.nx + tx; c < p.per_row; c += gridDim.y * p.nx) {
         const uint32_t group = p.per_group.div(c), e = (c - group * p.per_group.d) * V;
         const uint32_t part = p.by_heads.div(group), head = group - part * p.by_heads.d;
         const int8_t* const codes = p.codes + part * p.code_part + head * p.code_head + e;

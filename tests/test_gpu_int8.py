@@ -63,6 +63,29 @@ def test_quantize_rows_of_a_wider_matrix(first, step, dtype):
 
 
 @pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("n,d", [(3, 1), (40, 3), (7, 30), (2000, 31), (5, 250), (3000, 500), (5, 2000), (1200, 3000),
+                                 (2, 5001), (3, 9000), (2, 33001)])
+def test_quantize_rows_beside_nan(n, d, dtype):
+    """Rows that start anywhere in wider ones whose other values are NaN and infinities; nothing written beside them."""
+    from elips_b200 import _capi, int8
+    wide = torch.full((n, d + 11), float("nan"), dtype=dtype, device="cuda")
+    wide[:, ::2] = float("inf")
+    for first in range(0, 9, 2 if d > 1000 else 1):
+        wide[:, first:first + d] = activations(rng(n, d, first), (n, d), dtype)
+        x = wide[:, first:first + d]
+        assert_rows(*int8.quantize_rows(x), x)
+        codes, scales = torch.full((n, d + 40), 99, dtype=torch.int8, device="cuda"), torch.empty(n, device="cuda")
+        pitch = d + 40 if (d + 40) % 8 == 0 else (d + 40) // 8 * 8
+        _capi.check(_capi.LIB.elips_b200_quantize_rows(
+            0, x.data_ptr(), int8._TYPES[dtype], n, d, x.stride(0), codes.data_ptr(), pitch, scales.data_ptr(),
+            torch.cuda.current_stream().cuda_stream), "quantize")
+        got = codes.flatten()[:n * pitch].view(n, pitch)
+        assert_rows(got[:, :d], scales, x)
+        assert (got[:, d:] == 99).all()
+        wide[:, first:first + d] = float("nan")
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
 @pytest.mark.parametrize("d", [40, 64, 513])
 def test_quantize_values_next_to_a_border(d, dtype):
     """Values that are halves of the scale exactly, and their neighbours on both sides: the nearest integer, ties to
