@@ -86,12 +86,11 @@ struct LaunchConfig {
     }
 };
 
-template <class T, int V, int G, int NV>
+template <class T, int V, int G, int NV, bool SHIFT>
 void launch_rows(const QuantParams& p, cudaStream_t stream) {
-    const uint32_t blocks = blocks_for(p.groups, 256 / G);
-    LaunchConfig cfg(dim3(blocks), 256, 0, stream);
-    if (p.slots == nullptr) cfg.launch(quantize_rows_kernel<T, V, G, NV, false>, p);
-    else cfg.launch(quantize_rows_kernel<T, V, G, NV, true>, p);
+    LaunchConfig cfg(dim3(blocks_for(p.groups, 256 / G)), 256, 0, stream);
+    if (p.slots == nullptr) cfg.launch(quantize_rows_kernel<T, V, G, NV, false, SHIFT>, p);
+    else cfg.launch(quantize_rows_kernel<T, V, G, NV, true, SHIFT>, p);
 }
 
 // Few threads with many accesses each: what a thread spends on finding its row
@@ -100,48 +99,21 @@ void launch_rows(const QuantParams& p, cudaStream_t stream) {
 // four accesses a thread, 17.4 held in sixteen), and so do rows too few to
 // fill the SMs, whose time is that of one row (1 x 4096 bf16: 3.1 us with a
 // warp, 1.7 with a block).
-template <class T, int V>
+template <class T, int V, bool SHIFT>
 void launch_rows_of(const QuantParams& p, cudaStream_t stream) {
-    const uint32_t n = (p.d + V - 1) / V;  // accesses per row
+    const uint32_t n = cdiv(p.d + (SHIFT ? V - 1 : 0), V);  // accesses per row
     const bool few = p.groups <= 1024;
     if constexpr (V > 1) {
-        if (n <= 8) return launch_rows<T, V, 4, 2>(p, stream);
-        if (n <= 16) return launch_rows<T, V, 4, 4>(p, stream);
-    } else {
-        if (n > 512 && n <= 1024 && !few) return launch_rows<T, V, 32, 32>(p, stream);
+        if (n <= 8) return launch_rows<T, V, 4, 2, SHIFT>(p, stream);
+        if (n <= 16) return launch_rows<T, V, 4, 4, SHIFT>(p, stream);
     }
-    if (n <= 32) launch_rows<T, V, 8, 4>(p, stream);
-    else if (n > 64 && n <= 512 && few) launch_rows<T, V, 256, 2>(p, stream);
-    else if (n <= 128) launch_rows<T, V, 32, 4>(p, stream);
-    else if (n <= 256) launch_rows<T, V, 32, 8>(p, stream);
-    else if (n <= 512) launch_rows<T, V, 32, 16>(p, stream);
-    else if (n <= 1024) launch_rows<T, V, 256, 4>(p, stream);
-    else launch_rows<T, V, 256, 16>(p, stream);
-}
-
-template <class T, int G, int NV>
-void launch_shifted(const QuantParams& p, cudaStream_t stream) {
-    LaunchConfig cfg(dim3(blocks_for(p.groups, 256 / G)), 256, 0, stream);
-    cfg.launch(quantize_shifted_rows_kernel<T, 16 / static_cast<int>(sizeof(T)), G, NV>, p);
-}
-
-// Rows that start anywhere, by the accesses that one of them may span. False
-// where there are more than a block holds.
-template <class T>
-bool launch_shifted_of(const QuantParams& p, cudaStream_t stream) {
-    constexpr uint32_t V = 16 / sizeof(T);
-    const uint32_t n = (p.d + 2 * V - 2) / V;
-    const bool few = p.groups <= 1024;
-    if (n > 4096) return false;
-    if (n <= 16) launch_shifted<T, 4, 4>(p, stream);
-    else if (n <= 32) launch_shifted<T, 8, 4>(p, stream);
-    else if (n > 64 && n <= 512 && few) launch_shifted<T, 256, 2>(p, stream);
-    else if (n <= 128) launch_shifted<T, 32, 4>(p, stream);
-    else if (n <= 256) launch_shifted<T, 32, 8>(p, stream);
-    else if (n <= 512) launch_shifted<T, 32, 16>(p, stream);
-    else if (n <= 1024) launch_shifted<T, 256, 4>(p, stream);
-    else launch_shifted<T, 256, 16>(p, stream);
-    return true;
+    if (n <= 32) launch_rows<T, V, 8, 4, SHIFT>(p, stream);
+    else if (n > 64 && n <= 512 && few) launch_rows<T, V, 256, 2, SHIFT>(p, stream);
+    else if (n <= 128) launch_rows<T, V, 32, 4, SHIFT>(p, stream);
+    else if (n <= 256) launch_rows<T, V, 32, 8, SHIFT>(p, stream);
+    else if (n <= 512) launch_rows<T, V, 32, 16, SHIFT>(p, stream);
+    else if (n <= 1024) launch_rows<T, V, 256, 4, SHIFT>(p, stream);
+    else launch_rows<T, V, 256, 16, SHIFT>(p, stream);
 }
 
 // fn(first row, groups) for runs of rows whose (part, head) groups are fewer
@@ -152,31 +124,26 @@ void in_runs(size_t t, uint32_t per_t, Fn&& fn) {
     for (size_t t0 = 0; t0 < t; t0 += step) fn(static_cast<uint32_t>(t0), static_cast<uint32_t>(std::min(step, t - t0) * per_t));
 }
 
-// Rows are read 16 bytes at a time where every row starts on 16 bytes, holds a
-// whole number of them, and its codes can be stored as many at a time.
-template <class T>
-bool whole_accesses(const QuantParams& p, uint32_t parts) {
-    constexpr uint32_t V = 16 / sizeof(T);
-    uint64_t bits = p.d % V;
-    for (uint32_t i = 0; i < parts; ++i) {
-        bits |= reinterpret_cast<uintptr_t>(p.x[i]) % 16;
-        bits |= (static_cast<uint64_t>(p.x_stride_t[i]) | static_cast<uint64_t>(p.x_stride_h[i])) % V;
-    }
-    bits |= (reinterpret_cast<uintptr_t>(p.codes) | static_cast<uint64_t>(p.code_part | p.code_page | p.code_row | p.code_head)) % V;
-    return bits == 0;
-}
-
 void launch_quantize(int type, QuantParams p, uint32_t parts, cudaStream_t stream) {
     with_float_type(type, [&](auto tag) {
         using T = decltype(tag);
-        const bool whole = whole_accesses<T>(p, parts);
         constexpr uint32_t V = 16 / sizeof(T);
-        const bool shifted = p.slots == nullptr && reinterpret_cast<uintptr_t>(p.codes) % V == 0 && p.code_page % V == 0;
+        // Rows are read 16 bytes at a time where their codes can be stored as
+        // many at a time; as they are where each starts on 16 bytes and holds a
+        // whole number of them, else shifted (where a block holds a row).
+        uint64_t rows = p.d % V, codes = reinterpret_cast<uintptr_t>(p.codes);
+        for (uint32_t i = 0; i < parts; ++i) {
+            rows |= reinterpret_cast<uintptr_t>(p.x[i]) % 16;
+            rows |= (static_cast<uint64_t>(p.x_stride_t[i]) | static_cast<uint64_t>(p.x_stride_h[i])) % V;
+        }
+        codes |= static_cast<uint64_t>(p.code_part | p.code_page | p.code_row | p.code_head);
+        const bool wide = codes % V == 0, held = p.d + V - 1 <= 256u * 16u * V;
         in_runs(p.t, p.per_t.d, [&](uint32_t t0, uint32_t groups) {
             p.t0 = t0;
             p.groups = groups;
-            if (whole) launch_rows_of<T, 16 / sizeof(T)>(p, stream);
-            else if (!shifted || !launch_shifted_of<T>(p, stream)) launch_rows_of<T, 1>(p, stream);
+            if (wide && rows == 0) launch_rows_of<T, V, false>(p, stream);
+            else if (wide && held) launch_rows_of<T, V, true>(p, stream);
+            else launch_rows_of<T, 1, false>(p, stream);
         });
     });
     launch_ok("row quantisation launch");
@@ -319,6 +286,35 @@ void launch_read(ReadParams p, const elips_b200_cache& c, int num_sms, cudaStrea
     cfg.launch(cache_read_kernel<T, V>, p);
 }
 
+// Whether the outputs are runs of values that start on 16 bytes, of rows no
+// narrower than a store, and rows of codes start on as many bytes.
+template <class T>
+bool without_gaps(const ReadParams& p, const elips_b200_cache& c) {
+    constexpr uint64_t V = 16 / sizeof(T);
+    uint64_t codes = reinterpret_cast<uintptr_t>(c.codes);
+    for (int i = 0; i < 4; ++i) codes |= static_cast<uint64_t>(c.code_strides[i]);
+    if (codes % V != 0 || c.dim < static_cast<int64_t>(V) || c.heads * c.dim > (1 << 20)) return false;
+    for (int64_t i = 0; i < c.parts; ++i) {
+        if (reinterpret_cast<uintptr_t>(p.out[i]) % 16 != 0) return false;
+        if (p.total > 1 && p.out_stride_t[i] != c.heads * c.dim) return false;
+        if (c.heads > 1 && p.out_stride_h[i] != c.dim) return false;
+    }
+    return true;
+}
+
+template <class T>
+void launch_read_flat(ReadParams p, const elips_b200_cache& c, int num_sms, cudaStream_t stream) {
+    p.per_group = FastDiv(static_cast<uint32_t>(c.dim));
+    // Rows in multiples of eight, so that every block starts on 16 bytes: two
+    // stores a thread, four blocks an SM.
+    const uint64_t row = static_cast<uint64_t>(c.heads * c.dim);
+    uint64_t rows = std::max<uint64_t>(1, 512 * (16 / sizeof(T)) / row);
+    rows = std::min<uint64_t>(rows, cdiv(static_cast<uint64_t>(p.total) * static_cast<uint64_t>(c.parts), 4u * static_cast<uint32_t>(num_sms)));
+    p.rows = static_cast<uint32_t>(std::min<uint64_t>(kReadRows, (rows + 7) / 8 * 8));
+    LaunchConfig cfg(dim3(blocks_for(p.total, p.rows), static_cast<uint32_t>(c.parts)), 256, 0, stream);
+    cfg.launch(cache_read_flat_kernel<T>, p);
+}
+
 void cache_read(int num_sms, const elips_b200_cache& given, const elips_b200_sequences& q, const elips_b200_rows* out,
                 int type, int zero_behind, cudaStream_t stream) {
     const elips_b200_cache c = plain_strides(given);
@@ -345,6 +341,7 @@ void cache_read(int num_sms, const elips_b200_cache& given, const elips_b200_seq
     with_float_type(type, [&](auto tag) {
         using T = decltype(tag);
         const uint32_t v = read_width<T>(p, c);
+        if (v <= 2 && v < 16 / sizeof(T) && without_gaps<T>(p, c)) return launch_read_flat<T>(p, c, num_sms, stream);
         if constexpr (sizeof(T) == 2) {
             if (v == 8) return launch_read<T, 8>(p, c, num_sms, stream);
         }

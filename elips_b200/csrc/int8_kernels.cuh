@@ -300,9 +300,20 @@ static __global__ void __launch_bounds__(256) cache_claim_kernel(const __grid_co
 // 13.6 us (6.2 TB/s), 10,000 x 768 fp32 7.6 us (5.0 TB/s, the launch a fourth
 // of it); with a check for halves in every 16-bit value and a block per wide
 // row the first took 13.2.
-template <class T, int V, int G, int NV, bool CACHE>
+//
+// SHIFT: rows that start anywhere. The 16-byte accesses are those that hold the
+// row (what they hold beside it is set to zero; an access with one byte of the
+// row is in memory wherever that byte is), and the codes, which start `off`
+// values into the first access, are shifted into place through shared memory,
+// so that they are stored V at a time too. Codes start on V bytes. 10,000 x 767
+// bf16: 7.7 us, value by value 11.3 (10,000 x 768: 4.9); 60,000 x 67: 5.9 and
+// 11.1.
+template <class T, int V, int G, int NV, bool CACHE, bool SHIFT>
 static __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_constant__ QuantParams p) {
+    static_assert(!SHIFT || V > 1, "single values need no shift");
+    using Word = typename std::conditional<V == 8, uint64_t, uint32_t>::type;  // V codes
     __shared__ uint32_t block_max[8];
+    __shared__ Word words[SHIFT ? 256 * NV + 1 : 1];
     constexpr uint32_t kHeld = G * NV * V;
     if (!CACHE || p.dup != kDupClaim) await_previous();
     const uint32_t gl = threadIdx.x % G;
@@ -332,12 +343,20 @@ static __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_
         scale += t;
     }
 
+    const uint32_t off = SHIFT ? static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x) % 16u / sizeof(T)) : 0u;
     Access<T, V> v[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const uint32_t e = (j * G + gl) * V;
-        if (e < p.d && keep) v[j].load(x + e);
+        const uint32_t e = (j * G + gl) * V;  // from `off` values before the row
+        if (e < off + p.d && keep) v[j].load(x - off + e);
         else v[j].zero();
+    }
+    if constexpr (SHIFT) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int e = (j * G + gl) * V, first = static_cast<int>(off) - e, end = static_cast<int>(off + p.d) - e;
+            if (first > 0 || end < V) v[j].keep_only(first, end);
+        }
     }
     if constexpr (CACHE) {
         if (p.dup == kDupClaim) {
@@ -352,7 +371,7 @@ static __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_
     uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < NV; ++j) top = v[j].top(top);
-    if constexpr (G == 256) {
+    if constexpr (G == 256 && !SHIFT) {
         for (uint32_t e = kHeld + gl * V; e < p.d && keep; e += G * V) {
             Access<T, V> u;
             u.load(x + e);
@@ -390,7 +409,36 @@ static __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_
         else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(out + e) = w[0];
         else out[e] = static_cast<int8_t>(w[0]);
     };
-    if constexpr (V > 1) {
+    if constexpr (SHIFT) {
+        Word* const mine = words + threadIdx.x / G * (G * NV);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            uint32_t w[V / 4] = {};
+            if (rs.inv != 0.0f) {
+                float f[V];
+                v[j].values(f);
+                row_codes<V>(f, rs, w);
+            }
+            if constexpr (V == 8) mine[j * G + gl] = static_cast<uint64_t>(w[V / 4 - 1]) << 32 | w[0];
+            else mine[j * G + gl] = w[0];
+        }
+        if constexpr (G == 256) __syncthreads();
+        else __syncwarp();
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const uint32_t i = j * G + gl, e = i * V;
+            if (e >= p.d) continue;
+            // The next word is not needed where off is 0, and where it is past
+            // the row's accesses no code of the row is taken from it.
+            Word w = mine[i] >> (8u * off);
+            if (off != 0u) w |= mine[i + 1] << (8u * (V - off));
+            if (e + V <= p.d) {
+                *reinterpret_cast<Word*>(out + e) = w;
+            } else {
+                for (uint32_t b = 0; e + b < p.d; ++b) out[e + b] = static_cast<int8_t>(w >> (8u * b));
+            }
+        }
+    } else if constexpr (V > 1) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const uint32_t e = (j * G + gl) * V;
@@ -408,7 +456,7 @@ static __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_
             if (e < p.d) out[e] = static_cast<int8_t>(w[j / 4] >> (8 * (j % 4)));
         }
     }
-    if constexpr (G == 256) {
+    if constexpr (G == 256 && !SHIFT) {
         for (uint32_t e = kHeld + gl * V; e < p.d; e += G * V) {
             Access<T, V> u;
             u.load(x + e);
@@ -416,88 +464,6 @@ static __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_
         }
     }
     if (gl == 0) *scale = rs.s;
-}
-
-// quantize_rows_kernel without a cache for rows that start anywhere: the 16-byte
-// accesses are those that hold the row (what they hold beside it is set to
-// zero; an access with one byte of the row is in memory wherever that byte
-// is), and the codes, which start `off` values into the first access, are
-// shifted into place through shared memory, so that they are stored V at a time
-// too. Codes start on V bytes. 10,000 x 767 bf16: 7.7 us, value by value 11.3
-// (10,000 x 768: 4.9); 60,000 x 67: 5.9 and 11.1.
-template <class T, int V, int G, int NV>
-static __global__ void __launch_bounds__(256) quantize_shifted_rows_kernel(const __grid_constant__ QuantParams p) {
-    using Word = typename std::conditional<V == 8, uint64_t, uint32_t>::type;  // V codes
-    __shared__ uint32_t block_max[8];
-    __shared__ Word words[256 * NV + 1];
-    await_previous();
-    let_next_start();
-    const uint32_t gl = threadIdx.x % G;
-    const uint32_t g = blockIdx.x * (256 / G) + threadIdx.x / G;
-    const bool there = g < p.groups;
-    const uint32_t t = p.t0 + g;
-    const T* const row = static_cast<const T*>(p.x[0]) + t * p.x_stride_t[0];
-    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) % 16u / sizeof(T));
-    const T* const x = row - off;
-    Word* const mine = words + threadIdx.x / G * (G * NV);
-
-    Access<T, V> v[NV];
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const uint32_t a = (j * G + gl) * V;  // its first element, counted from x
-        if (there && a < off + p.d) v[j].load(x + a);
-        else v[j].zero();
-    }
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int a = (j * G + gl) * V, first = static_cast<int>(off) - a, end = static_cast<int>(off + p.d) - a;
-        if (first > 0 || end < V) v[j].keep_only(first, end);
-        top = v[j].top(top);
-    }
-    uint32_t amax = Access<T, V>::bits32(top);
-    if constexpr (G == 256) {
-        amax = __reduce_max_sync(0xFFFFFFFFu, amax);
-        if ((threadIdx.x & 31u) == 0) block_max[threadIdx.x >> 5] = amax;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) amax = max(amax, block_max[i]);
-    } else {
-#pragma unroll
-        for (int o = G / 2; o > 0; o /= 2) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-    }
-    const RowScale rs = make_scale<T>(amax);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        uint32_t w[V / 4] = {};
-        if (rs.inv != 0.0f) {
-            float f[V];
-            v[j].values(f);
-            row_codes<V>(f, rs, w);
-        }
-        if constexpr (V == 8) mine[j * G + gl] = static_cast<uint64_t>(w[V / 4 - 1]) << 32 | w[0];
-        else mine[j * G + gl] = w[0];
-    }
-    if constexpr (G == 256) __syncthreads();
-    else __syncwarp();
-    if (!there) return;
-    int8_t* const out = p.codes + t * p.code_page;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const uint32_t i = j * G + gl, e = i * V;
-        if (e >= p.d) continue;
-        // Where off is 0 the next word is not needed, and for a row's last word
-        // it holds nothing of the row: words[256 * NV] and the next row's are
-        // read for nothing.
-        Word w = mine[i] >> (8u * off);
-        if (off != 0u) w |= mine[i + 1] << (8u * (V - off));
-        if (e + V <= p.d) {
-            *reinterpret_cast<Word*>(out + e) = w;
-        } else {
-            for (uint32_t b = 0; e + b < p.d; ++b) out[e + b] = static_cast<int8_t>(w >> (8u * b));
-        }
-    }
-    if (gl == 0) p.scales[t] = rs.s;
 }
 
 // Reading pages back into packed rows. Sequence b owns the output rows
@@ -644,6 +610,75 @@ static __global__ void __launch_bounds__(kReadThreads) cache_read_kernel(const _
                 }
                 out += p.ny * step;
             }
+        }
+    }
+}
+
+// cache_read_kernel for widths that no wide store divides, into outputs without
+// gaps: the output rows of a block are one run of values, cut into 16-byte
+// stores whatever rows they hold. A store's V values come from one row of codes
+// or the ends of two (d >= V), whose words of V codes (rows of codes start on
+// one) are shifted together. 24 sequences of up to 2,964 rows of 2 x 189 fp32:
+// 23.3 us, value by value 31.8.
+template <class T>
+static __global__ void __launch_bounds__(256) cache_read_flat_kernel(const __grid_constant__ ReadParams p) {
+    constexpr uint32_t V = 16 / sizeof(T);
+    using Word = typename std::conditional<V == 8, unsigned long long, uint32_t>::type;
+    __shared__ longlong2 row_at[kReadRows];
+    await_previous();
+    let_next_start();
+    const uint32_t t0 = blockIdx.x * p.rows, rows = min(p.rows, p.total - t0), part = blockIdx.y;
+    if (threadIdx.x < rows) {
+        const int64_t s = read_slot(p, t0 + threadIdx.x);
+        longlong2 at = make_longlong2(s == kRowBehind && p.zero_behind ? kRowNoPage : s, 0);
+        if (s >= 0) {
+            const uint32_t pg = p.page.div(static_cast<uint32_t>(s)), i = static_cast<uint32_t>(s) - pg * p.page.d;
+            at.x = pg * p.code_page + i * p.code_row;
+            at.y = pg * p.scale_page + i * p.scale_row;
+        }
+        row_at[threadIdx.x] = at;
+    }
+    __syncthreads();
+    const int8_t* const codes = p.codes + part * p.code_part;
+    const float* const scales = p.scales + part * p.scale_part;
+    const uint32_t heads = p.by_heads.d, d = p.per_group.d, run = rows * heads * d;
+    T* const out = static_cast<T*>(part != 0u ? p.out[1] : p.out[0]) + static_cast<int64_t>(t0) * heads * d;
+    for (uint32_t f = threadIdx.x * V; f < run; f += 256u * V) {
+        // (row, head, place) of the first value, and the (row, head) after it
+        const uint32_t g0 = p.per_group.div(f), e = f - g0 * d, left = d - e, g1 = g0 + 1u;
+        const uint32_t r0 = p.by_heads.div(g0), h0 = g0 - r0 * heads;
+        const uint32_t r1 = min(p.by_heads.div(g1), rows - 1u), h1 = g1 - p.by_heads.div(g1) * heads;
+        const longlong2 at0 = row_at[r0], at1 = row_at[r1];
+        // The first row's codes from the one or two words that hold them, what
+        // is missing from the second row's first word.
+        Word w = 0, next = 0;
+        float s0 = 0.0f, s1 = 0.0f;
+        if (at0.x >= 0) {
+            const int8_t* const q = codes + at0.x + h0 * p.code_head + e;
+            const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(q) % V);
+            const Word* const from = reinterpret_cast<const Word*>(q - off);
+            w = __ldg(from) >> (8u * off);
+            if (off + min(V, left) > V) w |= __ldg(from + 1) << (8u * (V - off));
+            s0 = __ldg(scales + at0.y + h0 * p.scale_head);
+        }
+        if (left < V) {
+            if (at1.x >= 0) {
+                next = __ldg(reinterpret_cast<const Word*>(codes + at1.x + h1 * p.code_head));
+                s1 = __ldg(scales + at1.y + h1 * p.scale_head);
+            }
+            w = (w & ((Word{1} << (8u * left)) - 1u)) | next << (8u * left);
+        }
+        const uint32_t q[2] = {static_cast<uint32_t>(w), static_cast<uint32_t>(static_cast<uint64_t>(w) >> 32)};
+        alignas(16) T v[V];
+#pragma unroll
+        for (uint32_t j = 0; j < V; ++j)
+            v[j] = from_f32<T>(code_f32(q[j / 4] ^ 0x80808080u, j % 4) * (j >= left ? s1 : s0));
+        if (f + V <= run && at0.x != kRowBehind && at1.x != kRowBehind) {
+            *reinterpret_cast<uint4*>(out + f) = *reinterpret_cast<const uint4*>(v);
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < V; ++j)
+                if (f + j < run && (j >= left ? at1.x : at0.x) != kRowBehind) out[f + j] = v[j];
         }
     }
 }

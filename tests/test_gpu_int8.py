@@ -490,6 +490,31 @@ def test_cache_read_sequences(parts, heads, dim, page, dtype):
     assert_read(res, codes, scales, table, offsets, total, behind=5.0)
 
 
+@pytest.mark.parametrize("parts,heads,dim", [(2, 3, 67), (1, 1, 251), (2, 1, 9), (1, 8, 129), (1, 2, 8), (1, 5, 3), (2, 1, 2049)])
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("total", [1, 7, 8, 9, 500])
+def test_cache_read_runs_of_odd_rows(parts, heads, dim, dtype, total):
+    """Widths that no store divides, packed: stores that span rows, heads, sequences, bad pages and the rows behind,
+    which stay as they are."""
+    from elips_b200 import int8
+    g = rng(parts, heads, dim, total)
+    codes, scales = filled(g, parts, 9, 4, heads, dim)
+    kept = total - total // 5
+    cut = np.sort(g.integers(0, kept + 1, 5))
+    offsets = np.concatenate([[0], cut, [kept]])
+    table = g.integers(-1, 10, (6, kept // 4 + 1))
+    td, od = torch.from_numpy(table).cuda().int(), torch.from_numpy(offsets).cuda()
+    assert_read(int8.cache_read(codes, scales, td, od, total, dtype), codes, scales, table, offsets, total)
+    out = tuple(torch.full((total, heads, dim), 5.0, dtype=dtype, device="cuda") for _ in range(parts))
+    assert_read(int8.cache_read(codes, scales, td, od, total, out=out), codes, scales, table, offsets, total, behind=5.0)
+    # one value off 16 bytes, and codes without padding
+    held = codes.contiguous()
+    out = tuple(torch.full((total * heads * dim + 1,), 5.0, dtype=dtype, device="cuda")[1:].view(total, heads, dim)
+                for _ in range(parts))
+    assert_read(int8.cache_read(held, scales, td, od, total, out=out), held, scales, table, offsets, total, behind=5.0)
+    assert_read(int8.cache_read(held, scales, td, od, total, dtype), held, scales, table, offsets, total)
+
+
 @pytest.mark.parametrize("heads,dim", [(1, 96), (3, 20)])
 def test_cache_read_bad_pages_are_zeros(heads, dim):
     """Table entries that are no page, sequences longer than the table is wide."""
