@@ -256,7 +256,8 @@ __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.
 
 // A slot given twice in one call keeps the last of its rows. Up to
 // kDupScanRows rows each row looks for its slot among the later ones (which
-// stay in L1). Longer calls settle it before any row is written: a launch of
+// stay in L1; 256 rows of 2 x 8 x 128 take 3.7 us, 300 with claims 3.2 but one
+// launch more). Longer calls settle it before any row is written: a launch of
 // its own leaves the largest claim 0x80000001 + t in the slot's scale words,
 // and the row whose claim stands writes codes and scale. A scale is never
 // negative, so neither one that is written in between nor one that was there
@@ -287,6 +288,37 @@ static __global__ void __launch_bounds__(256) cache_claim_kernel(const __grid_co
         if (atomicCAS(w, old, claim) == old) return;
         old = atomicMax(w, claim);  // another row's claim came first
     }
+}
+
+// Whether a row after t has the same slot, by the G threads of the row (each
+// sees its own share) or, where they are few, by the whole warp for one after
+// the other of its rows, those of one t (its heads and parts) at once. The
+// loops have no early end, so that their loads do not wait for each other.
+template <int G>
+__device__ __forceinline__ bool again_later(const QuantParams& p, uint32_t t, uint32_t slot, bool wanted, uint32_t gl) {
+    bool again = false;
+    if constexpr (G >= 32) {
+#pragma unroll 4
+        for (uint32_t i = t + 1u + gl; i < p.t; i += G) again |= slot_of(p, i) == static_cast<int64_t>(slot);
+    } else {
+        const uint32_t lane = threadIdx.x & 31u;
+        uint32_t last_t = 0xFFFFFFFFu;
+        bool last = false;
+#pragma unroll 1
+        for (uint32_t r = 0; r < 32u / G; ++r) {
+            if (!__shfl_sync(0xFFFFFFFFu, wanted ? 1 : 0, r * G)) continue;
+            const uint32_t t_r = __shfl_sync(0xFFFFFFFFu, t, r * G), slot_r = __shfl_sync(0xFFFFFFFFu, slot, r * G);
+            if (t_r != last_t) {
+                bool found = false;
+#pragma unroll 4
+                for (uint32_t i = t_r + 1u + lane; i < p.t; i += 32) found |= slot_of(p, i) == static_cast<int64_t>(slot_r);
+                last = __any_sync(0xFFFFFFFFu, found);
+                last_t = t_r;
+            }
+            if (lane / G == r) again = last;
+        }
+    }
+    return again;
 }
 
 // G threads per row (4, 8, a warp, or the whole block), each holding NV
@@ -363,8 +395,10 @@ static __global__ void __launch_bounds__(256) quantize_rows_kernel(const __grid_
             // The row's own claim stands until it stores its scale below.
             await_previous();
             if (keep) keep = *reinterpret_cast<volatile uint32_t*>(scale) == claim_of(t);
-        } else if (p.dup == kDupScan && keep) {
-            for (uint32_t i = t + 1u + gl; i < p.t; i += G) keep = keep && slot_of(p, i) != static_cast<int64_t>(slot);
+        } else if (p.dup == kDupScan) {
+            // Every lane takes part, whatever its row: the search votes.
+            const bool again = again_later<G>(p, t, slot, keep, gl);
+            keep = keep && !again;
         }
     }
     let_next_start();
