@@ -297,10 +297,10 @@ static __global__ void __launch_bounds__(256) cache_claim_kernel(const __grid_co
 template <int G>
 __device__ __forceinline__ bool again_later(const QuantParams& p, uint32_t t, uint32_t slot, bool wanted, uint32_t gl) {
     bool again = false;
-    if constexpr (G >= 32) {
+    if (G >= 32 || p.t <= 4 * G) {
 #pragma unroll 4
         for (uint32_t i = t + 1u + gl; i < p.t; i += G) again |= slot_of(p, i) == static_cast<int64_t>(slot);
-    } else {
+    } else if constexpr (G < 32) {
         const uint32_t lane = threadIdx.x & 31u;
         uint32_t last_t = 0xFFFFFFFFu;
         bool last = false;
