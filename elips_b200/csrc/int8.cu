@@ -235,8 +235,7 @@ void cache_write(const elips_b200_cache& given, const elips_b200_rows* rows, int
         in_runs(t, p.per_t.d, [&](uint32_t t0, uint32_t groups) {
             p.t0 = t0;
             p.groups = groups;
-            const uint32_t blocks = blocks_for(groups, 256);
-            LaunchConfig cfg(dim3(blocks), 256, 0, stream);
+            LaunchConfig cfg(dim3(blocks_for(groups, 256)), 256, 0, stream);
             cfg.launch(cache_claim_kernel, p);
         });
         launch_ok("cache claim launch");
@@ -376,8 +375,7 @@ void launch_dot_rows(const GemmParams& p, int num_sms, cudaStream_t stream) {
     // launch (1 x 4096 x 4096 after another, weights in L2: 4.4 us, early 5.3).
     constexpr bool codes = std::is_same<X, int8_t>::value;
     const size_t smem = codes ? 0 : static_cast<size_t>(p.m) * ((p.k + 15u) / 16u * 16u);
-    const uint32_t blocks = blocks_for(groups * wk, 8);
-    LaunchConfig cfg(dim3(blocks), 256, smem, stream, codes);
+    LaunchConfig cfg(dim3(blocks_for(groups * wk, 8)), 256, smem, stream, codes);
     cfg.launch(gemm_int8_dot_kernel<MR, X, T>, p, wk);
     launch_ok("int8 product launch");
 }
@@ -583,7 +581,8 @@ void linear_int8(int num_sms, const elips_b200_gemm& g, cudaStream_t stream) {
     GemmParams p = gemm_params(g);
     const size_t pitch = (static_cast<size_t>(p.k) + 15) / 16 * 16;
     // Few values: the dot kernel quantises them itself.
-    if (gemm_form(p.m, p.n, p.k, g.out_type == ELIPS_B200_PRECISION_FP32, num_sms).rows == 1 && p.m * pitch <= kDotCodeBytes && on_16(p.b, p.b_pitch, p.n)) {
+    if (gemm_form(p.m, p.n, p.k, g.out_type == ELIPS_B200_PRECISION_FP32, num_sms).rows == 1 &&
+        p.m * pitch <= kDotCodeBytes && on_16(p.b, p.b_pitch, p.n)) {
         p.x = g.a;
         p.x_pitch = p.m > 1 ? g.a_stride : 0;
         Profiler::Scope prof("linear_int8", stream, static_cast<uint64_t>(p.m) * p.n);
