@@ -540,6 +540,46 @@ void gemm_int8(int num_sms, GemmParams p, int out_type, cudaStream_t stream) {
     product();
 }
 
+// Rows of `width` bytes, `pitch` bytes apart.
+struct Region {
+    uintptr_t base;
+    int64_t rows, width, pitch;
+    uintptr_t low() const { return pitch < 0 ? base + static_cast<uintptr_t>((rows - 1) * pitch) : base; }
+    uintptr_t high() const { return (pitch < 0 ? base : base + static_cast<uintptr_t>((rows - 1) * pitch)) + width; }
+};
+
+Region region(const void* p, int64_t rows, int64_t width, int64_t pitch) {
+    return {reinterpret_cast<uintptr_t>(p), rows, width, rows > 1 ? pitch : 0};
+}
+
+// Whether two regions share a byte. Columns side by side in one buffer do not;
+// rows of two different pitches that reach into one another are taken to.
+bool overlap(const Region& a, const Region& b) {
+    if (a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+    if (a.high() <= b.low() || b.high() <= a.low()) return false;
+    if (a.rows > 1 && b.rows > 1 && a.pitch != b.pitch) return true;
+    const int64_t pitch = a.rows > 1 ? a.pitch : b.pitch;
+    if (pitch <= 0) return true;
+    const int64_t ahead = (static_cast<int64_t>(b.base - a.base) % pitch + pitch) % pitch;
+    return ahead < a.width || ahead + b.width > pitch;
+}
+
+int64_t type_bytes(int type) {
+    return type == ELIPS_B200_PRECISION_INT8 ? 1 : type == ELIPS_B200_PRECISION_FP32 ? 4 : 2;
+}
+
+// The forms differ in what they have read when they first write (the dot
+// kernel's blocks each read every row), so no output may lie on an input.
+void check_gemm_apart(const elips_b200_gemm& g) {
+    const int64_t a = type_bytes(g.a_type), o = type_bytes(g.out_type);
+    const Region out = region(g.out, g.m, g.n * o, g.out_stride * o);
+    if (overlap(out, region(g.a, g.m, g.k * a, g.a_stride * a)) ||
+        overlap(out, region(g.b, g.n, g.k, g.b_stride)) || overlap(out, region(g.b_scales, 1, g.n * 4, 0)) ||
+        (g.a_type == ELIPS_B200_PRECISION_INT8 && overlap(out, region(g.a_scales, 1, g.m * 4, 0))) ||
+        (g.bias != nullptr && overlap(out, region(g.bias, 1, g.n * type_bytes(g.bias_type), 0))))
+        bad("the output shares memory with an input");
+}
+
 void check_gemm(const elips_b200_gemm& g) {
     check_float_type(g.out_type);
     if (g.bias != nullptr) check_float_type(g.bias_type);
@@ -553,6 +593,7 @@ void check_gemm(const elips_b200_gemm& g) {
     if (g.m == 0 || g.n == 0) return;
     if (g.b_scales == nullptr || g.out == nullptr || (codes && g.a_scales == nullptr)) bad("operand missing");
     if (g.k > 0 && (g.a == nullptr || g.b == nullptr)) bad("operand missing");
+    check_gemm_apart(g);
 }
 
 GemmParams gemm_params(const elips_b200_gemm& g) {
@@ -632,6 +673,12 @@ int elips_b200_quantize_rows(int device, const void* x, int type, size_t n, size
     return guarded([&] {
         eb::check_rows(n, d, type);
         if (code_stride < d) eb::bad("codes of neighbouring rows overlap");
+        const int64_t rows = static_cast<int64_t>(n), width = static_cast<int64_t>(d), bytes = eb::type_bytes(type);
+        const eb::Region in = eb::region(x, rows, width * bytes, x_stride * bytes);
+        const eb::Region out = eb::region(codes, rows, width, static_cast<int64_t>(code_stride));
+        const eb::Region held = eb::region(scales, 1, rows * 4, 0);
+        if (eb::overlap(in, out) || eb::overlap(in, held) || eb::overlap(out, held))
+            eb::bad("rows, codes and scales share memory");
         eb::DeviceGuard g(device);
         eb::device_props(device);
         eb::quantize_rows(x, type, n, d, x_stride, codes, code_stride, scales, eb::as_stream(stream));
@@ -674,6 +721,7 @@ int elips_b200_cache_read(int device, const elips_b200_cache* cache, const elips
     return guarded([&] {
         eb::check_cache(*cache);
         eb::check_cache_rows(*cache, out, type, static_cast<size_t>(q.total));
+        if (q.total > 0 && cache->parts == 2 && out[0].data == out[1].data) eb::bad("the parts share one output");
         if (q.sequences > static_cast<int64_t>(eb::kMaxRows) || q.table_width > static_cast<int64_t>(eb::kMaxRows))
             eb::bad("page table too large");
         if (q.total > 0 && q.sequences > 0 && q.offsets == nullptr) eb::bad("offsets missing");

@@ -191,7 +191,8 @@ def gemm_int8(a, b, a_scales, b_scales, bias=None, out_dtype=torch.bfloat16, out
     them: a activations and b a layer's weight with a scale per channel, or a
     queries and b stored rows. Operands whose rows start on multiples of 16
     bytes are read as they are, others are copied to such rows first. bias
-    [n] may have another float type than out."""
+    [n] may have another float type than out. An out that shares memory with an
+    input is refused (columns side by side in one buffer share none)."""
     if a.dtype is not torch.int8:
         raise ValueError(f"row codes must be int8, not {a.dtype}")
     return _product(a, capi.PRECISION_INT8, a_scales, b, b_scales, bias, out_dtype, out, stream)
@@ -199,7 +200,8 @@ def gemm_int8(a, b, a_scales, b_scales, bias=None, out_dtype=torch.bfloat16, out
 
 def linear_int8(x, weight, weight_scales, bias=None, out_dtype=None, out=None, stream=None):
     """gemm_int8 over the rows of x [m, k], quantised on the way as
-    quantize_rows quantises them; out_dtype defaults to x's type."""
+    quantize_rows quantises them; out_dtype defaults to x's type. x cannot be
+    its own out."""
     dtype = x.dtype
     kind = _float_type(dtype, "rows")
     if x.numel() == 0 and x.shape[-1:] == (0,):
@@ -307,7 +309,8 @@ def cache_read(codes, scales, page_table, offsets, total: int, dtype=torch.bfloa
     or lies past the table's width, reads as zeros, as do rows in front of
     offsets[0]. `total` is the number of output rows, offsets[-1] or more; rows
     behind the last sequence are zeros, or with `out` (a tuple of tensors like
-    the result, of any strides but the last) stay as they are."""
+    the result, of any strides but the last, that share no memory) stay as they
+    are."""
     cache, parts, heads, dim = _cache(codes, scales, False)
     table_wide, offsets_wide = _indexes(page_table, "page_table"), _indexes(offsets, "offsets")
     shape = page_table.shape

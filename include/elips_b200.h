@@ -588,7 +588,8 @@ ELIPS_B200_API int elips_b200_ivfpq_train(int device, int metric, const float* r
 
 /* codes[i * code_stride + j] and scales[i] of n rows of d values (d in
  * [1, 2^24]) at x + i * x_stride. A code_stride that is a multiple of 16 and
- * codes on 16 bytes let elips_b200_gemm_int8 read them without a copy. */
+ * codes on 16 bytes let elips_b200_gemm_int8 read them without a copy. Rows,
+ * codes and scales that share memory are refused. */
 ELIPS_B200_API int elips_b200_quantize_rows(int device, const void* x, int type, size_t n, size_t d, int64_t x_stride,
                                             int8_t* codes, size_t code_stride, float* scales, void* stream);
 
@@ -597,7 +598,8 @@ ELIPS_B200_API int elips_b200_quantize_rows(int device, const void* x, int type,
  * row-major. a_type is ELIPS_B200_PRECISION_INT8 for codes with a_scales, or a
  * float type for rows that are quantised on the way as
  * elips_b200_quantize_rows does (a_scales is not read then, and k >= 1).
- * bias may be NULL; its type is its own. */
+ * bias may be NULL; its type is its own. An output that shares memory with an
+ * input is refused; columns side by side in one buffer share none. */
 typedef struct {
     const void* a;
     const float* a_scales;
@@ -658,7 +660,8 @@ typedef struct {
 /* Reads sequences back into packed rows, one output per part. A page that is
  * no page of the cache, or past the table's width, reads as zeros, and so do
  * rows in front of offsets[0]. Rows from offsets[sequences] on are zeroed
- * where zero_behind, else left as they are. */
+ * where zero_behind, else left as they are. The outputs must share no memory
+ * with one another or with what is read (one output for two parts is refused). */
 ELIPS_B200_API int elips_b200_cache_read(int device, const elips_b200_cache* cache,
                                          const elips_b200_sequences* sequences, const elips_b200_rows* out, int type,
                                          int zero_behind, void* stream);

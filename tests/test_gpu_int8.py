@@ -807,3 +807,24 @@ def test_errors_leave_no_device_error():
         int8.gemm_int8(a, a, one, one)
     assert e.value.status == _capi.INVALID_ARGUMENT
     assert _capi.device_error(0) == 0
+
+
+@pytest.mark.parametrize("m", [1, 5, 40, 600])
+def test_outputs_beside_and_on_their_inputs(m):
+    """One buffer holds the rows and, in the columns next to them, the output; on the rows themselves it is refused
+    (few rows are quantised by every block of the product, which would find some of them overwritten)."""
+    from elips_b200 import ElipsB200Error, int8 as ops
+    torch.manual_seed(m)
+    n, k = 64, 96
+    buffer = torch.randn((m, k + n), device="cuda", dtype=torch.bfloat16)
+    weight, scales = ops.quantize_rows(torch.randn((n, k), device="cuda"))
+    x = buffer[:, :k]
+    want = ops.linear_int8(x.clone(), weight, scales)
+    before = x.clone()
+    assert torch.equal(ops.linear_int8(x, weight, scales, out=buffer[:, k:]), want)
+    assert torch.equal(x, before)
+    with pytest.raises(ElipsB200Error):
+        ops.linear_int8(x, weight, scales, out=buffer[:, k - 1:-1])
+    with pytest.raises(ElipsB200Error):
+        ops.linear_int8(x, weight, scales, out=x[:, :n])
+    assert torch.equal(x, before)

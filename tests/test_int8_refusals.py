@@ -147,3 +147,41 @@ def test_c_entry_points_refuse_before_the_device():
     assert read(described(), sequences=1 << 40) == bad
     assert lib.elips_b200_cache_read(0, ctypes.byref(described()), None, r, bf16, 1, None) == bad
     assert read(described(), offsets=None) == bad
+
+
+@pytest.mark.parametrize("kind", [_capi.PRECISION_INT8, _capi.PRECISION_BF16])
+def test_products_onto_their_inputs_refused(kind):
+    """An output on any byte of an input, from either side of it. Every address is far from the others' unless named."""
+    size = 1 if kind == _capi.PRECISION_INT8 else 2
+    m, n, k, a, b, a_scales, b_scales, bias, out = 4, 8, 16, 1 << 20, 2 << 20, 3 << 20, 4 << 20, 5 << 20, 6 << 20
+
+    def status(**kw):
+        d = dict(a=a, a_scales=a_scales, b=b, b_scales=b_scales, bias=bias, out=out, m=m, n=n, k=k, a_stride=k,
+                 b_stride=k, out_stride=n, a_type=kind, bias_type=_capi.PRECISION_BF16, out_type=_capi.PRECISION_FP32,
+                 reserved=0) | kw
+        return _capi.LIB.elips_b200_gemm_int8(0, ctypes.byref(_capi.Gemm(*d.values())), None)
+    out_bytes = 4 * m * n
+    inputs = [(a, m * k * size), (b, n * k), (b_scales, 4 * n), (bias, 2 * n)]
+    if kind == _capi.PRECISION_INT8:
+        inputs.append((a_scales, 4 * m))
+    for at, count in inputs:
+        assert status(out=at) == _capi.INVALID_ARGUMENT
+        assert status(out=at + count - 4) == _capi.INVALID_ARGUMENT
+        assert status(out=at - out_bytes + 4) == _capi.INVALID_ARGUMENT
+    # One column of the output lies on the rows' last one, in a buffer of 256 bytes a row.
+    assert status(a_stride=256 // size, out_stride=64, out=a + k * size - 4) == _capi.INVALID_ARGUMENT
+    # The output's last column reaches into the next row's first value.
+    assert status(a_stride=256 // size, out_stride=64, out=a + 256 - 4 * n + 4) == _capi.INVALID_ARGUMENT
+
+
+def test_rows_and_reads_onto_one_another_refused():
+    lib, bad, f32 = _capi.LIB, _capi.INVALID_ARGUMENT, _capi.PRECISION_FP32
+    x, codes_at, scales = 1 << 20, 2 << 20, 3 << 20
+    assert lib.elips_b200_quantize_rows(0, x, f32, 4, 16, 16, x, 16, scales, None) == bad
+    assert lib.elips_b200_quantize_rows(0, x, f32, 4, 16, 16, x + 255, 16, scales, None) == bad
+    assert lib.elips_b200_quantize_rows(0, x, f32, 4, 16, 16, codes_at, 16, x + 16, None) == bad
+    assert lib.elips_b200_quantize_rows(0, x, f32, 4, 16, 16, codes_at, 16, codes_at + 60, None) == bad
+    c = _capi.Cache(x, scales, 2, 3, 4, 2, 8, (192, 64, 16, 8), (24, 8, 2, 1))
+    r = (_capi.Rows * 2)(_capi.Rows(codes_at, 16, 8), _capi.Rows(codes_at, 16, 8))
+    q = _capi.Sequences(4 << 20, 5 << 20, 3, 2, 3, 2, 0, 0)
+    assert lib.elips_b200_cache_read(0, ctypes.byref(c), ctypes.byref(q), r, _capi.PRECISION_BF16, 1, None) == bad
