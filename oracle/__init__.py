@@ -20,6 +20,7 @@ from __future__ import annotations
 import ctypes
 import os
 import subprocess
+import unittest
 from ctypes import POINTER, c_float, c_int, c_int64, c_size_t, c_uint8, c_uint32, c_void_p
 from pathlib import Path
 
@@ -73,6 +74,19 @@ def ref_available() -> bool:
     return REF_SO.exists() or _ref_sources()
 
 
+class ReferenceMissing(OSError, unittest.SkipTest):
+    """Neither the reference's sources nor a library built from them are here. A test that needs them is skipped."""
+
+
+def _ref_lib(so: Path) -> ctypes.CDLL:
+    """A library of the reference's classes, built first where only the sources are there."""
+    if not so.exists():
+        if not _ref_sources():
+            raise ReferenceMissing(f"no reference sources at {REF_ROOT} and no {so.name}")
+        build(ref=True)
+    return _declare(ctypes.CDLL(str(so)))
+
+
 def _declare(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.ref_distance.restype = c_float
     lib.ref_distance.argtypes = [c_int, c_void_p, c_void_p, c_size_t]
@@ -85,9 +99,7 @@ def _declare(lib: ctypes.CDLL) -> ctypes.CDLL:
 def ref() -> ctypes.CDLL:
     global _ref
     if _ref is None:
-        if not REF_SO.exists():
-            build(ref=True)
-        _ref = _declare(ctypes.CDLL(str(REF_SO)))
+        _ref = _ref_lib(REF_SO)
     return _ref
 
 
@@ -95,9 +107,7 @@ def ref_b200() -> ctypes.CDLL:
     """The reference classes on the B200 CudaBackend (needs a GPU to run)."""
     global _ref_b200
     if _ref_b200 is None:
-        if not REF_B200_SO.exists():
-            build(ref=True)
-        _ref_b200 = _declare(ctypes.CDLL(str(REF_B200_SO)))
+        _ref_b200 = _ref_lib(REF_B200_SO)
     return _ref_b200
 
 
