@@ -108,33 +108,33 @@ static __global__ void __launch_bounds__(256) gemm_int8_dot_kernel(const __grid_
     const uint32_t tail = p.k & 15u;
 #pragma unroll 4
     for (uint32_t i = kw * 32u + lane; i < chunks; i += wk * 32u) {
-        int4 w[kDotChannels];
+        uint4 w[kDotChannels];
 #pragma unroll
-        for (int c = 0; c < kDotChannels; ++c) w[c] = __ldg(reinterpret_cast<const int4*>(br[c]) + i);
+        for (int c = 0; c < kDotChannels; ++c) w[c] = ld16(br[c] + i * 16u);
 #pragma unroll
         for (int m = 0; m < MR; ++m) {
-            int4 x;
+            uint4 x;
             const uint32_t mm = min(static_cast<uint32_t>(m), p.m - 1u);
             if constexpr (kFloat) {
-                x = *reinterpret_cast<const int4*>(row_codes_smem + (mm * chunks + i) * 16u);
+                x = *reinterpret_cast<const uint4*>(row_codes_smem + (mm * chunks + i) * 16u);
             } else {
-                x = __ldg(reinterpret_cast<const int4*>(p.a + static_cast<int64_t>(mm) * p.a_pitch) + i);
+                x = ld16(p.a + static_cast<int64_t>(mm) * p.a_pitch + i * 16u);
                 if (tail != 0u && i == chunks - 1u) {
-                    int* xw = reinterpret_cast<int*>(&x);
+                    uint32_t* xw = reinterpret_cast<uint32_t*>(&x);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int keep = static_cast<int>(tail) - 4 * j;
-                        xw[j] = keep >= 4 ? xw[j] : keep <= 0 ? 0 : xw[j] & ((1 << (8 * keep)) - 1);
+                        xw[j] = keep >= 4 ? xw[j] : keep <= 0 ? 0 : xw[j] & ((1u << (8 * keep)) - 1u);
                     }
                 }
             }
 #pragma unroll
             for (int c = 0; c < kDotChannels; ++c) {
                 int32_t s = acc[m][c];
-                s = __dp4a(x.x, w[c].x, s);
-                s = __dp4a(x.y, w[c].y, s);
-                s = __dp4a(x.z, w[c].z, s);
-                acc[m][c] = __dp4a(x.w, w[c].w, s);
+                s = __dp4a(static_cast<int>(x.x), static_cast<int>(w[c].x), s);
+                s = __dp4a(static_cast<int>(x.y), static_cast<int>(w[c].y), s);
+                s = __dp4a(static_cast<int>(x.z), static_cast<int>(w[c].z), s);
+                acc[m][c] = __dp4a(static_cast<int>(x.w), static_cast<int>(w[c].w), s);
             }
         }
     }
@@ -631,15 +631,13 @@ static __global__ void __launch_bounds__(kPairThreads, 1)
         auto fetch = [&](uint32_t i) {
             const PairUnit u = pair_unit(i, whole, n_mt, n_nt);
             const uint32_t m = u.mt * kPairM + rank * (kPairM / 2) + quad * 32u + lane;
-            sa = m < p.m ? __ldg(p.a_scales + m) : 0.0f;
+            sa = ld_float_if(p.a_scales + m, m < p.m);
 #pragma unroll
             for (uint32_t j = 0; j < kOwn; ++j) {
                 const uint32_t n = u.n0 + half * (u.bn / 2) + j * 32u + lane;
-                sb[j] = make_float2(0.0f, 0.0f);
-                if (n < p.n && j * 32u < u.bn / 2) {
-                    sb[j].x = __ldg(p.b_scales + n);
-                    if (p.bias != nullptr) sb[j].y = bias_at(p.bias, p.bias_type, n);
-                }
+                const bool there = n < p.n && j * 32u < u.bn / 2;
+                sb[j] = make_float2(ld_float_if(p.b_scales + n, there), 0.0f);
+                if (there && p.bias != nullptr) sb[j].y = bias_at(p.bias, p.bias_type, n);
             }
         };
         if (pair < units) fetch(pair);
@@ -767,7 +765,7 @@ static __global__ void __launch_bounds__(256) repack_codes_kernel(const __grid_c
             // is read only where it holds one of them.
             const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src)) & 3u;
             const uint32_t* at = reinterpret_cast<const uint32_t*>(src - off);
-            const uint32_t lo = __ldg(at), hi = off != 0u ? __ldg(at + 1) : 0u;
+            const uint32_t lo = ld4_if(at, true), hi = ld4_if(at + 1, off != 0u);
             w = __funnelshift_r(lo, hi, 8u * off);
         } else {
             for (uint32_t j = 0; c + j < p.k; ++j) w |= static_cast<uint32_t>(static_cast<uint8_t>(src[j])) << (8u * j);

@@ -250,9 +250,54 @@ __device__ __forceinline__ void group_at(const QuantParams& p, uint32_t g, uint3
 // and only then lets the next one start (let_next_start), so whatever a kernel
 // finds running has itself seen the end of all before it. The one exception:
 // a cache write after its claims reads rows and slots first, which nothing in
-// between writes.
+// between writes. Because a kernel may start before its inputs are written, none
+// of them is read through the non-coherent path (__ldg), which is for data that
+// stays as it is for as long as the kernel runs.
 __device__ __forceinline__ void await_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Coherent loads that stay behind await_previous (volatile, as that is) and that
+// the compiler may otherwise place as it does __ldg, before stores that they do
+// not depend on among others: as plain loads, which may not pass a store, the
+// batches of cache_read_kernel hold more registers and 131,072 rows of 2 x 8 x
+// 128 bf16 take 156 us in place of 128.
+__device__ __forceinline__ uint4 ld16(const void* at) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at));
+    return v;
+}
+// Zero where not `there`: predicated, so that a batch of them is under way at once.
+__device__ __forceinline__ uint2 ld8_if(const void* at, bool there) {
+    uint2 v;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\t"
+        "@p ld.global.v2.u32 {%0, %1}, [%2];\n\t}"
+        : "=&r"(v.x), "=&r"(v.y)
+        : "l"(at), "r"(there ? 1u : 0u));
+    return v;
+}
+__device__ __forceinline__ uint32_t ld4_if(const void* at, bool there) {
+    uint32_t v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u32 %0, 0;\n\t@p ld.global.u32 %0, [%1];\n\t}"
+                 : "=&r"(v)
+                 : "l"(at), "r"(there ? 1u : 0u));
+    return v;
+}
+__device__ __forceinline__ uint32_t ld2_if(const void* at, bool there) {
+    uint32_t v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u32 %0, 0;\n\t@p ld.global.u16 %0, [%1];\n\t}"
+                 : "=&r"(v)
+                 : "l"(at), "r"(there ? 1u : 0u));
+    return v;
+}
+__device__ __forceinline__ uint32_t ld1_if(const void* at, bool there) {
+    uint32_t v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u32 %0, 0;\n\t@p ld.global.u8 %0, [%1];\n\t}"
+                 : "=&r"(v)
+                 : "l"(at), "r"(there ? 1u : 0u));
+    return v;
+}
+__device__ __forceinline__ float ld_float_if(const float* at, bool there) { return __uint_as_float(ld4_if(at, there)); }
 
 // A slot given twice in one call keeps the last of its rows. Up to
 // kDupScanRows rows each row looks for its slot among the later ones (which
@@ -559,19 +604,15 @@ __device__ __forceinline__ float code_f32(uint32_t turned, uint32_t byte) {
 template <int V>
 __device__ __forceinline__ void load_codes(const int8_t* src, bool there, uint32_t (&w)[(V + 3) / 4]) {
     if constexpr (V == 8) {
-        uint2 u = make_uint2(0, 0);
-        if (there) u = __ldg(reinterpret_cast<const uint2*>(src));
+        const uint2 u = ld8_if(src, there);
         w[0] = u.x;
         w[V / 4 - 1] = u.y;
+    } else if constexpr (V == 4) {
+        w[0] = ld4_if(src, there);
+    } else if constexpr (V == 2) {
+        w[0] = ld2_if(src, there);
     } else {
-        w[0] = 0;
-        if constexpr (V == 4) {
-            if (there) w[0] = __ldg(reinterpret_cast<const uint32_t*>(src));
-        } else if constexpr (V == 2) {
-            if (there) w[0] = __ldg(reinterpret_cast<const uint16_t*>(src));
-        } else {
-            if (there) w[0] = static_cast<uint8_t>(__ldg(src));
-        }
+        w[0] = ld1_if(src, there);
     }
 }
 
@@ -627,10 +668,7 @@ static __global__ void __launch_bounds__(kReadThreads) cache_read_kernel(const _
 #pragma unroll
             for (int b = 0; b < kReadBatch; ++b) load_codes<V>(codes + at[b].x, at[b].x >= 0, w[b]);
 #pragma unroll
-            for (int b = 0; b < kReadBatch; ++b) {
-                sc[b] = 0.0f;
-                if (at[b].x >= 0) sc[b] = __ldg(scales + at[b].y);
-            }
+            for (int b = 0; b < kReadBatch; ++b) sc[b] = ld_float_if(scales + at[b].y, at[b].x >= 0);
 #pragma unroll
             for (int b = 0; b < kReadBatch; ++b) {
                 if (r0 + b * p.ny < rows && at[b].x != kRowBehind) {
@@ -659,6 +697,11 @@ static __global__ void __launch_bounds__(256) cache_read_flat_kernel(const __gri
     constexpr uint32_t V = 16 / sizeof(T);
     using Word = typename std::conditional<V == 8, unsigned long long, uint32_t>::type;
     __shared__ longlong2 row_at[kReadRows];
+    auto ld_word = [](const Word* at) -> Word {
+        if constexpr (V == 4) return ld4_if(at, true);
+        const uint2 u = ld8_if(at, true);
+        return static_cast<Word>(static_cast<uint64_t>(u.y) << 32 | u.x);
+    };
     await_previous();
     let_next_start();
     const uint32_t t0 = blockIdx.x * p.rows, rows = min(p.rows, p.total - t0), part = blockIdx.y;
@@ -691,14 +734,14 @@ static __global__ void __launch_bounds__(256) cache_read_flat_kernel(const __gri
             const int8_t* const q = codes + at0.x + h0 * p.code_head + e;
             const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(q) % V);
             const Word* const from = reinterpret_cast<const Word*>(q - off);
-            w = __ldg(from) >> (8u * off);
-            if (off + min(V, left) > V) w |= __ldg(from + 1) << (8u * (V - off));
-            s0 = __ldg(scales + at0.y + h0 * p.scale_head);
+            w = ld_word(from) >> (8u * off);
+            if (off + min(V, left) > V) w |= ld_word(from + 1) << (8u * (V - off));
+            s0 = ld_float_if(scales + at0.y + h0 * p.scale_head, true);
         }
         if (left < V) {
             if (at1.x >= 0) {
-                next = __ldg(reinterpret_cast<const Word*>(codes + at1.x + h1 * p.code_head));
-                s1 = __ldg(scales + at1.y + h1 * p.scale_head);
+                next = ld_word(reinterpret_cast<const Word*>(codes + at1.x + h1 * p.code_head));
+                s1 = ld_float_if(scales + at1.y + h1 * p.scale_head, true);
             }
             w = (w & ((Word{1} << (8u * left)) - 1u)) | next << (8u * left);
         }
