@@ -1,0 +1,37 @@
+"""CUDA tensors handed to the C ABI as bare addresses: what is checked before, and the streams they are used on."""
+from __future__ import annotations
+
+
+def as_stream(stream, device: int):
+    """The torch stream of `stream`: a stream of torch's, or a handle. Handle 0 is the default stream; ExternalStream
+    takes it for none given, and makes a new stream."""
+    import torch
+    if not isinstance(stream, int):
+        return stream
+    if stream == 0:
+        return torch.cuda.default_stream(device)
+    return torch.cuda.ExternalStream(stream, device=device)
+
+
+def device_rows(rows, dimension: int, dtype, what: str, stream=None):
+    """`rows`, checked, as a CUDA tensor [n, dimension] of `dtype` whose rows follow one another: the entry points take
+    an address and read n * dimension values from it. A view of other strides (rows of wider ones, such as the codes
+    that quantize_rows gives; a broadcast row; a transpose) is copied, on `stream` where one is given."""
+    import torch
+
+    from .exact import DimensionMismatch
+    if rows.dim() != 2 or rows.shape[1] != dimension:
+        raise DimensionMismatch(f"{what} dimension does not match index")
+    if rows.dtype is not dtype:
+        raise ValueError(f"{what} rows must be {dtype}, not {rows.dtype}")
+    if not rows.is_cuda:
+        raise ValueError(f"{what} rows must be on a CUDA device, not on {rows.device}")
+    if rows.is_contiguous():
+        return rows
+    if stream is None:
+        return rows.contiguous()
+    s = as_stream(stream, rows.get_device())
+    with torch.cuda.stream(s):
+        copy = rows.contiguous()
+    rows.record_stream(s)
+    return copy

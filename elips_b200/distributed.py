@@ -213,6 +213,8 @@ class ShardedExactIndex:
     def _search_peer(self, queries, k, mask, cand):
         import torch
         from . import _capi as capi
+        from ._device import device_rows
+        queries = device_rows(queries, self.local.dimension, self.local._torch_dtype(), "query")
         nq = queries.shape[0]
         self.peer.ensure(nq, k)
         my_slot, bounds, blocks = self.peer.slots(nq)

@@ -19,6 +19,7 @@ from typing import Optional
 import numpy as np
 
 from . import _capi as capi
+from ._device import device_rows
 
 METRICS = {"cosine": capi.METRIC_COSINE, "euclidean": capi.METRIC_EUCLIDEAN,
            "dot_product": capi.METRIC_DOT_PRODUCT}
@@ -60,6 +61,10 @@ class ExactIndex:
                    "elips_b200_exact_create")
         self._h = handle
 
+    def _torch_dtype(self):
+        import torch
+        return torch.int8 if self.precision == "int8" else torch.float32
+
     # -- IndexPort ---------------------------------------------------------
     def add(self, rows: np.ndarray) -> None:
         """Appends rows (n x dimension) to the next slots."""
@@ -72,9 +77,7 @@ class ExactIndex:
     def add_device(self, rows, stream=None) -> None:
         """Appends rows held in a CUDA tensor [n, dimension] (float32, int8 for int8)."""
         import torch
-        if rows.dim() != 2 or rows.shape[1] != self.dimension:
-            raise DimensionMismatch("vector dimension does not match index")
-        rows = rows.contiguous()
+        rows = device_rows(rows, self.dimension, self._torch_dtype(), "vector", stream)
         s = stream if stream is not None else torch.cuda.current_stream(rows.device).cuda_stream
         capi.check(capi.LIB.elips_b200_exact_add_device(self._h, rows.data_ptr(), rows.shape[0], s),
                    "elips_b200_exact_add_device")
@@ -152,12 +155,12 @@ class ExactIndex:
 
     # -- device-pointer entry points (torch tensors as plumbing) -----------
     def search_device(self, queries, k: int, mask=None, out_dist=None, out_rows=None, stream=None):
-        """queries: CUDA tensor [nq, dimension] (float32, int8 for int8). Asynchronous on
-        `stream` (default: torch's current stream). Returns (dist, rows) CUDA tensors."""
+        """queries: CUDA tensor [nq, dimension] (float32, int8 for int8), of any strides (rows
+        that do not follow one another are copied). Asynchronous on `stream` (default: torch's
+        current stream). Returns (dist, rows) CUDA tensors."""
         import torch
+        queries = device_rows(queries, self.dimension, self._torch_dtype(), "query", stream)
         nq = queries.shape[0]
-        if queries.shape[1] != self.dimension:
-            raise DimensionMismatch("query dimension does not match index")
         if out_dist is None:
             out_dist = torch.empty((nq, k), dtype=torch.float32, device=queries.device)
         if out_rows is None:
@@ -171,6 +174,7 @@ class ExactIndex:
     def search_candidates_device(self, queries, k: int, row_offset: int, out_cand, mask=None, stream=None):
         """Shard-level search: writes [nq, k, 2] uint32-as-int32 candidate pairs to out_cand."""
         import torch
+        queries = device_rows(queries, self.dimension, self._torch_dtype(), "query", stream)
         s = stream if stream is not None else torch.cuda.current_stream(queries.device).cuda_stream
         capi.check(capi.LIB.elips_b200_exact_search_candidates_device(
             self._h, queries.data_ptr(), queries.shape[0], k,
@@ -184,6 +188,7 @@ class ExactIndex:
         an int32 CUDA tensor [nq] of ordered keys, all ones = none) are shared
         with the other shards searching the same queries."""
         import torch
+        queries = device_rows(queries, self.dimension, self._torch_dtype(), "query", stream)
         s = stream if stream is not None else torch.cuda.current_stream(queries.device).cuda_stream
         capi.check(capi.LIB.elips_b200_exact_search_candidates_shared_device(
             self._h, queries.data_ptr(), queries.shape[0], k, mask.data_ptr() if mask is not None else None,

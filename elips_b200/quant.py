@@ -19,6 +19,7 @@ from typing import Optional
 import numpy as np
 
 from . import _capi as capi
+from ._device import device_rows
 from .exact import METRICS, DimensionMismatch
 
 CODECS = {"pq": capi.CODEC_PQ, "opq": capi.CODEC_OPQ, "sq8": capi.CODEC_SQ8}
@@ -89,6 +90,7 @@ class QuantizedIndex:
 
     def search_device(self, queries, k: int, stream=None):
         import torch
+        queries = device_rows(queries, self.dimension, torch.float32, "query", stream)
         nq = queries.shape[0]
         d = torch.empty((nq, k), dtype=torch.float32, device=queries.device)
         r = torch.empty((nq, k), dtype=torch.int64, device=queries.device)
