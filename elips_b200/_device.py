@@ -3,14 +3,18 @@ from __future__ import annotations
 
 
 def as_stream(stream, device: int):
-    """The torch stream of `stream`: a stream of torch's, or a handle. Handle 0 is the default stream; ExternalStream
-    takes it for none given, and makes a new stream."""
+    """The torch stream of `stream` (a stream of torch's, an object with its handle as `cuda_stream`, or a handle) for
+    work on `device`. The default stream's handle is 0, or 1 for the legacy one that it is; ExternalStream takes 0 for
+    none given, and would make a new stream."""
     import torch
-    if not isinstance(stream, int):
-        return stream
-    if stream == 0:
+    handle = stream if isinstance(stream, int) else stream.cuda_stream
+    if handle in (0, 1):
         return torch.cuda.default_stream(device)
-    return torch.cuda.ExternalStream(stream, device=device)
+    if isinstance(stream, torch.cuda.Stream):
+        if stream.device_index != device:
+            raise ValueError(f"the stream is on cuda:{stream.device_index}, the tensors on cuda:{device}")
+        return stream
+    return torch.cuda.ExternalStream(handle, device=device)
 
 
 def device_rows(rows, dimension: int, dtype, what: str, stream=None):

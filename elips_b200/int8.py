@@ -36,6 +36,7 @@ import struct
 import torch
 
 from . import _capi as capi
+from ._device import as_stream
 from .exact import DimensionMismatch
 
 _LIB = capi.LIB
@@ -93,15 +94,11 @@ def _vector(t, n: int, what: str) -> int:
     return t.data_ptr()
 
 
-def _handle(stream) -> int:
-    return stream if isinstance(stream, int) else stream.cuda_stream
-
-
 @contextlib.contextmanager
 def _using(stream, device: int, *tensors):
     """Makes `stream` current, so that what is allocated belongs to it, and
     keeps the tensors' memory until its work is done."""
-    s = torch.cuda.ExternalStream(_handle(stream), device=device)
+    s = as_stream(stream, device)
     with torch.cuda.stream(s):
         yield
     for t in tensors:
