@@ -58,7 +58,10 @@ int elips_b200_device_count(int* count_out) {
 
 int elips_b200_device_error(int device, int* code_out) {
     if (code_out == nullptr) return ELIPS_B200_INVALID_ARGUMENT;
-    return guarded([&] { *code_out = eb::read_and_clear_device_error(device); });
+    return guarded([&] {
+        *code_out = eb::read_and_clear_device_error(device);
+        if (*code_out == 0) *code_out = eb::take_int8_error(device);  // else the next call finds it
+    });
 }
 
 int elips_b200_wait_selftest(int device, uint64_t cycles) {

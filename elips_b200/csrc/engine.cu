@@ -13,6 +13,7 @@
 #include "engine.cuh"
 #include "exact_topk.cuh"
 #include "profiler.cuh"
+#include "wait_selftest.cuh"
 
 namespace eb {
 
@@ -992,25 +993,6 @@ void merge_candidates(int device, const uint2* cand, uint32_t nq, uint32_t lists
     check_cuda(cudaGetLastError(), ELIPS_B200_KERNEL_LAUNCH_FAILED, "merge kernel launch");
 }
 
-namespace {
-
-// One thread waits on an mbarrier that nothing arrives on, for `budget`
-// cycles: the bounded wait expires, records the device error word and raises
-// the CTA's abort flag, the path every pipeline wait takes when a producer or
-// consumer is lost. Nothing asynchronous is in flight, so returning with the
-// barrier pending is safe.
-__global__ void wait_selftest_kernel(long long budget) {
-    __shared__ __align__(8) uint64_t bar;
-    __shared__ int abort_flag;
-    if (threadIdx.x != 0) return;
-    mbar_init(smem_u32(&bar), 1);
-    abort_flag = 0;
-    fence_mbarrier_init();
-    mbar_wait_for(smem_u32(&bar), 0, &abort_flag, budget);
-}
-
-}  // namespace
-
 int wait_selftest(int device, long long budget) {
     if (budget < 1 || budget > kWaitTimeoutCycles)
         fail(ELIPS_B200_INVALID_ARGUMENT, "wait budget must be in [1, 2^31] cycles");
@@ -1031,8 +1013,7 @@ int read_and_clear_device_error(int device) {
     const int zero = 0;
     check_cuda(cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int)), ELIPS_B200_TRANSFER_FAILED,
                "clear device error");
-    const int rows8 = take_int8_error(device);
-    return code != 0 ? code : rows8;
+    return code;
 }
 
 }  // namespace eb

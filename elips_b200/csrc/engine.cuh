@@ -205,6 +205,9 @@ void merge_candidates(int device, const uint2* cand, uint32_t nq, uint32_t lists
                       int64_t* out_rows, uint2* out_cand, cudaStream_t stream, uint32_t sub = 1,
                       uint32_t lists_last = 0, uint32_t len = 0);
 
+// The error word of the search kernels, read and cleared after the device's
+// work is done. A search reports only this one: what another call's 8-bit
+// product left is not its failure.
 int read_and_clear_device_error(int device);
 // The error word of the 8-bit operators' kernels, read and cleared (no
 // synchronisation of its own).

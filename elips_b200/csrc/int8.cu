@@ -13,6 +13,7 @@
 #include "int8_gemm.cuh"
 #include "int8_kernels.cuh"
 #include "profiler.cuh"
+#include "wait_selftest.cuh"
 
 namespace eb {
 namespace {
@@ -649,6 +650,15 @@ cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
 
 }  // namespace
 
+void int8_wait_selftest(int device, long long budget) {
+    if (budget < 1 || budget > kWaitTimeoutCycles) bad("wait budget must be in [1, 2^31] cycles");
+    DeviceGuard g(device);
+    device_props(device);
+    wait_selftest_kernel<<<1, 32>>>(budget);
+    launch_ok("wait self-test launch");
+    check_cuda(cudaDeviceSynchronize(), ELIPS_B200_KERNEL_LAUNCH_FAILED, "wait self-test");
+}
+
 int take_int8_error(int device) {
     DeviceGuard g(device);
     int code = 0;
@@ -666,6 +676,10 @@ int take_int8_error(int device) {
 using eb::guarded;
 
 extern "C" {
+
+int elips_b200_int8_wait_selftest(int device, uint64_t cycles) {
+    return guarded([&] { eb::int8_wait_selftest(device, static_cast<long long>(cycles)); });
+}
 
 int elips_b200_quantize_rows(int device, const void* x, int type, size_t n, size_t d, int64_t x_stride, int8_t* codes,
                              size_t code_stride, float* scales, void* stream) {

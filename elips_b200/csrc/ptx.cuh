@@ -15,9 +15,8 @@
 namespace eb {
 
 // Device-global error word (0 = ok). Written with atomicCAS so the first error
-// wins; read and cleared by the host through read_and_clear_device_error().
-// Each translation unit that includes this header has its own word; the host
-// reads engine.cu's and int8.cu's.
+// wins. Each translation unit that includes this header has its own word: a
+// search reads engine.cu's, elips_b200_device_error that and int8.cu's.
 static __device__ int g_device_error = 0;
 
 enum DeviceError : int {

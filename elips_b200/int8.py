@@ -20,6 +20,9 @@ Everything takes CUDA tensors, runs asynchronously on `stream` (default: the
 current stream of the tensors' device) and can be captured into a CUDA graph.
 With another stream the outputs belong to it and the inputs are held until its
 work is done; ordering that work after the inputs are written is the caller's.
+A product one of whose device-side waits expired (about a second; a lost load)
+leaves its output unwritten without an error of its call: the next
+elips_b200._capi.device_error(device) is not 0.
 These are the serving forms: rounding has no gradient, so an input that
 requires one is refused while gradients are recorded.
 

@@ -75,7 +75,9 @@ ELIPS_B200_API const char* elips_b200_status_string(int status);
 ELIPS_B200_API int elips_b200_device_count(int* count_out);
 
 /* Reads and clears the device-side error word of `device` that bounded waits
- * write on timeout (0 = none). Synchronises the device. */
+ * write on timeout (0 = none). Synchronises the device. The 8-bit operators
+ * have a word of their own, read where the searches' is 0; a search neither
+ * reports nor clears it. */
 ELIPS_B200_API int elips_b200_device_error(int device, int* code_out);
 
 /* Self-test of the bounded device waits; no counterpart in the reference.
@@ -86,6 +88,11 @@ ELIPS_B200_API int elips_b200_device_error(int device, int* code_out);
  * reported (the expected outcome; the error word is cleared again and the
  * context stays usable), ELIPS_B200_OK if the wait completed. */
 ELIPS_B200_API int elips_b200_wait_selftest(int device, uint64_t cycles);
+
+/* The same wait among the 8-bit operators' kernels. It leaves their error word
+ * set, as a product whose wait expired does: the call returns ELIPS_B200_OK
+ * and elips_b200_device_error reports it. */
+ELIPS_B200_API int elips_b200_int8_wait_selftest(int device, uint64_t cycles);
 
 /* ------------------------------------------------ exact brute-force index */
 /* Replaces ExactIndex (include/elips/index_engine/ExactIndex.hpp:26-66) and
@@ -584,7 +591,9 @@ ELIPS_B200_API int elips_b200_ivfpq_train(int device, int metric, const float* r
  * Element types are ELIPS_B200_PRECISION_FP32, _FP16 or _BF16. All pointers
  * are DEVICE pointers on `device`, every call is asynchronous on `stream` and
  * can be captured into a CUDA graph. Strides are in elements; the innermost
- * axis has stride 1. No sizes are too small: zero rows launch nothing. */
+ * axis has stride 1. No sizes are too small: zero rows launch nothing. A
+ * product one of whose device-side waits expires leaves its output unwritten,
+ * which its call, being asynchronous, cannot say: elips_b200_device_error does. */
 
 /* codes[i * code_stride + j] and scales[i] of n rows of d values (d in
  * [1, 2^24]) at x + i * x_stride. A code_stride that is a multiple of 16 and
