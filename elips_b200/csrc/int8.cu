@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 
 #include "../../include/elips_b200.h"
@@ -541,28 +542,64 @@ void gemm_int8(int num_sms, GemmParams p, int out_type, cudaStream_t stream) {
     product();
 }
 
-// Rows of `width` bytes, `pitch` bytes apart.
+// Runs of `width` bytes, one at each combination of up to four axes' steps.
 struct Region {
-    uintptr_t base;
-    int64_t rows, width, pitch;
-    uintptr_t low() const { return pitch < 0 ? base + static_cast<uintptr_t>((rows - 1) * pitch) : base; }
-    uintptr_t high() const { return (pitch < 0 ? base : base + static_cast<uintptr_t>((rows - 1) * pitch)) + width; }
+    using Wide = __int128;  // no product of a size and a stride passes it
+    uintptr_t base = 0;     // of the lowest run
+    int64_t width = 0;
+    int64_t count[4] = {1, 1, 1, 1};
+    Wide step[4] = {};
+    Wide all = 0;           // bytes from the first to behind the last of the runs
+    // The same without the axes whose step is a multiple of `whole`.
+    Wide extent(Wide whole) const {
+        Wide e = width;
+        for (int i = 0; i < 4; ++i)
+            if (step[i] % whole != 0) e += (count[i] - 1) * step[i];
+        return e;
+    }
 };
 
-Region region(const void* p, int64_t rows, int64_t width, int64_t pitch) {
-    return {reinterpret_cast<uintptr_t>(p), rows, width, rows > 1 ? pitch : 0};
+struct Axis {
+    int64_t count;
+    Region::Wide step;  // bytes
+};
+
+Region region(const void* p, int64_t width, std::initializer_list<Axis> axes) {
+    Region r;
+    r.width = r.all = width;
+    Region::Wide base = reinterpret_cast<uintptr_t>(p);
+    int i = 0;
+    for (const Axis& a : axes) {
+        if (a.count <= 0) r.width = 0;
+        if (a.count > 1) {
+            r.count[i] = a.count;
+            r.step[i] = a.step < 0 ? -a.step : a.step;
+            r.all += (a.count - 1) * r.step[i];
+            if (a.step < 0) base += (a.count - 1) * a.step;
+        }
+        ++i;
+    }
+    r.base = static_cast<uintptr_t>(base);
+    return r;
 }
 
-// Whether two regions share a byte. Columns side by side in one buffer do not;
-// rows of two different pitches that reach into one another are taken to.
+// Whether two regions share a byte. They do not where one ends before the
+// other starts, or where for some step S all bytes of one are, modulo S, before
+// or behind those of the other: columns side by side in one buffer, parts or
+// heads that take turns, codes and scales of each page one after the other.
+// Layouts that interlace in no such way are taken to share one.
 bool overlap(const Region& a, const Region& b) {
-    if (a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
-    if (a.high() <= b.low() || b.high() <= a.low()) return false;
-    if (a.rows > 1 && b.rows > 1 && a.pitch != b.pitch) return true;
-    const int64_t pitch = a.rows > 1 ? a.pitch : b.pitch;
-    if (pitch <= 0) return true;
-    const int64_t ahead = (static_cast<int64_t>(b.base - a.base) % pitch + pitch) % pitch;
-    return ahead < a.width || ahead + b.width > pitch;
+    using Wide = Region::Wide;
+    if (a.width <= 0 || b.width <= 0) return false;
+    const Wide from_a = static_cast<Wide>(b.base) - static_cast<Wide>(a.base);
+    if (from_a >= a.all || -from_a >= b.all) return false;
+    for (int i = 0; i < 8; ++i) {
+        const Wide s = i < 4 ? a.step[i] : b.step[i - 4];
+        if (s <= 0) continue;
+        const Wide ea = a.extent(s), eb = b.extent(s), ahead = (from_a % s + s) % s;
+        if (ahead >= ea && ahead + eb <= s) return false;
+    }
+    return true;
 }
 
 int64_t type_bytes(int type) {
@@ -573,12 +610,59 @@ int64_t type_bytes(int type) {
 // kernel's blocks each read every row), so no output may lie on an input.
 void check_gemm_apart(const elips_b200_gemm& g) {
     const int64_t a = type_bytes(g.a_type), o = type_bytes(g.out_type);
-    const Region out = region(g.out, g.m, g.n * o, g.out_stride * o);
-    if (overlap(out, region(g.a, g.m, g.k * a, g.a_stride * a)) ||
-        overlap(out, region(g.b, g.n, g.k, g.b_stride)) || overlap(out, region(g.b_scales, 1, g.n * 4, 0)) ||
-        (g.a_type == ELIPS_B200_PRECISION_INT8 && overlap(out, region(g.a_scales, 1, g.m * 4, 0))) ||
-        (g.bias != nullptr && overlap(out, region(g.bias, 1, g.n * type_bytes(g.bias_type), 0))))
+    const Region out = region(g.out, g.n * o, {{g.m, Region::Wide{g.out_stride} * o}});
+    if (overlap(out, region(g.a, g.k * a, {{g.m, Region::Wide{g.a_stride} * a}})) ||
+        overlap(out, region(g.b, g.k, {{g.n, g.b_stride}})) || overlap(out, region(g.b_scales, g.n * 4, {})) ||
+        (g.a_type == ELIPS_B200_PRECISION_INT8 && overlap(out, region(g.a_scales, g.m * 4, {}))) ||
+        (g.bias != nullptr && overlap(out, region(g.bias, g.n * type_bytes(g.bias_type), {}))))
         bad("the output shares memory with an input");
+}
+
+Region codes_region(const elips_b200_cache& c) {
+    const int64_t* s = c.code_strides;
+    return region(c.codes, c.dim, {{c.parts, s[0]}, {c.pages, s[1]}, {c.page_size, s[2]}, {c.heads, s[3]}});
+}
+
+Region scales_region(const elips_b200_cache& c) {
+    Region::Wide s[4];
+    for (int i = 0; i < 4; ++i) s[i] = Region::Wide{c.scale_strides[i]} * 4;
+    return region(c.scales, 4, {{c.parts, s[0]}, {c.pages, s[1]}, {c.page_size, s[2]}, {c.heads, s[3]}});
+}
+
+Region rows_region(const elips_b200_cache& c, const elips_b200_rows& r, size_t t, int type) {
+    const int64_t bytes = type_bytes(type);
+    return region(r.data, c.dim * bytes, {{static_cast<int64_t>(t), Region::Wide{r.stride_row} * bytes},
+                                          {c.heads, Region::Wide{r.stride_head} * bytes}});
+}
+
+// Claims overwrite scale words, and rows their codes, before other rows and
+// slots have been read.
+void check_write_apart(const elips_b200_cache& c, const elips_b200_rows* rows, int type, size_t t, const void* slots,
+                       int slots64) {
+    if (t == 0 || c.pages == 0) return;
+    const Region codes = codes_region(c), scales = scales_region(c);
+    const Region list = region(slots, static_cast<int64_t>(t) * (slots64 ? 8 : 4), {});
+    bool shared = overlap(codes, scales) || overlap(list, codes) || overlap(list, scales);
+    for (int64_t i = 0; i < c.parts; ++i) {
+        const Region x = rows_region(c, rows[i], t, type);
+        shared = shared || overlap(x, codes) || overlap(x, scales);
+    }
+    if (shared) bad("the cache shares memory with the rows or slots, or its codes with its scales");
+}
+
+void check_read_apart(const elips_b200_cache& c, const elips_b200_sequences& q, const elips_b200_rows* out, int type) {
+    if (q.total == 0) return;
+    const size_t total = static_cast<size_t>(q.total);
+    const int64_t entry = q.table_64bit ? 8 : 4, columns = q.sequences > 0 ? q.table_width : 0;
+    const Region inputs[4] = {c.pages > 0 ? codes_region(c) : Region{}, c.pages > 0 ? scales_region(c) : Region{},
+                              region(q.page_table, columns * entry, {{q.sequences, Region::Wide{q.table_stride} * entry}}),
+                              region(q.offsets, q.sequences > 0 ? (q.sequences + 1) * (q.offsets_64bit ? 8 : 4) : 0, {})};
+    bool shared = c.parts == 2 && overlap(rows_region(c, out[0], total, type), rows_region(c, out[1], total, type));
+    for (int64_t i = 0; i < c.parts; ++i) {
+        const Region x = rows_region(c, out[i], total, type);
+        for (const Region& in : inputs) shared = shared || overlap(x, in);
+    }
+    if (shared) bad("an output shares memory with what is read or with the other part's output");
 }
 
 void check_gemm(const elips_b200_gemm& g) {
@@ -688,9 +772,9 @@ int elips_b200_quantize_rows(int device, const void* x, int type, size_t n, size
         eb::check_rows(n, d, type);
         if (code_stride < d) eb::bad("codes of neighbouring rows overlap");
         const int64_t rows = static_cast<int64_t>(n), width = static_cast<int64_t>(d), bytes = eb::type_bytes(type);
-        const eb::Region in = eb::region(x, rows, width * bytes, x_stride * bytes);
-        const eb::Region out = eb::region(codes, rows, width, static_cast<int64_t>(code_stride));
-        const eb::Region held = eb::region(scales, 1, rows * 4, 0);
+        const eb::Region in = eb::region(x, width * bytes, {{rows, eb::Region::Wide{x_stride} * bytes}});
+        const eb::Region out = eb::region(codes, width, {{rows, static_cast<eb::Region::Wide>(code_stride)}});
+        const eb::Region held = eb::region(scales, rows * 4, {});
         if (eb::overlap(in, out) || eb::overlap(in, held) || eb::overlap(out, held))
             eb::bad("rows, codes and scales share memory");
         eb::DeviceGuard g(device);
@@ -720,6 +804,7 @@ int elips_b200_cache_write(int device, const elips_b200_cache* cache, const elip
         eb::check_cache(*cache);
         eb::check_cache_rows(*cache, rows, type, t);
         if (t > 0 && slots == nullptr) eb::bad("slots missing");
+        eb::check_write_apart(*cache, rows, type, t, slots, slots_64bit);
         eb::DeviceGuard g(device);
         eb::device_props(device);
         eb::cache_write(*cache, rows, type, t, slots, slots_64bit, eb::as_stream(stream));
@@ -735,11 +820,11 @@ int elips_b200_cache_read(int device, const elips_b200_cache* cache, const elips
     return guarded([&] {
         eb::check_cache(*cache);
         eb::check_cache_rows(*cache, out, type, static_cast<size_t>(q.total));
-        if (q.total > 0 && cache->parts == 2 && out[0].data == out[1].data) eb::bad("the parts share one output");
         if (q.sequences > static_cast<int64_t>(eb::kMaxRows) || q.table_width > static_cast<int64_t>(eb::kMaxRows))
             eb::bad("page table too large");
         if (q.total > 0 && q.sequences > 0 && q.offsets == nullptr) eb::bad("offsets missing");
         if (q.total > 0 && q.sequences > 0 && q.table_width > 0 && q.page_table == nullptr) eb::bad("page table missing");
+        eb::check_read_apart(*cache, q, out, type);
         eb::DeviceGuard g(device);
         eb::cache_read(eb::device_props(device).num_sms, *cache, q, out, type, zero_behind, eb::as_stream(stream));
     });

@@ -273,7 +273,8 @@ def cache_write(codes, scales, rows, slots, stream=None) -> None:
     part; each of its rows gets a scale per head. Row i goes to slot slots[i]
     (int32 or int64): row s % page of page s // page. A slot below 0 or past
     the last one is skipped (padding); of a slot given twice the last row is
-    kept. Slots that are not named stay as they are."""
+    kept. Slots that are not named stay as they are. A cache that shares memory
+    with rows or slots is refused."""
     cache, parts, heads, dim = _cache(codes, scales, True)
     if len(rows) != parts:
         raise DimensionMismatch(f"{len(rows)} tensors of rows for a cache of {parts} parts")
@@ -309,8 +310,8 @@ def cache_read(codes, scales, page_table, offsets, total: int, dtype=torch.bfloa
     or lies past the table's width, reads as zeros, as do rows in front of
     offsets[0]. `total` is the number of output rows, offsets[-1] or more; rows
     behind the last sequence are zeros, or with `out` (a tuple of tensors like
-    the result, of any strides but the last, that share no memory) stay as they
-    are."""
+    the result, of any strides but the last) stay as they are. Outputs that
+    share memory with one another or with what is read are refused."""
     cache, parts, heads, dim = _cache(codes, scales, False)
     table_wide, offsets_wide = _indexes(page_table, "page_table"), _indexes(offsets, "offsets")
     shape = page_table.shape

@@ -649,7 +649,8 @@ typedef struct {
 /* Quantises rows[part][i] into slot slots[i] (int32, or int64 where
  * slots_64bit) for i < t, one scale per row and head. A slot below 0 or past
  * the last one is skipped; of a slot given twice the last row is kept. rows:
- * one entry per part. Calls on different streams may run at once on disjoint
+ * one entry per part. A cache that shares memory with rows or slots, or whose
+ * codes share some with its scales, is refused. Calls on different streams may run at once on disjoint
  * slots. */
 ELIPS_B200_API int elips_b200_cache_write(int device, const elips_b200_cache* cache, const elips_b200_rows* rows,
                                           int type, size_t t, const void* slots, int slots_64bit, void* stream);
@@ -669,8 +670,9 @@ typedef struct {
 /* Reads sequences back into packed rows, one output per part. A page that is
  * no page of the cache, or past the table's width, reads as zeros, and so do
  * rows in front of offsets[0]. Rows from offsets[sequences] on are zeroed
- * where zero_behind, else left as they are. The outputs must share no memory
- * with one another or with what is read (one output for two parts is refused). */
+ * where zero_behind, else left as they are. Outputs that share memory with one
+ * another or with what is read are refused; rows, heads or parts that take
+ * turns in one buffer share none. */
 ELIPS_B200_API int elips_b200_cache_read(int device, const elips_b200_cache* cache,
                                          const elips_b200_sequences* sequences, const elips_b200_rows* out, int type,
                                          int zero_behind, void* stream);
