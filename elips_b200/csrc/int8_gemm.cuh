@@ -631,12 +631,12 @@ static __global__ void __launch_bounds__(kPairThreads, 1)
         auto fetch = [&](uint32_t i) {
             const PairUnit u = pair_unit(i, whole, n_mt, n_nt);
             const uint32_t m = u.mt * kPairM + rank * (kPairM / 2) + quad * 32u + lane;
-            sa = ld_float_if(p.a_scales + m, m < p.m);
+            sa = ld_float_if(p.a_scales + m, m < p.m ? 0 : -1);
 #pragma unroll
             for (uint32_t j = 0; j < kOwn; ++j) {
                 const uint32_t n = u.n0 + half * (u.bn / 2) + j * 32u + lane;
                 const bool there = n < p.n && j * 32u < u.bn / 2;
-                sb[j] = make_float2(ld_float_if(p.b_scales + n, there), 0.0f);
+                sb[j] = make_float2(ld_float_if(p.b_scales + n, there ? 0 : -1), 0.0f);
                 if (there && p.bias != nullptr) sb[j].y = bias_at(p.bias, p.bias_type, n);
             }
         };
@@ -765,7 +765,7 @@ static __global__ void __launch_bounds__(256) repack_codes_kernel(const __grid_c
             // is read only where it holds one of them.
             const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src)) & 3u;
             const uint32_t* at = reinterpret_cast<const uint32_t*>(src - off);
-            const uint32_t lo = ld4_if(at, true), hi = ld4_if(at + 1, off != 0u);
+            const uint32_t lo = ld4_if(at), hi = ld4_if(at + 1, off != 0u ? 0 : -1);
             w = __funnelshift_r(lo, hi, 8u * off);
         } else {
             for (uint32_t j = 0; c + j < p.k; ++j) w |= static_cast<uint32_t>(static_cast<uint8_t>(src[j])) << (8u * j);

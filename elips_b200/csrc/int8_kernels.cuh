@@ -266,38 +266,39 @@ __device__ __forceinline__ uint4 ld16(const void* at) {
     asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at));
     return v;
 }
-// Zero where not `there`: predicated, so that a batch of them is under way at once.
-__device__ __forceinline__ uint2 ld8_if(const void* at, bool there) {
+// Zero where `there` is negative: predicated, so that a batch of them is under
+// way at once, on the value that a row's place is.
+__device__ __forceinline__ uint2 ld8_if(const void* at, int64_t there = 0) {
     uint2 v;
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\t"
+        "{\n\t.reg .pred p;\n\tsetp.ge.s64 p, %3, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\t"
         "@p ld.global.v2.u32 {%0, %1}, [%2];\n\t}"
         : "=&r"(v.x), "=&r"(v.y)
-        : "l"(at), "r"(there ? 1u : 0u));
+        : "l"(at), "l"(there));
     return v;
 }
-__device__ __forceinline__ uint32_t ld4_if(const void* at, bool there) {
+__device__ __forceinline__ uint32_t ld4_if(const void* at, int64_t there = 0) {
     uint32_t v;
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u32 %0, 0;\n\t@p ld.global.u32 %0, [%1];\n\t}"
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ge.s64 p, %2, 0;\n\tmov.u32 %0, 0;\n\t@p ld.global.u32 %0, [%1];\n\t}"
                  : "=&r"(v)
-                 : "l"(at), "r"(there ? 1u : 0u));
+                 : "l"(at), "l"(there));
     return v;
 }
-__device__ __forceinline__ uint32_t ld2_if(const void* at, bool there) {
+__device__ __forceinline__ uint32_t ld2_if(const void* at, int64_t there = 0) {
     uint32_t v;
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u32 %0, 0;\n\t@p ld.global.u16 %0, [%1];\n\t}"
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ge.s64 p, %2, 0;\n\tmov.u32 %0, 0;\n\t@p ld.global.u16 %0, [%1];\n\t}"
                  : "=&r"(v)
-                 : "l"(at), "r"(there ? 1u : 0u));
+                 : "l"(at), "l"(there));
     return v;
 }
-__device__ __forceinline__ uint32_t ld1_if(const void* at, bool there) {
+__device__ __forceinline__ uint32_t ld1_if(const void* at, int64_t there = 0) {
     uint32_t v;
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u32 %0, 0;\n\t@p ld.global.u8 %0, [%1];\n\t}"
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ge.s64 p, %2, 0;\n\tmov.u32 %0, 0;\n\t@p ld.global.u8 %0, [%1];\n\t}"
                  : "=&r"(v)
-                 : "l"(at), "r"(there ? 1u : 0u));
+                 : "l"(at), "l"(there));
     return v;
 }
-__device__ __forceinline__ float ld_float_if(const float* at, bool there) { return __uint_as_float(ld4_if(at, there)); }
+__device__ __forceinline__ float ld_float_if(const float* at, int64_t there = 0) { return __uint_as_float(ld4_if(at, there)); }
 
 // A slot given twice in one call keeps the last of its rows. Up to
 // kDupScanRows rows each row looks for its slot among the later ones (which
@@ -600,9 +601,9 @@ __device__ __forceinline__ float code_f32(uint32_t turned, uint32_t byte) {
     return __uint_as_float(__byte_perm(turned, 0x4B000000u, 0x7440u | byte)) - 8388736.0f;  // 2^23 + 128
 }
 
-// V codes, zeros where there are none.
+// V codes, zeros where there are none (`there` is negative).
 template <int V>
-__device__ __forceinline__ void load_codes(const int8_t* src, bool there, uint32_t (&w)[(V + 3) / 4]) {
+__device__ __forceinline__ void load_codes(const int8_t* src, int64_t there, uint32_t (&w)[(V + 3) / 4]) {
     if constexpr (V == 8) {
         const uint2 u = ld8_if(src, there);
         w[0] = u.x;
@@ -666,9 +667,9 @@ static __global__ void __launch_bounds__(kReadThreads) cache_read_kernel(const _
 #pragma unroll
             for (int b = 0; b < kReadBatch; ++b) at[b] = row_at[min(r0 + b * p.ny, rows - 1u)];
 #pragma unroll
-            for (int b = 0; b < kReadBatch; ++b) load_codes<V>(codes + at[b].x, at[b].x >= 0, w[b]);
+            for (int b = 0; b < kReadBatch; ++b) load_codes<V>(codes + at[b].x, at[b].x, w[b]);
 #pragma unroll
-            for (int b = 0; b < kReadBatch; ++b) sc[b] = ld_float_if(scales + at[b].y, at[b].x >= 0);
+            for (int b = 0; b < kReadBatch; ++b) sc[b] = ld_float_if(scales + at[b].y, at[b].x);
 #pragma unroll
             for (int b = 0; b < kReadBatch; ++b) {
                 if (r0 + b * p.ny < rows && at[b].x != kRowBehind) {
@@ -698,8 +699,8 @@ static __global__ void __launch_bounds__(256) cache_read_flat_kernel(const __gri
     using Word = typename std::conditional<V == 8, unsigned long long, uint32_t>::type;
     __shared__ longlong2 row_at[kReadRows];
     auto ld_word = [](const Word* at) -> Word {
-        if constexpr (V == 4) return ld4_if(at, true);
-        const uint2 u = ld8_if(at, true);
+        if constexpr (V == 4) return ld4_if(at);
+        const uint2 u = ld8_if(at);
         return static_cast<Word>(static_cast<uint64_t>(u.y) << 32 | u.x);
     };
     await_previous();
@@ -736,12 +737,12 @@ static __global__ void __launch_bounds__(256) cache_read_flat_kernel(const __gri
             const Word* const from = reinterpret_cast<const Word*>(q - off);
             w = ld_word(from) >> (8u * off);
             if (off + min(V, left) > V) w |= ld_word(from + 1) << (8u * (V - off));
-            s0 = ld_float_if(scales + at0.y + h0 * p.scale_head, true);
+            s0 = ld_float_if(scales + at0.y + h0 * p.scale_head);
         }
         if (left < V) {
             if (at1.x >= 0) {
                 next = ld_word(reinterpret_cast<const Word*>(codes + at1.x + h1 * p.code_head));
-                s1 = ld_float_if(scales + at1.y + h1 * p.scale_head, true);
+                s1 = ld_float_if(scales + at1.y + h1 * p.scale_head);
             }
             w = (w & ((Word{1} << (8u * left)) - 1u)) | next << (8u * left);
         }
