@@ -24,7 +24,8 @@ A product one of whose device-side waits expired (about a second; a lost load)
 leaves its output unwritten without an error of its call: the next
 elips_b200._capi.device_error(device) is not 0.
 These are the serving forms: rounding has no gradient, so an input that
-requires one is refused while gradients are recorded.
+requires one is refused while gradients are recorded, and one with a tangent of
+forward-mode differentiation always.
 
 Rows that cannot be held: a row whose largest magnitude is below 127 * 2^-126
 becomes zeros with scale 0; a row with an infinity or a NaN gets a scale that
@@ -37,6 +38,7 @@ import contextlib
 import struct
 
 import torch
+from torch.autograd import forward_ad as _forward
 
 from . import _capi as capi
 from ._device import as_stream
@@ -57,6 +59,13 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
 
 def _refuse_grad() -> None:
     raise ValueError("8-bit operators have no gradient: detach the inputs or use torch.no_grad()")
+
+
+def _refuse_tangents(*tensors) -> None:
+    """Inside a level of forward-mode differentiation: refuses tensors with a tangent, which the result would lack.
+    torch.no_grad() does not turn that mode off."""
+    if any(t is not None and _forward.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError("8-bit operators have no gradient: unpack the dual tensors first")
 
 
 def _refuse_devices(*tensors) -> None:
@@ -115,6 +124,8 @@ def quantize_rows(x, stream=None):
     where d is no such multiple): gemm_int8 reads them as they are."""
     if x.requires_grad and torch.is_grad_enabled():
         _refuse_grad()
+    if _forward._current_level >= 0:
+        _refuse_tangents(x)
     kind = _float_type(x.dtype, "rows")
     pitch = _pitch(x, "rows", apart=False)
     n, d = x.shape
@@ -164,6 +175,8 @@ def _product(x, x_kind, x_scales, b, b_scales, bias, dtype, out, stream):
     if torch.is_grad_enabled() and (b_scales.requires_grad or x.requires_grad or (codes and x_scales.requires_grad) or
                                     (bias is not None and bias.requires_grad) or (out is not None and out.requires_grad)):
         _refuse_grad()
+    if _forward._current_level >= 0:
+        _refuse_tangents(x, x_scales, b_scales, bias, out)
     device = x.get_device()
     if device < 0 or b.get_device() != device or b_scales.get_device() != device or \
             (codes and x_scales.get_device() != device) or \
@@ -287,6 +300,8 @@ def cache_write(codes, scales, rows, slots, stream=None) -> None:
     packed = _rows(rows, t, heads, dim, dtype, "rows", False)
     if torch.is_grad_enabled() and (scales.requires_grad or rows[0].requires_grad or rows[-1].requires_grad):
         _refuse_grad()
+    if _forward._current_level >= 0:
+        _refuse_tangents(scales, *rows)
     device = codes.get_device()
     if device < 0 or scales.get_device() != device or slots.get_device() != device or \
             rows[0].get_device() != device or rows[-1].get_device() != device:
@@ -334,6 +349,8 @@ def cache_read(codes, scales, page_table, offsets, total: int, dtype=torch.bfloa
     kind = _float_type(dtype, "out")
     if torch.is_grad_enabled() and (scales.requires_grad or (not fresh and any(x.requires_grad for x in out))):
         _refuse_grad()
+    if _forward._current_level >= 0:
+        _refuse_tangents(scales, *(out or ()))
     device = codes.get_device()
     if device < 0 or scales.get_device() != device or page_table.get_device() != device or \
             offsets.get_device() != device or (not fresh and any(x.get_device() != device for x in out)):
