@@ -39,6 +39,7 @@ import struct
 
 import torch
 from torch.autograd import forward_ad as _forward
+from torch.autograd.graph import increment_version as _increment_version  # a written tensor that autograd saved is stale
 
 from . import _capi as capi
 from ._device import as_stream
@@ -185,7 +186,8 @@ def _product(x, x_kind, x_scales, b, b_scales, bias, dtype, out, stream):
     if stream is not None:
         with _using(stream, device, x, b, x_scales, b_scales, bias, out):
             return _product(x, x_kind, x_scales, b, b_scales, bias, dtype, out, None)
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = x.new_empty((m, n), dtype=dtype)
         out_pitch = n or 1
     status = _LIB.elips_b200_gemm_int8(
@@ -193,6 +195,8 @@ def _product(x, x_kind, x_scales, b, b_scales, bias, dtype, out, stream):
                            b_pitch, out_pitch, x_kind, bias_kind, kind, 0), _raw_stream(device))
     if status:
         capi.check(status, "elips_b200_gemm_int8")
+    if not fresh:
+        _increment_version(out)
     return out
 
 
@@ -312,6 +316,7 @@ def cache_write(codes, scales, rows, slots, stream=None) -> None:
     status = _LIB.elips_b200_cache_write(device, cache, packed, kind, t, slots.data_ptr(), wide, _raw_stream(device))
     if status:
         capi.check(status, "elips_b200_cache_write")
+    _increment_version((codes, scales))
 
 
 def cache_read(codes, scales, page_table, offsets, total: int, dtype=torch.bfloat16, out=None, stream=None):
@@ -373,4 +378,6 @@ def cache_read(codes, scales, page_table, offsets, total: int, dtype=torch.bfloa
     status = _LIB.elips_b200_cache_read(device, cache, seqs, packed, kind, fresh, _raw_stream(device))
     if status:
         capi.check(status, "elips_b200_cache_read")
+    if not fresh:
+        _increment_version(out)
     return out

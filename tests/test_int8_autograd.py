@@ -46,3 +46,50 @@ def test_tensors_without_tangents_go_on():
             ops.quantize_rows(torch.ones((4, 8)))
         with pytest.raises(ValueError, match="CUDA"):
             ops.linear_int8(forward_ad.unpack_dual(dual(4, 8)).primal, codes(4, 8), ONE)
+
+
+def writes(t):
+    """(what is written, the call) for every entry point that writes into tensors it is given."""
+    x, w = torch.ones((t, 32), device="cuda"), torch.ones((16, 32), device="cuda")
+    codes_x, sx = ops.quantize_rows(x)
+    codes_w, sw = ops.quantize_rows(w)
+    cache = torch.zeros((2, 4, 8, 1, 32), dtype=torch.int8, device="cuda")
+    scales = torch.zeros((2, 4, 8, 1), device="cuda")
+    slots, table = torch.arange(t, device="cuda"), torch.arange(4, device="cuda")[None]
+    offsets = torch.tensor([0, t], device="cuda")
+    out = torch.zeros((t, 16), device="cuda")
+    read = tuple(torch.zeros((t, 1, 32), device="cuda") for _ in range(2))
+    return [((out,), lambda: ops.gemm_int8(codes_x, codes_w, sx, sw, out=out)),
+            ((out,), lambda: ops.linear_int8(x, codes_w, sw, out=out)),
+            ((cache, scales), lambda: ops.cache_write(cache, scales, (x[:, None], x[:, None]), slots)),
+            (read, lambda: ops.cache_read(cache, scales, table, offsets, t, out=read))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("mode", ["plain", "no_grad", "inference"])
+def test_written_tensors_have_a_new_version(which, mode):
+    written, call = writes(5)[which]
+    before = [w._version for w in written]
+    with {"no_grad": torch.no_grad, "inference": torch.inference_mode}.get(mode, torch.enable_grad)():
+        call()
+    assert [w._version for w in written] == [v + 1 for v in before]
+
+
+@pytest.mark.gpu
+def test_written_inference_tensors():
+    """They have no version to raise."""
+    with torch.inference_mode():
+        for _, call in writes(5):
+            call()
+
+
+@pytest.mark.gpu
+def test_backward_through_a_tensor_that_was_written():
+    """What autograd saved for a product is no longer what the product read."""
+    (out,), call = writes(5)[0]
+    p = torch.ones((5, 16), device="cuda", requires_grad=True)
+    y = (p * out).sum()
+    call()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
