@@ -2,8 +2,7 @@
 
 One format: a row x is held as int8 codes q and one fp32 scale s with
 s = max|x| / 127 and q the integers nearest to x / s (ties to even), so x is
-s * q to within s / 2. It is what ExactIndex(precision="int8") takes as rows
-and queries, and what every function here makes or reads:
+s * q to within s / 2. It is what every function here makes or reads:
 
   quantize_rows   rows -> codes, scales (activations per token, weights per
                   output channel)
@@ -12,6 +11,13 @@ and queries, and what every function here makes or reads:
   linear_int8     rows x codes: quantize_rows and gemm_int8 in one call
   cache_write     rows quantised into the slots of a paged cache
   cache_read      sequences of pages back into packed rows
+
+ExactIndex(precision="int8") ranks by the integer product of the codes alone. A
+query's scale does not change its order, so quantize_rows makes its queries;
+stored rows have to have one scale for all of them (round(x / s) for s the
+largest magnitude of the whole base over 127). Rows with a scale each are scored
+by gemm_int8 with those scales: without them they are ordered as if all had the
+same largest value.
 
 The reference has no such operators: its scalar quantiser has one affine scale
 per dimension and scores by lookup (src/quant_engine/ScalarQuantizer.cpp:83-128).
