@@ -172,6 +172,8 @@ SIGNATURES = [
     ("elips_b200_quantize_rows", c_int,
      [c_int, c_void_p, c_int, c_size_t, c_size_t, c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
     ("elips_b200_gemm_int8", c_int, [c_int, c_void_p, c_void_p]),
+    ("elips_b200_gemm_int8_form", c_int,
+     [c_int64, c_int64, c_int64, c_int, c_int, POINTER(c_int), POINTER(c_int)]),
     ("elips_b200_cache_write", c_int, [c_int, c_void_p, c_void_p, c_int, c_size_t, c_void_p, c_int, c_void_p]),
     ("elips_b200_cache_read", c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     ("elips_b200_profiler_enable", c_int, [c_int]),

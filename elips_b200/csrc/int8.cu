@@ -797,6 +797,20 @@ int elips_b200_gemm_int8(int device, const elips_b200_gemm* args, void* stream) 
     });
 }
 
+int elips_b200_gemm_int8_form(int64_t m, int64_t n, int64_t k, int out_type, int num_sms, int* rows_out, int* splits_out) {
+    if (rows_out == nullptr || splits_out == nullptr) return ELIPS_B200_INVALID_ARGUMENT;
+    return guarded([&] {
+        eb::check_float_type(out_type);
+        const int64_t most = static_cast<int64_t>(eb::kMaxRows);
+        if (m < 1 || n < 1 || k < 0 || m > most || n > most || k > static_cast<int64_t>(eb::kMaxK) || num_sms < 2)
+            eb::bad("no such product");
+        const eb::GemmForm f = eb::gemm_form(static_cast<uint32_t>(m), static_cast<uint32_t>(n), static_cast<uint32_t>(k),
+                                             out_type == ELIPS_B200_PRECISION_FP32, num_sms);
+        *rows_out = static_cast<int>(f.rows);
+        *splits_out = static_cast<int>(f.splits);
+    });
+}
+
 int elips_b200_cache_write(int device, const elips_b200_cache* cache, const elips_b200_rows* rows, int type, size_t t,
                            const void* slots, int slots_64bit, void* stream) {
     if (cache == nullptr || (t > 0 && rows == nullptr)) return ELIPS_B200_INVALID_ARGUMENT;

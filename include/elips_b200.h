@@ -627,6 +627,13 @@ typedef struct {
  * always give the same bits. */
 ELIPS_B200_API int elips_b200_gemm_int8(int device, const elips_b200_gemm* args, void* stream);
 
+/* The kernel that a product of these sizes takes on a device of num_sms SMs
+ * (needs no device): *rows_out is 1 for the one of a few rows, 0 for the one of
+ * CTA pairs, else the rows of a tile of the third, of which *splits_out CTAs
+ * share k. The results are the same whichever it is. */
+ELIPS_B200_API int elips_b200_gemm_int8_form(int64_t m, int64_t n, int64_t k, int out_type, int num_sms, int* rows_out,
+                                             int* splits_out);
+
 /* A paged cache of quantised rows: codes [parts][pages][page_size][heads][dim]
  * and scales [parts][pages][page_size][heads] with the given strides (the
  * innermost one of codes is 1). One part holds one kind of row (vectors), two
