@@ -445,11 +445,28 @@ struct GemmForm {
     uint32_t rows = 0, splits = 1;
 };
 
-// The dot kernel is for single tokens: its dp4a takes over from the loads at
-// about 2^25 products (device times, bf16 out: 1 x 4096 x 4096 5.3 us and wide
-// 7.0, 4 x 2048 x 2048 3.1 and 4.6, 4 x 4096 x 4096 8.5 and 7.1). Between the
-// others the least time that a simple model gives, in us, from what was
-// measured over sizes from 16 x 1024 x 1024 to 8192^3:
+// The dot kernel is for single tokens. A warp takes four channels whatever k
+// is, so what it spends on each counts where there are many (us on the device,
+// to bf16, dot kernel / wide kernel with its best split):
+//   1 row:  4096 x 4096 4.4 / 6.7, 8192 x 8192 13.0 / 14.4, 40,000 x 4096 28.4 /
+//           29.7, 10,000 x 768 2.9 / 3.8, 50,000 x 1024 10.5 / 11.1, 60,000 x
+//           1024 12.3 / 12.2, 100,000 x 768 16.3 / 14.6, 100,000 x 128 9.1 / 5.5,
+//           1,000,000 x 128 79 / 33
+//   2 rows: 4096 x 4096 5.3 / 6.8, 8192 x 4096 8.7 / 9.3, 10,000 x 768 3.8 / 3.7
+//           (rows of floats 3.8 / 5.3), 16,000 x 4096 14.0 / 12.9, 100,000 x 768
+//           21.8 / 14.8, 1,000,000 x 128 108 / 34
+// From three rows on its dp4a takes over from the loads at about 2^25 products:
+// 4 x 2048 x 2048 2.7 / 4.6, 8 x 1024 x 1024 2.7 / 3.8, 4 x 4096 x 4096 7.2 / 6.8,
+// 8 x 4096 x 4096 8.5 / 6.9, 4 x 10,000 x 768 4.3 / 3.7.
+bool dot_form(uint32_t m, uint32_t n, uint32_t k) {
+    if (k == 0 || m > 8) return false;
+    if (m == 1 && n <= uint64_t{52} * k) return true;
+    if (m <= 2) return n <= 12288;
+    return n <= 8192 && static_cast<uint64_t>(m) * n * k <= (1u << 25);
+}
+
+// Between the others the least time that a simple model gives, in us, from what
+// was measured over sizes from 16 x 1024 x 1024 to 8192^3:
 //  * wide: 4 for the launch and its ends; a CTA loads 127 KB/us, four fifths
 //    of that when all SMs do; a cluster's summing costs 0.35 and 0.0145 a row.
 //    With more tiles than SMs, each takes 0.2 and its loads or, if longer, its
@@ -457,11 +474,11 @@ struct GemmForm {
 //  * pair: 4.5 for the launch and its ends, then waves of tiles at 0.36 per
 //    128 of k (1670 T products/s, the tensor cores' pace at this power) + 1.2,
 //    2.4 at least, 0.8 more to fp32; 0.7 of that for a last wave of half tiles.
-// E.g. 512 x 4096 x 4096: wide of 128 rows 12.6 us, pair 16.3; 1024 x 4096 x
-// 4096: 19.1 and 16.9; 64 x 100,000 x 384 to fp32: 14.5 (64 rows) and 23.2;
-// 10,000 x 1536 x 768: 21.5 and 16.9.
+// Measured on both sides (wide of 128 rows or as named / pair): 512 x 4096 x 4096
+// 11.8 / 12.5, 1024 x 4096 x 4096 18.6 / 16.2, 64 x 100,000 x 384 to fp32 14.0 (64
+// rows) / 20.7, 10,000 x 1536 x 768 21.8 / 14.7, to fp32 22.4 / 18.4.
 GemmForm gemm_form(uint32_t m, uint32_t n, uint32_t k, bool fp32, int num_sms) {
-    if (k > 0 && (m <= 2 || (m <= 8 && static_cast<uint64_t>(m) * n * k <= (1u << 25)))) return {1, 1};
+    if (dot_form(m, n, k)) return {1, 1};
     const uint32_t kb = cdiv(k, kGemmStageK);
     const double sms = num_sms;
     GemmForm best{0, 1};

@@ -95,3 +95,27 @@ def test_forms(want, size, dtype, bias, first):
                                              for d in ([FLOATS[0], FLOATS[1 + i % 2]])])
 def test_three_tiles_a_cta(want, size, dtype):
     run(want, size, dtype, torch.float16, 16)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_one_and_two_rows_against_many_channels(dtype):
+    """The kernel of a few rows spends as much on four channels of 64 codes as of 512, so many narrow ones go to the
+    tensor cores; single tokens through a layer do not."""
+    for size in ((1, 10000, 768), (1, 4096, 4096), (1, 40000, 4096), (2, 4096, 4096), (2, 10000, 768), (4, 2048, 2048)):
+        assert form(*size, dtype, 148) == (1, 1), size
+    for size in ((1, 1000000, 128), (1, 100000, 128), (1, 200000, 384), (2, 100000, 768), (4, 100000, 64), (4, 4096, 4096)):
+        assert form(*size, dtype, 148)[0] == 16, size
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(1, 200000, 64), (2, 50000, 100), (1, 60001, 384), (4, 100000, 70), (8, 9000, 64)])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_few_rows_against_many_channels(size, dtype):
+    from elips_b200 import int8
+    m, n, k = size
+    a, b, sa, sb, bv = gemm_case(m, n, k, dtype, torch.bfloat16)
+    out = int8.gemm_int8(a, b, sa, sb, bv, out_dtype=dtype)
+    assert_product(out, a, b, sa, sb, bv, dtype)
+    x = torch.randn((m, k), generator=torch.Generator(device="cuda").manual_seed(m), device="cuda")
+    codes, scales = int8.quantize_rows(x)
+    assert torch.equal(int8.linear_int8(x, b, sb, bv, out_dtype=dtype), int8.gemm_int8(codes, b, scales, sb, bv, out_dtype=dtype))
