@@ -1,6 +1,7 @@
 // The int8 matrix product with a scale per row and channel,
 //   out[i][j] = (sum_l a[i][l] b[j][l]) sa[i] sb[j] + bias[j],
-// in three forms; the host picks one by the number of rows (int8.cu).
+// in three forms; the host picks one by sizes and a model of their times (dot_form
+// and gemm_form in int8.cu).
 //
 //  * gemm_int8_dot_kernel: a few rows (the codes of single tokens). The
 //    weight is read once, 16 bytes a lane, and multiplied with dp4a.
@@ -430,7 +431,7 @@ static __global__ void __launch_bounds__(kWideThreads)
 // ------------------------------------------------------------- pair kernel
 
 constexpr uint32_t kPairM = 256, kPairN = 256;
-constexpr uint32_t kPairStages = 5;  // four lose 5 % on 8192^3, six gain nothing
+constexpr uint32_t kPairStages = 5;  // four lose 5 % on 8192^3, six do not fit
 constexpr uint32_t kPairEpilogueWarps = 8;
 constexpr int kPairThreads = 32 * (2 + kPairEpilogueWarps);
 constexpr uint32_t kPairStageBytes = (kPairM / 2 + kPairN / 2) * kGemmStageK;

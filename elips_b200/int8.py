@@ -208,7 +208,9 @@ def _product(x, x_kind, x_scales, b, b_scales, bias, dtype, out, stream):
 
 def gemm_int8(a, b, a_scales, b_scales, bias=None, out_dtype=torch.bfloat16, out=None, stream=None):
     """out[i, j] = (sum_l a[i, l] b[j, l]) * a_scales[i] * b_scales[j] + bias[j],
-    the sum exact in int32 (so the width is below 2^17), rounded once.
+    the sum exact in int32 (so the width is below 2^17). The sum's conversion to
+    fp32, its product with a_scales, the fused b_scales and bias, and out's type
+    round once each, in this order.
 
     a [m, k] and b [n, k] are int8 with contiguous rows, as quantize_rows gives
     them: a activations and b a layer's weight with a scale per channel, or a

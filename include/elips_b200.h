@@ -622,8 +622,9 @@ typedef struct {
 } elips_b200_gemm;
 
 /* out[i][j] = (sum_l a[i][l] * b[j][l]) * a_scales[i] * b_scales[j] + bias[j],
- * the sum exact in int32 (k < 2^17), the rest in fp32 in this order, rounded
- * once to out_type. The order of the sum does not matter, so the same inputs
+ * the sum exact in int32 (k < 2^17), the rest in fp32 in this order (sum to
+ * fp32, a_scales, b_scales and bias fused: one rounding each) and then rounded
+ * to out_type. The order of the sum does not matter, so the same inputs
  * always give the same bits. */
 ELIPS_B200_API int elips_b200_gemm_int8(int device, const elips_b200_gemm* args, void* stream);
 
