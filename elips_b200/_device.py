@@ -7,13 +7,13 @@ def as_stream(stream, device: int):
     work on `device`. The default stream's handle is 0, or 1 for the legacy one that it is; ExternalStream takes 0 for
     none given, and would make a new stream."""
     import torch
-    handle = stream if isinstance(stream, int) else stream.cuda_stream
-    if handle in (0, 1):
-        return torch.cuda.default_stream(device)
     if isinstance(stream, torch.cuda.Stream):
         if stream.device_index != device:
             raise ValueError(f"the stream is on cuda:{stream.device_index}, the tensors on cuda:{device}")
         return stream
+    handle = stream if isinstance(stream, int) else stream.cuda_stream
+    if handle in (0, 1):
+        return torch.cuda.default_stream(device)
     return torch.cuda.ExternalStream(handle, device=device)
 
 

@@ -1,5 +1,5 @@
-"""The example of INTEGRATION.md's section on the 8-bit row operators, run as it stands: what it calls neighbours are
-the rows' neighbours, also where the rows' sizes differ widely."""
+"""The documented example of the 8-bit row operators, run as it stands: what it calls neighbours are the rows'
+neighbours, also where the rows' sizes differ widely."""
 import re
 from pathlib import Path
 

@@ -15,6 +15,18 @@ def test_default_stream_is_no_new_one(monkeypatch):
         assert as_stream(type("Foreign", (), {"cuda_stream": stream})(), 3) == ("default", 3)
 
 
+@pytest.mark.parametrize("handle", [0, 1 << 40])
+def test_torch_streams(monkeypatch, handle):
+    """Used as they are on their own device, the default one too, and on no other."""
+    class Stream:
+        device_index, cuda_stream = 2, handle
+    monkeypatch.setattr(torch.cuda, "Stream", Stream)
+    stream = Stream()
+    assert as_stream(stream, 2) is stream
+    with pytest.raises(ValueError, match="cuda:2"):
+        as_stream(stream, 0)
+
+
 def test_foreign_handles(monkeypatch):
     monkeypatch.setattr(torch.cuda, "ExternalStream", lambda handle, device: (handle, device))
     assert as_stream(1 << 40, 2) == (1 << 40, 2)
