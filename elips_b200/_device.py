@@ -17,8 +17,8 @@ def as_stream(stream, device: int):
     return torch.cuda.ExternalStream(handle, device=device)
 
 
-def device_rows(rows, dimension: int, dtype, what: str, stream=None):
-    """`rows`, checked, as a CUDA tensor [n, dimension] of `dtype` whose rows follow one another: the entry points take
+def device_rows(rows, dimension: int, dtype, device: int, what: str, stream=None):
+    """`rows`, checked, as a tensor [n, dimension] of `dtype` on cuda:`device` whose rows follow one another: the entry points take
     an address and read n * dimension values from it. A view of other strides (rows of wider ones, such as the codes
     that quantize_rows gives; a broadcast row; a transpose) is copied, on `stream` where one is given."""
     import torch
@@ -28,8 +28,8 @@ def device_rows(rows, dimension: int, dtype, what: str, stream=None):
         raise DimensionMismatch(f"{what} dimension does not match index")
     if rows.dtype is not dtype:
         raise ValueError(f"{what} rows must be {dtype}, not {rows.dtype}")
-    if not rows.is_cuda:
-        raise ValueError(f"{what} rows must be on a CUDA device, not on {rows.device}")
+    if not rows.is_cuda or rows.get_device() != device:
+        raise ValueError(f"{what} rows must be on cuda:{device}, the index's CUDA device, not on {rows.device}")
     if rows.is_contiguous():
         return rows
     if stream is None:

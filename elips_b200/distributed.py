@@ -214,7 +214,7 @@ class ShardedExactIndex:
         import torch
         from . import _capi as capi
         from ._device import device_rows
-        queries = device_rows(queries, self.local.dimension, self.local._torch_dtype(), "query")
+        queries = device_rows(queries, self.local.dimension, self.local._torch_dtype(), self.device, "query")
         nq = queries.shape[0]
         self.peer.ensure(nq, k)
         my_slot, bounds, blocks = self.peer.slots(nq)

@@ -77,7 +77,7 @@ class ExactIndex:
     def add_device(self, rows, stream=None) -> None:
         """Appends rows held in a CUDA tensor [n, dimension] (float32, int8 for int8)."""
         import torch
-        rows = device_rows(rows, self.dimension, self._torch_dtype(), "vector", stream)
+        rows = device_rows(rows, self.dimension, self._torch_dtype(), self.device, "vector", stream)
         s = stream if stream is not None else torch.cuda.current_stream(rows.device).cuda_stream
         capi.check(capi.LIB.elips_b200_exact_add_device(self._h, rows.data_ptr(), rows.shape[0], s),
                    "elips_b200_exact_add_device")
@@ -159,7 +159,7 @@ class ExactIndex:
         that do not follow one another are copied). Asynchronous on `stream` (default: torch's
         current stream). Returns (dist, rows) CUDA tensors."""
         import torch
-        queries = device_rows(queries, self.dimension, self._torch_dtype(), "query", stream)
+        queries = device_rows(queries, self.dimension, self._torch_dtype(), self.device, "query", stream)
         nq = queries.shape[0]
         if out_dist is None:
             out_dist = torch.empty((nq, k), dtype=torch.float32, device=queries.device)
@@ -174,7 +174,7 @@ class ExactIndex:
     def search_candidates_device(self, queries, k: int, row_offset: int, out_cand, mask=None, stream=None):
         """Shard-level search: writes [nq, k, 2] uint32-as-int32 candidate pairs to out_cand."""
         import torch
-        queries = device_rows(queries, self.dimension, self._torch_dtype(), "query", stream)
+        queries = device_rows(queries, self.dimension, self._torch_dtype(), self.device, "query", stream)
         s = stream if stream is not None else torch.cuda.current_stream(queries.device).cuda_stream
         capi.check(capi.LIB.elips_b200_exact_search_candidates_device(
             self._h, queries.data_ptr(), queries.shape[0], k,
@@ -188,7 +188,7 @@ class ExactIndex:
         an int32 CUDA tensor [nq] of ordered keys, all ones = none) are shared
         with the other shards searching the same queries."""
         import torch
-        queries = device_rows(queries, self.dimension, self._torch_dtype(), "query", stream)
+        queries = device_rows(queries, self.dimension, self._torch_dtype(), self.device, "query", stream)
         s = stream if stream is not None else torch.cuda.current_stream(queries.device).cuda_stream
         capi.check(capi.LIB.elips_b200_exact_search_candidates_shared_device(
             self._h, queries.data_ptr(), queries.shape[0], k, mask.data_ptr() if mask is not None else None,

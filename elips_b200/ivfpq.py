@@ -52,10 +52,10 @@ class IvfPqIndex:
     def add_device(self, vectors, assignments, codes=None, stream=None) -> None:
         """CUDA tensors: vectors [n, d] float32, assignments [n] int32 (list ids)."""
         import torch
-        vectors = device_rows(vectors, self.dimension, torch.float32, "vector", stream)
+        vectors = device_rows(vectors, self.dimension, torch.float32, self.device, "vector", stream)
         assignments = assignments.contiguous()
         if codes is not None:
-            codes = device_rows(codes, self.pq_dim, torch.uint8, "code", stream)
+            codes = device_rows(codes, self.pq_dim, torch.uint8, self.device, "code", stream)
         s = stream if stream is not None else torch.cuda.current_stream(vectors.device).cuda_stream
         capi.check(capi.LIB.elips_b200_ivfpq_add_device(self._h, vectors.data_ptr(), assignments.data_ptr(),
                                                         codes.data_ptr() if codes is not None else None,
@@ -108,7 +108,7 @@ class IvfPqIndex:
     def probe_device(self, queries, stream=None):
         """The nprobe nearest lists of each query: [nq, nprobe] int32, ascending."""
         import torch
-        queries = device_rows(queries, self.dimension, torch.float32, "query", stream)
+        queries = device_rows(queries, self.dimension, torch.float32, self.device, "query", stream)
         nq = queries.shape[0]
         nprobe = min(self.nprobe, self.n_lists)
         out = torch.empty((nq, nprobe), dtype=torch.int32, device=queries.device)
@@ -124,7 +124,7 @@ class IvfPqIndex:
         admission bounds, possibly a peer GPU's, shared by the shards of one
         list-sharded index searching this batch) replaces the search's own."""
         import torch
-        queries = device_rows(queries, self.dimension, torch.float32, "query", stream)
+        queries = device_rows(queries, self.dimension, torch.float32, self.device, "query", stream)
         nq = queries.shape[0]
         if out is None:
             out = torch.empty((nq, 4 * k, 2), dtype=torch.int32, device=queries.device)
@@ -149,7 +149,7 @@ class IvfPqIndex:
     def rerank_device(self, queries, k: int, cand, out_dist=None, out_rows=None, stream=None):
         """The exact stage over cand [nq, 4k, 2] (slot -1 = none): (dist, slot) [nq, k]."""
         import torch
-        queries = device_rows(queries, self.dimension, torch.float32, "query", stream)
+        queries = device_rows(queries, self.dimension, torch.float32, self.device, "query", stream)
         nq = queries.shape[0]
         if out_dist is None:
             out_dist = torch.empty((nq, k), dtype=torch.float32, device=queries.device)
@@ -184,7 +184,7 @@ class IvfPqIndex:
 
     def search_device(self, queries, k: int, out_dist=None, out_rows=None, stream=None):
         import torch
-        queries = device_rows(queries, self.dimension, torch.float32, "query", stream)
+        queries = device_rows(queries, self.dimension, torch.float32, self.device, "query", stream)
         nq = queries.shape[0]
         if out_dist is None:
             out_dist = torch.empty((nq, k), dtype=torch.float32, device=queries.device)
@@ -233,7 +233,7 @@ class IvfFlatIndex:
     def add_device(self, vectors, assignments, stream=None) -> None:
         """CUDA tensors: vectors [n, d] float32, assignments [n] int32 (list ids)."""
         import torch
-        vectors = device_rows(vectors, self.dimension, torch.float32, "vector", stream)
+        vectors = device_rows(vectors, self.dimension, torch.float32, self.device, "vector", stream)
         assignments = assignments.contiguous()
         s = stream if stream is not None else torch.cuda.current_stream(vectors.device).cuda_stream
         capi.check(capi.LIB.elips_b200_ivfflat_add_device(self._h, vectors.data_ptr(), assignments.data_ptr(),
@@ -273,7 +273,7 @@ class IvfFlatIndex:
 
     def search_device(self, queries, k: int, out_dist=None, out_rows=None, stream=None):
         import torch
-        queries = device_rows(queries, self.dimension, torch.float32, "query", stream)
+        queries = device_rows(queries, self.dimension, torch.float32, self.device, "query", stream)
         nq = queries.shape[0]
         if out_dist is None:
             out_dist = torch.empty((nq, k), dtype=torch.float32, device=queries.device)

@@ -90,7 +90,7 @@ class QuantizedIndex:
 
     def search_device(self, queries, k: int, stream=None):
         import torch
-        queries = device_rows(queries, self.dimension, torch.float32, "query", stream)
+        queries = device_rows(queries, self.dimension, torch.float32, self.device, "query", stream)
         nq = queries.shape[0]
         d = torch.empty((nq, k), dtype=torch.float32, device=queries.device)
         r = torch.empty((nq, k), dtype=torch.int64, device=queries.device)

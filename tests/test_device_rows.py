@@ -13,7 +13,7 @@ from elips_b200.quant import QuantizedIndex
 def bare(kind, **attributes):
     """An index without its device half: the checks come before it is touched."""
     ix = kind.__new__(kind)
-    ix.__dict__.update(dimension=8, _h=None, **attributes)
+    ix.__dict__.update(dimension=8, device=0, _h=None, **attributes)
     return ix
 
 
@@ -50,6 +50,17 @@ def test_int8_index_takes_codes():
         bare(ExactIndex, precision="int8").search_device(torch.zeros((4, 8)), 1)
     with pytest.raises(ValueError, match="CUDA"):
         bare(ExactIndex, precision="int8").search_device(torch.zeros((4, 8), dtype=torch.int8), 1)
+
+
+def test_rows_on_another_device():
+    """A tensor of cuda:1 for an index on cuda:0 (a stand-in: this needs no GPU)."""
+    class Elsewhere:
+        shape, dtype, is_cuda, device = (4, 8), torch.float32, True, "cuda:1"
+        dim, get_device = (lambda self: 2), (lambda self: 1)
+    with pytest.raises(ValueError, match="cuda:0"):
+        bare(ExactIndex, precision="fp32").search_device(Elsewhere(), 1)
+    with pytest.raises(ValueError, match="cuda:0"):
+        bare(IvfFlatIndex).search_device(Elsewhere(), 1)
 
 
 def views(x):
